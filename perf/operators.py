@@ -279,7 +279,8 @@ def prepare(case, seed):
                                            max_rows=max(rows), max_len=max(lens), cu_groups=s["cu_groups"].data_ptr(),
                                            shared=s["shared"].data_ptr(), n_groups=c["groups"],
                                            max_group_rows=max(sum(rows[i:i + c["hyps"]]) for i in range(0, len(rows), c["hyps"])),
-                                           max_shared=max(shared) // pg * pg)
+                                           max_shared=max(shared) // pg * pg,
+                                           max_own=max(n - shared[i // c["hyps"]] // pg * pg for i, n in enumerate(lens)))
             s["attn_ws"] = torch.empty(s["cache"].attention_workspace_bytes(s["batch"], c["heads"]), dtype=torch.uint8, device=dev)
     return s
 
