@@ -170,6 +170,129 @@ int q3asr_op_gemm_q4(q3asr_model* m, const uint16_t* a, const uint32_t* wq, cons
 int q3asr_op_attention(q3asr_model* m, const uint16_t* q, const uint16_t* k, const uint16_t* v, const int32_t* cu_seqlens,
                        int n_seq, int heads, int group, int head_dim, int causal, uint16_t* out);
 
+/* ---- Serving operators on device buffers: decoding several hypotheses of a clip ----
+ * The reference decodes one greedy hypothesis per clip (Qwen3ASR.swift:562-632) over a contiguous cache
+ * (QuantizedTextDecoder.swift:203-209); these operators have no counterpart there.  A host that keeps several
+ * hypotheses, languages or continuations of one clip shares the pages of the clip's prompt between them, reads the
+ * prompt once per step for all of them, and may run the projections on 8-bit weights.
+ *
+ * All pointers are device memory of the model's GPU unless marked (host); nothing is allocated, and nothing is copied
+ * from or to the host except where said.  The model only names the GPU and the default stream: it needs no weights.
+ * stream: a hipStream_t to enqueue on (the call then returns without waiting; it may be under graph capture), or NULL
+ * for the model's own stream (the call then waits).  Workspaces belong to the caller, who asks for their size first;
+ * calls that may run at the same time, and graphs that may be replayed at the same time, need one each.  A workspace
+ * holds nothing from one call to the next and must be aligned to 16 bytes. */
+
+/* -- 8-bit integer products --
+ * Rows are rounded to whole numbers with one scale per row: scale = max |x| / 127 (fp32), q = x / scale rounded to the
+ * nearest whole number, ties to even, decided without a rounding of the quotient.  A row of zeros has scale 0; a row that
+ * holds an infinity or a NaN has scale NaN and q = 0, so whatever is computed from it is NaN.  Weights take one such scale
+ * per output channel (quantise the [N][K] matrix by rows). */
+
+/* x: [rows][cols] Q3ASR_F32 or Q3ASR_BF16, rows ldx values apart (any stride >= cols, any alignment of the type);
+ * q: [rows][ldq] bytes, ldq a multiple of 16 and >= cols rounded up to 16, aligned to 16: columns from cols to the next
+ * multiple of 16 are set to zero.  scales: [rows]. */
+int q3asr_i8_quantize(q3asr_model* m, const void* x, int dtype, int64_t ldx, int rows, int cols, int8_t* q, int64_t ldq,
+                      float* scales, void* stream);
+/* out[M][N] = (sum_k a[m][k] w[n][k]) * a_scales[m] * w_scales[n] + bias[n], the sum in 32-bit whole numbers, out Q3ASR_F32
+ * or Q3ASR_BF16 (rounded once) in rows ldo values apart.  a, w: rows lda / ldw bytes apart, both multiples of 16 and
+ * aligned to 16; K a multiple of 16, at most 131056.  bias: [N] fp32 or NULL. */
+int q3asr_i8_matmul(q3asr_model* m, const int8_t* a, int64_t lda, const float* a_scales, const int8_t* w, int64_t ldw,
+                    const float* w_scales, const float* bias, int M, int N, int K, void* out, int out_dtype, int64_t ldo,
+                    void* workspace, int64_t workspace_bytes, void* stream);
+/* The two together: activations x as in q3asr_i8_quantize, weights as in q3asr_i8_matmul but any K (at most 131056): a
+ * weight row then has K rounded up to 16 readable bytes, of which those from K on may hold anything. */
+int q3asr_i8_linear(q3asr_model* m, const void* x, int x_dtype, int64_t ldx, const int8_t* w, int64_t ldw, const float* w_scales,
+                    const float* bias, int M, int N, int K, void* out, int out_dtype, int64_t ldo, void* workspace,
+                    int64_t workspace_bytes, void* stream);
+/* Bytes of workspace that q3asr_i8_linear and q3asr_i8_matmul need for these sizes (-1: sizes out of range). */
+int64_t q3asr_i8_workspace(q3asr_model* m, int M, int N, int K);
+
+/* -- A KV cache in pages --
+ * A page holds page_tokens tokens of every layer and KV head.  A sequence s of lens[s] tokens owns the pages
+ * table[s][0 .. ceil(lens[s] / page_tokens)); its other table entries are -1.  refs[p] counts the table entries that name
+ * page p; a page with refs 0 is free.  All of it lives on the device and is changed there, in stream order, by the calls
+ * below; several sequences may share a page, and a shared page is never written except through q3asr_pages_reserve's copy. */
+typedef struct q3asr_kv_pages {
+    uint16_t* k;               /* bf16 [layers][pages][kv_heads][page_tokens][head_dim], aligned to 16 bytes */
+    uint16_t* v;
+    int32_t* table;            /* [max_seqs][max_seq_pages] */
+    int32_t* lens;             /* [max_seqs] */
+    int32_t* refs;             /* [pages] */
+    int32_t* status;           /* [4], see q3asr_pages_status */
+    int layers, pages, kv_heads;
+    int head_dim;              /* 64 or 128 */
+    int page_tokens;           /* a power of two from 16 to 256 */
+    int max_seqs, max_seq_pages;
+    void* workspace;           /* q3asr_pages_workspace bytes (not needed by reset, write and attention) */
+    int64_t workspace_bytes;
+} q3asr_kv_pages;
+
+enum {
+    Q3ASR_PAGES_OK = 0,
+    Q3ASR_PAGES_BAD_INDEX = 1,   /* a sequence or page number out of range, a negative token count */
+    Q3ASR_PAGES_DUPLICATE = 2,   /* a sequence named twice */
+    Q3ASR_PAGES_NO_PAGES = 3,    /* not enough free pages */
+    Q3ASR_PAGES_TOO_LONG = 4,    /* a sequence would need more than max_seq_pages pages */
+    Q3ASR_PAGES_BAD_BATCH = 5    /* a batch that breaks the bounds it was given with (q3asr_attn_batch) */
+};
+/* Numbers in device arrays cannot be refused by the host, so every call checks them on the device.  fork, free, reserve and
+ * compact do all of their work or, where an entry is wrong, none of it; write leaves out what is wrong, and the results of an
+ * attention that reports an error are not to be used.  The first
+ * such error since the last reset of the status is kept: status[0] = code, [1] = number of the (first) wrong entry in the list,
+ * [2] = pages short of (NO_PAGES), and [3] = pages in use after the last compact.  Calls on the model's own stream (stream
+ * NULL) return the error at once and reset the status; after calls on another stream the host asks here: waits for the stream, copies the status to out
+ * (host, 4 numbers) and, where clear is non-zero, sets it to zeros.  Not under graph capture. */
+int q3asr_pages_status(q3asr_model* m, const q3asr_kv_pages* c, int32_t* out, int clear, void* stream);
+int64_t q3asr_pages_workspace(const q3asr_kv_pages* c);
+/* No sequences, all pages free, status zero.  The pages' contents stay as they are. */
+int q3asr_pages_reset(q3asr_model* m, const q3asr_kv_pages* c, void* stream);
+/* Sequence dst[i] becomes sequence src[i] as it was before the call (-1: it becomes empty), for all i at once: what dst[i] held
+ * is given up, the pages of src[i] are shared.  dst holds no sequence twice; dst and src may overlap in any way (a beam search's
+ * reordering is dst = 0 .. n-1, src = parents). */
+int q3asr_pages_fork(q3asr_model* m, const q3asr_kv_pages* c, const int32_t* dst, const int32_t* src, int n, void* stream);
+/* fork with src = -1 throughout. */
+int q3asr_pages_free(q3asr_model* m, const q3asr_kv_pages* c, const int32_t* seqs, int n, void* stream);
+/* Room for tokens[i] >= 0 more tokens in seqs[i], which lens then counts.  A last page that is partly filled and that other
+ * sequences hold too is copied first (its filled tokens, all layers); where all of its holders are in the list with tokens to
+ * add, the first of them keeps it.  Free pages are taken from the lowest number on, in the order of the list and, within a
+ * sequence, the copy first.  The new tokens' contents are what the pages held. */
+int q3asr_pages_reserve(q3asr_model* m, const q3asr_kv_pages* c, const int32_t* seqs, const int32_t* tokens, int n, void* stream);
+/* Moves pages so that those in use are the first ones of the pool: the lowest page behind them goes to their lowest gap, and so on. */
+int q3asr_pages_compact(q3asr_model* m, const q3asr_kv_pages* c, void* stream);
+
+/* The rows of a step: sequence seqs[i] has rows cu_rows[i] .. cu_rows[i + 1) of it, which are its last tokens (lens counts them
+ * already: q3asr_pages_reserve).  A sequence stands in the list once.  Optionally, consecutive sequences of the list form groups
+ * (group g: entries cu_groups[g] .. cu_groups[g + 1)) whose first shared[g] tokens lie in the same pages; those are then read
+ * once for the group.  shared[g] counts at most the tokens before the step's rows and is rounded down to whole pages.  The host
+ * numbers bound what the arrays hold; smaller bounds make smaller grids. */
+typedef struct q3asr_attn_batch {
+    const int32_t* seqs;       /* [n] */
+    const int32_t* cu_rows;    /* [n + 1], from 0 to rows */
+    const int32_t* cu_groups;  /* [n_groups + 1], from 0 to n, or NULL */
+    const int32_t* shared;     /* [n_groups] or NULL */
+    int n, rows, n_groups;
+    int max_rows;              /* rows of one sequence */
+    int max_group_rows;        /* rows of one group */
+    int max_len;               /* tokens of one sequence */
+    int max_shared;            /* tokens shared by one group */
+    int max_own;               /* tokens of one sequence behind its group's whole shared pages (without groups: max_len) */
+} q3asr_attn_batch;
+/* Puts the step's keys and values (bf16 [rows][kv_heads * head_dim], rows k_ld / v_ld values apart, multiples of 8, aligned to
+ * 16 bytes) into the pages of a layer.  A sequence that stands in the list twice keeps its first rows, and a page that other
+ * sequences hold too is not written (both are errors). */
+int q3asr_pages_write(q3asr_model* m, const q3asr_kv_pages* c, int layer, const uint16_t* k_rows, int64_t k_ld,
+                      const uint16_t* v_rows, int64_t v_ld, const q3asr_attn_batch* b, void* stream);
+/* out[r][h] = sum_j p_j v_j, p = softmax_j(scale * q[r][h] . k_j) over the tokens j of row r's sequence up to its own; query heads
+ * h * kv_heads / heads share a KV head.  q, out: bf16 [rows][heads * head_dim], rows q_ld / o_ld values apart (multiples of 8,
+ * aligned to 16 bytes); lse: fp32 [rows][heads], the logarithm of the sum of exp(scale * q . k_j), or NULL.  A row without keys
+ * gives zeros and lse -inf.  Tokens behind a sequence's last are not read into the result whatever they hold; the step's own
+ * rows must be finite. */
+int q3asr_paged_attention(q3asr_model* m, const q3asr_kv_pages* c, int layer, const uint16_t* q, int64_t q_ld, int heads,
+                          float scale, const q3asr_attn_batch* b, uint16_t* out, int64_t o_ld, float* lse, void* workspace,
+                          int64_t workspace_bytes, void* stream);
+int64_t q3asr_paged_attention_workspace(q3asr_model* m, const q3asr_kv_pages* c, const q3asr_attn_batch* b, int heads);
+
 #ifdef __cplusplus
 }
 #endif

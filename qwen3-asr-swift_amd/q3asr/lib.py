@@ -27,6 +27,27 @@ class Q3Request(ctypes.Structure):
     ]
 
 
+class Q3Pages(ctypes.Structure):
+    """Image of ``q3asr_kv_pages``."""
+    _fields_ = [
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("table", ctypes.c_void_p), ("lens", ctypes.c_void_p),
+        ("refs", ctypes.c_void_p), ("status", ctypes.c_void_p),
+        ("layers", ctypes.c_int), ("pages", ctypes.c_int), ("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int),
+        ("page_tokens", ctypes.c_int), ("max_seqs", ctypes.c_int), ("max_seq_pages", ctypes.c_int),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64),
+    ]
+
+
+class AttentionBatch(ctypes.Structure):
+    """Image of ``q3asr_attn_batch``: the rows of a step (device addresses as whole numbers) and what bounds them."""
+    _fields_ = [
+        ("seqs", ctypes.c_void_p), ("cu_rows", ctypes.c_void_p), ("cu_groups", ctypes.c_void_p), ("shared", ctypes.c_void_p),
+        ("n", ctypes.c_int), ("rows", ctypes.c_int), ("n_groups", ctypes.c_int),
+        ("max_rows", ctypes.c_int), ("max_group_rows", ctypes.c_int), ("max_len", ctypes.c_int), ("max_shared", ctypes.c_int),
+        ("max_own", ctypes.c_int),
+    ]
+
+
 class Q3Result(ctypes.Structure):
     _fields_ = [
         ("tokens", ctypes.POINTER(ctypes.c_int32)), ("n_tokens", ctypes.POINTER(ctypes.c_int32)),
@@ -43,6 +64,9 @@ EXPORTS = [
     "q3asr_mel", "q3asr_encode", "q3asr_output_length", "q3asr_transcribe_tokens", "q3asr_op_gemm", "q3asr_op_gemm_q4",
     "q3asr_op_attention", "q3asr_profile_start", "q3asr_profile_stop", "q3asr_op_gemm_time", "q3asr_op_greedy_rules",
     "q3asr_op_read_bandwidth", "q3asr_op_mfma_f32_rate", "q3asr_workspace_bytes", "q3asr_mel_noalloc", "q3asr_decode_attention_cus",
+    "q3asr_i8_quantize", "q3asr_i8_matmul", "q3asr_i8_linear", "q3asr_i8_workspace", "q3asr_pages_status", "q3asr_pages_workspace",
+    "q3asr_pages_reset", "q3asr_pages_fork", "q3asr_pages_free", "q3asr_pages_reserve", "q3asr_pages_compact", "q3asr_pages_write",
+    "q3asr_paged_attention", "q3asr_paged_attention_workspace",
 ]
 
 
@@ -77,6 +101,28 @@ def load():
     lib.q3asr_op_greedy_rules.argtypes = [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p]
     lib.q3asr_op_read_bandwidth.argtypes = [c_void_p, ctypes.c_int64, P(ctypes.c_float)]
     lib.q3asr_op_mfma_f32_rate.argtypes = [c_void_p, c_int, c_int, P(ctypes.c_float)]
+    c_i64 = ctypes.c_int64
+    lib.q3asr_i8_quantize.argtypes = [c_void_p, c_void_p, c_int, c_i64, c_int, c_int, c_void_p, c_i64, c_void_p, c_void_p]
+    lib.q3asr_i8_matmul.argtypes = [c_void_p, c_void_p, c_i64, c_void_p, c_void_p, c_i64, c_void_p, c_void_p, c_int, c_int, c_int,
+                                    c_void_p, c_int, c_i64, c_void_p, c_i64, c_void_p]
+    lib.q3asr_i8_linear.argtypes = [c_void_p, c_void_p, c_int, c_i64, c_void_p, c_i64, c_void_p, c_void_p, c_int, c_int, c_int,
+                                    c_void_p, c_int, c_i64, c_void_p, c_i64, c_void_p]
+    lib.q3asr_i8_workspace.argtypes = [c_void_p, c_int, c_int, c_int]
+    lib.q3asr_i8_workspace.restype = c_i64
+    pages, batch = P(Q3Pages), P(AttentionBatch)
+    lib.q3asr_pages_status.argtypes = [c_void_p, pages, P(ctypes.c_int32), c_int, c_void_p]
+    lib.q3asr_pages_workspace.argtypes = [pages]
+    lib.q3asr_pages_workspace.restype = c_i64
+    lib.q3asr_pages_reset.argtypes = [c_void_p, pages, c_void_p]
+    lib.q3asr_pages_fork.argtypes = [c_void_p, pages, c_void_p, c_void_p, c_int, c_void_p]
+    lib.q3asr_pages_free.argtypes = [c_void_p, pages, c_void_p, c_int, c_void_p]
+    lib.q3asr_pages_reserve.argtypes = [c_void_p, pages, c_void_p, c_void_p, c_int, c_void_p]
+    lib.q3asr_pages_compact.argtypes = [c_void_p, pages, c_void_p]
+    lib.q3asr_pages_write.argtypes = [c_void_p, pages, c_int, c_void_p, c_i64, c_void_p, c_i64, batch, c_void_p]
+    lib.q3asr_paged_attention.argtypes = [c_void_p, pages, c_int, c_void_p, c_i64, c_int, ctypes.c_float, batch, c_void_p, c_i64,
+                                          c_void_p, c_void_p, c_i64, c_void_p]
+    lib.q3asr_paged_attention_workspace.argtypes = [c_void_p, pages, batch, c_int]
+    lib.q3asr_paged_attention_workspace.restype = c_i64
     lib.q3asr_profile_start.argtypes = [c_void_p, c_int]
     lib.q3asr_profile_stop.argtypes = [c_void_p, ctypes.c_char_p, c_int]
     return lib
