@@ -158,8 +158,11 @@ int q3asr_i8_linear(q3asr_model* m, const void* x, int x_dtype, int64_t ldx, con
     p.sa = (const float*)((char*)workspace + round256((int64_t)M * p.lda));
     p.W = w; p.ldw = ldw; p.sw = w_scales; p.bias = bias;
     p.M = M; p.N = N; p.K = K; p.out = out; p.ldo = ldo; p.out_f32 = out_dtype == Q3ASR_F32;
-    launch_i8_quantize({x, x_dtype == Q3ASR_F32, ldx}, M, K, (int8_t*)p.A, p.lda, (float*)p.sa, call.s);
-    launch_i8_matmul(p, (char*)workspace + quantized, workspace_bytes - quantized, call.s);
+    const I8Source src{x, x_dtype == Q3ASR_F32, ldx};
+    if (!launch_i8_linear_few_rows(p, src, call.s)) {
+        launch_i8_quantize(src, M, K, (int8_t*)p.A, p.lda, (float*)p.sa, call.s);
+        launch_i8_matmul(p, (char*)workspace + quantized, workspace_bytes - quantized, call.s);
+    }
     call.done();
     Q3_API_END
 }

@@ -22,6 +22,8 @@ struct I8Params {
 };
 
 void launch_i8_quantize(const I8Source& src, int rows, int cols, int8_t* q, int64_t ldq, float* scales, hipStream_t s);
+// Both steps in one kernel where the rows are few; false: it does not apply.
+bool launch_i8_linear_few_rows(const I8Params& p, const I8Source& src, hipStream_t s);
 // bytes of scratch that launch_i8_matmul wants for split sums
 int64_t i8_matmul_scratch(int M, int N, int K);
 void launch_i8_matmul(I8Params p, void* scratch, int64_t scratch_bytes, hipStream_t s);

@@ -45,40 +45,92 @@ __device__ __forceinline__ float i8_load(const void* row, int k) {
     else return bf16_to_f32(((const bf16_t*)row)[k]);
 }
 
-// Maximum magnitude that turns into NaN where a NaN is among the values (fmaxf would drop it).
-__device__ __forceinline__ float amax_of(float m, float x) {
-    const float a = fabsf(x);
-    return a > m || !(a == a) ? a : m;
-}
-__device__ __forceinline__ float wave_amax(float v) {
+// 8 consecutive values of a row.  `vec`: the row is aligned to 16 bytes; values from `cols` on read as zero.
+template <bool F32>
+__device__ __forceinline__ void i8_load8(const void* row, int k, int cols, bool vec, float* v) {
+    if (vec && k + 8 <= cols) {
+        if constexpr (F32) {
+            const float4 a = *(const float4*)((const float*)row + k), b = *(const float4*)((const float*)row + k + 4);
+            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+            v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        } else {
+            const uint4 a = *(const uint4*)((const bf16_t*)row + k);
+            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const float t = __shfl_xor(v, o, 64);
-        v = t > v || !(t == t) ? t : v;
+            for (int e = 0; e < 4; ++e) {
+                v[2 * e] = __uint_as_float(w[e] << 16);
+                v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+            }
+        }
+        return;
     }
-    return v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = k + e < cols ? i8_load<F32>(row, k + e) : 0.f;
+}
+__device__ __forceinline__ uint2 i8_pack8(const RowScale& rs, const float* v) {
+    uint32_t b[2] = {0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) b[e >> 2] |= (uint32_t)(rs.whole(v[e]) & 255) << (8 * (e & 3));
+    return make_uint2(b[0], b[1]);
+}
+// Magnitudes are compared as the bits of non-negative floats, an order in which a NaN lies above infinity.
+__device__ __forceinline__ uint32_t i8_max8(uint32_t m, const float* v) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(v[e]) & 0x7fffffffu);
+    return m;
+}
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_max_bits(uint32_t v) {
+    return max(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xf, 0xf, false));
+}
+// Maximum over the 64 lanes (all active), the same in every lane.
+__device__ __forceinline__ uint32_t wave_max_bits(uint32_t v) {
+    v = dpp_max_bits<0xB1>(v);    // quad_perm [1,0,3,2]
+    v = dpp_max_bits<0x4E>(v);    // quad_perm [2,3,0,1]
+    v = dpp_max_bits<0x124>(v);   // row_ror:4
+    v = dpp_max_bits<0x128>(v);   // row_ror:8
+    const uint32_t a = __builtin_amdgcn_readlane(v, 0), b = __builtin_amdgcn_readlane(v, 16), c = __builtin_amdgcn_readlane(v, 32),
+                   d = __builtin_amdgcn_readlane(v, 48);
+    return max(max(a, b), max(c, d));
 }
 
-// One wave per row.
-template <bool F32>
+// One wave per row, 8 values per lane and step; rows of up to 512 * HELD values stay in registers between the maximum and the
+// rounding, longer ones are read twice.
+template <bool F32, int HELD>
 __global__ __launch_bounds__(256) void i8_quantize_kernel(const void* x, int64_t ldx, int rows, int cols, int8_t* q, int64_t ldq, float* scales) {
     const int lane = threadIdx.x & 63;
     const int row = blockIdx.x * 4 + (threadIdx.x >> 6);
     if (row >= rows) return;
     const void* src = (const char*)x + (int64_t)row * ldx * (F32 ? 4 : 2);
-    float m = 0.f;
-    for (int k = lane; k < cols; k += 64) m = amax_of(m, i8_load<F32>(src, k));
-    const RowScale rs(wave_amax(m));
-    if (lane == 0) scales[row] = rs.scale;
+    const bool vec = (uintptr_t)src % 16 == 0;
     int8_t* dst = q + (int64_t)row * ldq;
-    for (int k4 = lane; k4 * 4 < ((cols + 15) & ~15); k4 += 64) {
-        uint32_t b = 0;
+    const int k16 = (cols + 15) & ~15;
+    uint32_t m = 0;
+    if constexpr (HELD > 0) {
+        float v[HELD][8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int k = k4 * 4 + e;
-            if (k < cols) b |= (uint32_t)(rs.whole(i8_load<F32>(src, k)) & 255) << (8 * e);
+        for (int i = 0; i < HELD; ++i) i8_load8<F32>(src, (i * 64 + lane) * 8, cols, vec, v[i]);
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) m = i8_max8(m, v[i]);
+        const RowScale rs(__uint_as_float(wave_max_bits(m)));
+        if (lane == 0) scales[row] = rs.scale;
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            const int k = (i * 64 + lane) * 8;
+            if (k < k16) *(uint2*)(dst + k) = i8_pack8(rs, v[i]);
         }
-        *(uint32_t*)(dst + k4 * 4) = b;
+    } else {
+        float v[8];
+        for (int k = lane * 8; k < cols; k += 512) {
+            i8_load8<F32>(src, k, cols, vec, v);
+            m = i8_max8(m, v);
+        }
+        const RowScale rs(__uint_as_float(wave_max_bits(m)));
+        if (lane == 0) scales[row] = rs.scale;
+        for (int k = lane * 8; k < k16; k += 512) {
+            i8_load8<F32>(src, k, cols, vec, v);
+            *(uint2*)(dst + k) = i8_pack8(rs, v);
+        }
     }
 }
 
@@ -257,6 +309,373 @@ __global__ __launch_bounds__(256, 2) void i8_gemm_kernel(I8Params p) {
     }
 }
 
+// ---- many rows: 256 x 256 x 128 tiles ----
+//
+// Matrix-core bound.  The bf16 kernel's scheme (one 512-thread workgroup per CU, 8 waves as 2 x 4, eight phases per two K tiles,
+// each {LDS -> registers, one staging unit's loads, barrier, 16 MFMAs, barrier}, waves 4-7 one barrier behind waves 0-3) carries
+// over byte for byte: a K tile is 128 bytes of a row, which are 64 bf16 or 128 int8 values, and a 16-byte fragment feeds one
+// 16x16x32 bf16 or one 16x16x64 int8 MFMA of the same length.  Twice the work per byte moved, so the phases are the same and
+// the rate doubles.
+constexpr int UNIT = 128 * 128, BUF = 4 * UNIT, LDS256 = 2 * BUF;   // A0 | A1 | W0 | W1, two K tiles
+
+__global__ __launch_bounds__(512, 2) void i8_gemm256_kernel(I8Params p) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int uwave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wr = uwave >> 2, wc = uwave & 3, li = lane & 15, lg = lane >> 4;
+    const int tiles_m = (p.M + 255) >> 8, tiles_n = (p.N + 255) >> 8, total = tiles_m * tiles_n;
+    constexpr int GROUP = 8;
+    const int per_group = GROUP * tiles_n;
+    const int k16 = (p.K + 15) & ~15, nt = (k16 + 127) >> 7;
+
+    // thread t fills 16-byte slots t and 512 + t of every unit: LDS row q * 64 + (t >> 3), slot t & 7, which holds chunk
+    // (t & 7) ^ ((row >> 1) & 7) of the K tile
+    const int srow = tid >> 3, koff = ((tid & 7) ^ ((srow >> 1) & 7)) * 16;
+    constexpr int BUF_RANGE = 0x40000000, BUF_OOB = 0x7f000000;
+    int m0 = 0, n0 = 0;
+    int a_off[2][2], w_off[2][2];
+    __amdgpu_buffer_rsrc_t a_rsrc, w_rsrc;
+    auto setup = [&](int b) {
+        const int q8 = total >> 3, r8 = total & 7, x = b & 7;
+        const int L = (x < r8 ? x * (q8 + 1) : r8 * (q8 + 1) + (x - r8) * q8) + (b >> 3);
+        const int first_m = L / per_group * GROUP, gsz = min(GROUP, tiles_m - first_m);
+        m0 = (first_m + (L % per_group) % gsz) << 8;
+        n0 = ((L % per_group) / gsz) << 8;
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                a_off[q][u] = (min(m0 + q * 128 + u * 64 + srow, p.M - 1) - m0) * (int)p.lda + koff;
+                const int rho = q * 64 + srow, i = rho & 15, j = (rho >> 4) & 1, c = rho >> 5;
+                w_off[q][u] = (min(n0 + c * 64 + (i >> 2) * 16 + u * 8 + j * 4 + (i & 3), p.N - 1) - n0) * (int)p.ldw + koff;
+            }
+        a_rsrc = uniform_buffer(p.A + (int64_t)m0 * p.lda, BUF_RANGE);
+        w_rsrc = uniform_buffer(p.W + (int64_t)n0 * p.ldw, BUF_RANGE);
+    };
+    const int lds_lane0 = uwave * 64 * 16;
+    auto stage = [&](int buf, int unit, int kt) {
+        char* dst = smem + buf * BUF + unit * UNIT + lds_lane0;
+        const bool past = kt >= nt;
+        const int kbase = past ? 0 : kt * 128;
+        const bool masked = past || kbase + koff >= k16;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const int v = masked ? BUF_OOB : (unit < 2 ? a_off[q][unit & 1] : w_off[q][unit & 1]);
+            if (unit < 2) __builtin_amdgcn_raw_ptr_buffer_load_lds(a_rsrc, LDS_PTR(dst + q * 512 * 16), 16, v, kbase, 0, 0);
+            else __builtin_amdgcn_raw_ptr_buffer_load_lds(w_rsrc, LDS_PTR(dst + q * 512 * 16), 16, v, kbase, 0, 0);
+        }
+    };
+    const int sw = (li >> 1) & 7;
+    const int a_rd = (wr * 64 + li) * 128 + ((lg ^ (sw & 3)) << 4) + ((sw >> 2) << 6);
+    const int w_rd = (wc * 32 + li) * 128 + ((lg ^ (sw & 3)) << 4) + ((sw >> 2) << 6);
+
+    i32x4 acc[2][4][2][2];
+    auto prefetch = [&]() {
+        stage(0, 2, 0); stage(0, 0, 0); stage(0, 3, 0); stage(0, 1, 0);
+        stage(1, 2, 1); stage(1, 0, 1); stage(1, 3, 1);
+    };
+    setup(blockIdx.x);
+    prefetch();
+    for (int vb = blockIdx.x; vb < total; vb += gridDim.x) {
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int f = 0; f < 4; ++f)
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) acc[a][f][u][j] = (i32x4){0, 0, 0, 0};
+        // first tile: only its own loads are out; later ones: the previous epilogue's stores as well
+        if (vb == (int)blockIdx.x) asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        if (wr == 1) __builtin_amdgcn_s_barrier();
+        i32x4 af[4][2], w0f[2][2], w1f[2][2];
+        const int iters = (nt + 1) >> 1;
+        for (int it = 0; it < iters; ++it) {
+            const int te = 2 * it;
+            bool tail = false;
+#pragma unroll
+            for (int ph = 0; ph < 8; ++ph) {
+                const int buf = ph >> 2, sub = ph & 3;
+                if (ph == 4 && te + 1 >= nt) { tail = true; break; }
+                const char* sb = smem + buf * BUF;
+                if (sub == 0) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int ks = 0; ks < 2; ++ks) w0f[j][ks] = *(const i32x4*)(sb + 2 * UNIT + ((w_rd + j * 2048) ^ (ks << 6)));
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int f = 0; f < 4; ++f)
+#pragma unroll
+                        for (int ks = 0; ks < 2; ++ks) af[f][ks] = *(const i32x4*)(sb + ((a_rd + f * 2048) ^ (ks << 6)));
+                } else if (sub == 1) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int ks = 0; ks < 2; ++ks) w1f[j][ks] = *(const i32x4*)(sb + 3 * UNIT + ((w_rd + j * 2048) ^ (ks << 6)));
+                } else if (sub == 2) {
+#pragma unroll
+                    for (int f = 0; f < 4; ++f)
+#pragma unroll
+                        for (int ks = 0; ks < 2; ++ks) af[f][ks] = *(const i32x4*)(sb + UNIT + ((a_rd + f * 2048) ^ (ks << 6)));
+                }
+                switch (ph) {
+                    case 0: stage(1, 1, te + 1); break;
+                    case 1: stage(0, 2, te + 2); break;
+                    case 2: stage(0, 0, te + 2); break;
+                    case 3: stage(0, 3, te + 2); break;
+                    case 4: stage(0, 1, te + 2); break;
+                    case 5: stage(1, 2, te + 3); break;
+                    case 6: stage(1, 0, te + 3); break;
+                    default: stage(1, 3, te + 3); break;
+                }
+                if (sub == 0) asm volatile("s_waitcnt lgkmcnt(8)" ::: "memory");
+                if (sub == 3) asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
+                __builtin_amdgcn_s_barrier();
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                __builtin_amdgcn_s_setprio(1);
+                const int ua = sub >> 1, uw = (sub == 1 || sub == 2) ? 1 : 0;
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                    for (int f = 0; f < 4; ++f)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j)
+                            acc[ua][f][uw][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(uw ? w1f[j][ks] : w0f[j][ks], af[f][ks], acc[ua][f][uw][j], 0, 0, 0);
+                __builtin_amdgcn_s_setprio(0);
+                __builtin_amdgcn_s_barrier();
+            }
+            if (tail) break;
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (wr == 0) __builtin_amdgcn_s_barrier();
+
+        // the next tile's first loads travel under this tile's epilogue
+        const int e_m0 = m0, e_n0 = n0;
+        if (vb + (int)gridDim.x < total) {
+            setup(vb + gridDim.x);
+            prefetch();
+        }
+        // lane (li, lg) owns rows e_m0 + wr * 128 + a * 64 + f * 16 + li, columns c0 .. c0 + 15
+        const int c0 = e_n0 + wc * 64 + lg * 16;
+        float scale[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) scale[e] = p.sw[min(c0 + e, p.N - 1)];
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int f = 0; f < 4; ++f) {
+                const int m = e_m0 + wr * 128 + a * 64 + f * 16 + li;
+                if (m >= p.M) continue;
+                const float sa = p.sa[m];
+                float y[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    y[e] = i8_scaled(acc[a][f][e >> 3][(e >> 2) & 1][e & 3], sa, scale[e]);
+                    if (p.bias) y[e] += p.bias[min(c0 + e, p.N - 1)];
+                }
+                i8_store<16>(p, m, c0, y);
+            }
+    }
+}
+
+void launch_gemm256(const I8Params& p, hipStream_t s) {
+    static PerDeviceOnce once;
+    once.run([&] { HIP_CHECK(hipFuncSetAttribute((const void*)i8_gemm256_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS256)); });
+    // persistent: one workgroup per CU, a multiple of 8 so that a workgroup's tiles all map to its XCD
+    const int tiles = cdiv(p.M, 256) * cdiv(p.N, 256), cus = std::max(8, device_cus() & ~7);
+    ProfScope ps("i8_gemm256_kernel", 2.0 * p.M * p.N * p.K, s);
+    hipLaunchKernelGGL(i8_gemm256_kernel, dim3(std::min(tiles, cus)), dim3(512), LDS256, s, p);
+    HIP_CHECK(hipGetLastError());
+}
+
+// ---- a few rows: weights stream once, straight into registers ----
+//
+// HBM-bound (N * K bytes of weights): one workgroup takes 16 weight rows, its 8 waves take 64-wide steps of K in turn, and a
+// wave's share of up to NS steps is requested at once.  The activation rows are rounded to 8 bits by every workgroup for itself,
+// underneath those loads: they are a few KB from the L2, and a second kernel in front would cost more than the whole product.
+// Weight rows are the MFMA "A" operand (lane: row li, bytes 16 lg ..), the activation rows in LDS the "B".
+// FROM: 0 bf16 rows, 1 fp32 rows, 2 rows that are rounded already.  HELD > 0: the rows are aligned to 16 bytes, K is a multiple
+// of 8 and a thread's share of the rows, at most HELD pieces of 8 values, is requested before the weights and held in registers, so
+// that nothing waits behind the weights; 0: rows of any alignment and number, read twice.
+constexpr int FEW_THREADS = 512, FEW_WAVES = 8, FEW_ROWS = 16, FEW_LDS = 100 * 1024;
+constexpr int FEW_RED = FEW_WAVES * 256 * 4;
+__host__ __device__ inline int few_stride(int K) { return ((K + 63) & ~63) + 16; }   // rows 16 bytes apart modulo the banks
+
+template <int FROM, int NS, int HELD>
+__global__ __launch_bounds__(FEW_THREADS, 2) void i8_few_rows_kernel(I8Params p, I8Source src) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    __shared__ uint32_t amax[FEW_ROWS];
+    __shared__ float scale[FEW_ROWS];
+    constexpr bool F32 = FROM == 1;
+    const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int k16 = (p.K + 15) & ~15, steps = (p.K + 63) >> 6, stride = few_stride(p.K);
+    const int per_row = stride >> 3, pieces = p.M * per_row;   // pieces of 8 values, those behind K zero
+    int* const red = (int*)smem;                 // [wave][row][column]
+    char* const xq = smem + FEW_RED;             // [M][stride]
+
+    i32x4 w[NS];
+    // steps i0 + wave, i0 + wave + 8, ... of 16 weight rows.  Loads are unconditional (one behind a branch would make the waits
+    // count as if it had not been issued): what lies behind a row's end is read from its last 16 bytes and meets zeros.
+    auto request = [&](int n0, int i0) {
+        const int8_t* row = p.W + (int64_t)min(n0 + li, p.N - 1) * p.ldw;
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+            w[i] = __builtin_nontemporal_load((const i32x4*)(row + min((i0 + wave + FEW_WAVES * i) * 64 + lg * 16, k16 - 16)));
+    };
+    int n0 = blockIdx.x * 16;
+    if (tid < FEW_ROWS) amax[tid] = 0;
+    if constexpr (HELD > 0) {
+        constexpr int WORDS = F32 ? 2 : 1;
+        uint4 held[HELD][WORDS];
+        int row_of[HELD], k_of[HELD];
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            const int c = min(tid + FEW_THREADS * i, pieces - 1);
+            row_of[i] = c / per_row;
+            k_of[i] = (c - row_of[i] * per_row) * 8;
+            const char* at = (const char*)src.x + ((int64_t)row_of[i] * src.ldx + min(k_of[i], p.K - 8)) * (F32 ? 4 : 2);
+#pragma unroll
+            for (int j = 0; j < WORDS; ++j) held[i][j] = *(const uint4*)(at + 16 * j);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        request(n0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        __syncthreads();
+        auto values = [&](int i, float* v) {
+            const uint32_t word[8] = {held[i][0].x, held[i][0].y, held[i][0].z, held[i][0].w,
+                                      held[i][WORDS - 1].x, held[i][WORDS - 1].y, held[i][WORDS - 1].z, held[i][WORDS - 1].w};
+            const bool in = k_of[i] < p.K;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t bits = F32 ? word[e] : (e & 1) ? word[e >> 1] & 0xffff0000u : word[e >> 1] << 16;
+                v[e] = in ? __uint_as_float(bits) : 0.f;
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            float v[8];
+            values(i, v);
+            const uint32_t top = i8_max8(0, v);
+            const int first = __builtin_amdgcn_readfirstlane(row_of[i]);
+            if (first == __builtin_amdgcn_readlane(row_of[i], 63)) {   // the wave's pieces lie in one row
+                const uint32_t all = wave_max_bits(top);
+                if (lane == 0) atomicMax(&amax[first], all);
+            } else {
+                atomicMax(&amax[row_of[i]], top);
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            const RowScale rs(__uint_as_float(amax[row_of[i]]));
+            float v[8];
+            values(i, v);
+            if (tid + FEW_THREADS * i < pieces) {
+                *(uint2*)(xq + row_of[i] * stride + k_of[i]) = i8_pack8(rs, v);
+                if (k_of[i] == 0) scale[row_of[i]] = rs.scale;
+            }
+        }
+    } else if constexpr (FROM == 2) {
+        request(n0, 0);
+        for (int c = tid; c < pieces; c += FEW_THREADS) {
+            const int m = c / per_row, k = (c - m * per_row) * 8;
+            *(uint2*)(xq + m * stride + k) = k < k16 ? *(const uint2*)(p.A + (int64_t)m * p.lda + k) : make_uint2(0, 0);
+        }
+        if (tid < p.M) scale[tid] = p.sa[tid];
+    } else {
+        __syncthreads();
+        for (int c0 = 0; c0 < pieces; c0 += FEW_THREADS) {
+            const int c = min(c0 + tid, pieces - 1), m = c / per_row, k = (c - m * per_row) * 8;
+            const char* row = (const char*)src.x + (int64_t)m * src.ldx * (F32 ? 4 : 2);
+            float v[8];
+            i8_load8<F32>(row, k, p.K, (uintptr_t)row % 16 == 0, v);
+            const uint32_t top = i8_max8(0, v);
+            const int first = __builtin_amdgcn_readfirstlane(m);
+            if (first == __builtin_amdgcn_readlane(m, 63)) {
+                const uint32_t all = wave_max_bits(top);
+                if (lane == 0) atomicMax(&amax[first], all);
+            } else {
+                atomicMax(&amax[m], top);
+            }
+        }
+        __syncthreads();
+        for (int c = tid; c < pieces; c += FEW_THREADS) {
+            const int m = c / per_row, k = (c - m * per_row) * 8;
+            const RowScale rs(__uint_as_float(amax[m]));
+            const char* row = (const char*)src.x + (int64_t)m * src.ldx * (F32 ? 4 : 2);
+            float v[8];
+            i8_load8<F32>(row, k, p.K, (uintptr_t)row % 16 == 0, v);
+            *(uint2*)(xq + m * stride + k) = i8_pack8(rs, v);
+            if (k == 0) scale[m] = rs.scale;
+        }
+        request(n0, 0);
+    }
+    __syncthreads();
+
+    const char* const xr = xq + min(li, p.M - 1) * stride + lg * 16;
+    for (;;) {
+        i32x4 acc = (i32x4){0, 0, 0, 0};
+        for (int i0 = 0; i0 < steps; i0 += FEW_WAVES * NS) {
+            if (i0 > 0) request(n0, i0);
+#pragma unroll
+            for (int i = 0; i < NS; ++i) {
+                const int step = i0 + wave + FEW_WAVES * i;
+                if (step < steps) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[i], *(const i32x4*)(xr + step * 64), acc, 0, 0, 0);
+            }
+        }
+        const int done = n0;
+        n0 += gridDim.x * 16;
+        if (n0 < p.N) request(n0, 0);            // the next rows' weights travel while these are summed
+        // lane (li, lg) holds activation row li against weight rows 4 lg .. 4 lg + 3
+        *(i32x4*)(red + wave * 256 + li * 16 + 4 * lg) = acc;
+        __syncthreads();
+        if (tid < 256) {
+            const int m = tid >> 4, n = done + (tid & 15);
+            if (m < p.M && n < p.N) {
+                int sum = 0;
+#pragma unroll
+                for (int v = 0; v < FEW_WAVES; ++v) sum += red[v * 256 + tid];
+                const float y = i8_scaled(sum, scale[m], p.sw[n]) + (p.bias ? p.bias[n] : 0.f);
+                if (p.out_f32) ((float*)p.out)[(int64_t)m * p.ldo + n] = y;
+                else ((bf16_t*)p.out)[(int64_t)m * p.ldo + n] = f32_to_bf16(y);
+            }
+        }
+        if (n0 >= p.N) return;                   // the same for the whole workgroup
+        __syncthreads();
+    }
+}
+
+template <int FROM, int NS, int HELD>
+void launch_few(const I8Params& p, const I8Source& src, hipStream_t s) {
+    const int lds = FEW_RED + p.M * few_stride(p.K);
+    static PerDeviceOnce once;
+    once.run([&] {
+        HIP_CHECK(hipFuncSetAttribute((const void*)i8_few_rows_kernel<FROM, NS, HELD>, hipFuncAttributeMaxDynamicSharedMemorySize, FEW_RED + FEW_LDS));
+    });
+    ProfScope ps("i8_few_rows_kernel", (double)p.N * p.K, s);
+    hipLaunchKernelGGL((i8_few_rows_kernel<FROM, NS, HELD>), dim3(std::min(cdiv(p.N, 16), 512)), dim3(FEW_THREADS), lds, s, p, src);
+    HIP_CHECK(hipGetLastError());
+}
+template <int FROM, int HELD>
+void launch_few_steps(const I8Params& p, const I8Source& src, hipStream_t s) {
+    const int per_wave = cdiv(cdiv(p.K, 64), FEW_WAVES);
+    if (per_wave <= 4) launch_few<FROM, 4, HELD>(p, src, s);
+    else launch_few<FROM, 12, HELD>(p, src, s);
+}
+bool few_rows(int M, int K) { return M <= FEW_ROWS && M * (int64_t)few_stride(K) <= FEW_LDS; }
+template <int FROM>
+void launch_few_rows(const I8Params& p, const I8Source& src, hipStream_t s) {
+    const int held = cdiv((int64_t)p.M * (few_stride(p.K) >> 3), FEW_THREADS);
+    const bool vec = p.K % 8 == 0 && (uintptr_t)src.x % 16 == 0 && src.ldx * (src.f32 ? 4 : 2) % 16 == 0;
+    if (vec && held <= 2) launch_few_steps<FROM, 2>(p, src, s);
+    else if (vec && held <= 8) launch_few_steps<FROM, 8>(p, src, s);
+    else launch_few_steps<FROM, 0>(p, src, s);
+}
+
 // Sums of the parts of a split K.
 __global__ __launch_bounds__(256) void i8_reduce_kernel(I8Params p) {
     const int64_t total = (int64_t)p.M * p.N;
@@ -283,10 +702,11 @@ void launch_tile(const I8Params& p, hipStream_t s) {
 }
 
 struct I8Plan {
-    int tile;     // 0: 128 x 128, 1: 64 x 64
+    int tile;     // 0: 128 x 128, 1: 64 x 64, 2: 256 x 256
     int ksplit;
 };
 I8Plan i8_plan(int M, int N, int K) {
+    if ((int64_t)cdiv(M, 256) * cdiv(N, 256) >= 224) return {2, 1};
     if ((int64_t)cdiv(M, 128) * cdiv(N, 128) >= 384) return {0, 1};
     return {1, 1};
 }
@@ -296,9 +716,19 @@ I8Plan i8_plan(int M, int N, int K) {
 void launch_i8_quantize(const I8Source& src, int rows, int cols, int8_t* q, int64_t ldq, float* scales, hipStream_t s) {
     ProfScope ps("i8_quantize_kernel", (double)rows * cols * (src.f32 ? 5 : 3), s);
     const dim3 grid(cdiv(rows, 4)), block(256);
-    if (src.f32) hipLaunchKernelGGL((i8_quantize_kernel<true>), grid, block, 0, s, src.x, src.ldx, rows, cols, q, ldq, scales);
-    else hipLaunchKernelGGL((i8_quantize_kernel<false>), grid, block, 0, s, src.x, src.ldx, rows, cols, q, ldq, scales);
+#define I8_QUANTIZE(F32, HELD) hipLaunchKernelGGL((i8_quantize_kernel<F32, HELD>), grid, block, 0, s, src.x, src.ldx, rows, cols, q, ldq, scales)
+    if (cols <= 2048) { if (src.f32) I8_QUANTIZE(true, 4); else I8_QUANTIZE(false, 4); }
+    else if (cols <= 6144) { if (src.f32) I8_QUANTIZE(true, 12); else I8_QUANTIZE(false, 12); }
+    else { if (src.f32) I8_QUANTIZE(true, 0); else I8_QUANTIZE(false, 0); }
+#undef I8_QUANTIZE
     HIP_CHECK(hipGetLastError());
+}
+
+bool launch_i8_linear_few_rows(const I8Params& p, const I8Source& src, hipStream_t s) {
+    if (!few_rows(p.M, p.K)) return false;
+    if (src.f32) launch_few_rows<1>(p, src, s);
+    else launch_few_rows<0>(p, src, s);
+    return true;
 }
 
 int64_t i8_matmul_scratch(int M, int N, int K) {
@@ -307,12 +737,17 @@ int64_t i8_matmul_scratch(int M, int N, int K) {
 }
 
 void launch_i8_matmul(I8Params p, void* scratch, int64_t scratch_bytes, hipStream_t s) {
+    if (few_rows(p.M, p.K)) {
+        launch_few_steps<2, 0>(p, {}, s);
+        return;
+    }
     const I8Plan plan = i8_plan(p.M, p.N, p.K);
     Q3_REQUIRE(i8_matmul_scratch(p.M, p.N, p.K) <= scratch_bytes, "i8_matmul: workspace too small");
     p.vec_out = ((uintptr_t)p.out % 16 == 0) && p.ldo % (p.out_f32 ? 4 : 8) == 0;
     p.ksplit = plan.ksplit;
     p.slab = (int*)scratch;
-    if (plan.tile == 0) launch_tile<4, 4, 2>(p, s);
+    if (plan.tile == 2) launch_gemm256(p, s);
+    else if (plan.tile == 0) launch_tile<4, 4, 2>(p, s);
     else launch_tile<2, 2, 4>(p, s);
     if (p.ksplit > 1) {
         hipLaunchKernelGGL(i8_reduce_kernel, dim3((int)std::min<int64_t>(cdiv((int64_t)p.M * p.N, 256), 4096)), dim3(256), 0, s, p);
