@@ -138,7 +138,8 @@ int q3asr_i8_matmul(q3asr_model* m, const int8_t* a, int64_t lda, const float* a
     I8Params p;
     p.A = a; p.lda = lda; p.sa = a_scales; p.W = w; p.ldw = ldw; p.sw = w_scales; p.bias = bias;
     p.M = M; p.N = N; p.K = K; p.out = out; p.ldo = ldo; p.out_f32 = out_dtype == Q3ASR_F32;
-    launch_i8_matmul(p, workspace, workspace ? workspace_bytes : 0, call.s);
+    (void)workspace_bytes;   // the product alone keeps nothing
+    launch_i8_matmul(p, call.s);
     call.done();
     Q3_API_END
 }
@@ -150,8 +151,7 @@ int q3asr_i8_linear(q3asr_model* m, const void* x, int x_dtype, int64_t ldx, con
     Q3_REQUIRE(m && x && workspace, "i8_linear: null argument");
     check_product(w, ldw, w_scales, M, N, K, out, out_dtype, ldo, workspace);
     check_rows("i8_linear: x", x, x_dtype, ldx, K);
-    const int64_t quantized = quantized_bytes(M, K);
-    Q3_REQUIRE(workspace_bytes >= quantized + i8_matmul_scratch(M, N, K), "i8_linear: workspace too small");
+    Q3_REQUIRE(workspace_bytes >= quantized_bytes(M, K), "i8_linear: workspace too small");
     Call call(m, stream);
     I8Params p;
     p.A = (const int8_t*)workspace; p.lda = (K + 15) & ~15;
@@ -161,7 +161,7 @@ int q3asr_i8_linear(q3asr_model* m, const void* x, int x_dtype, int64_t ldx, con
     const I8Source src{x, x_dtype == Q3ASR_F32, ldx};
     if (!launch_i8_linear_few_rows(p, src, call.s)) {
         launch_i8_quantize(src, M, K, (int8_t*)p.A, p.lda, (float*)p.sa, call.s);
-        launch_i8_matmul(p, (char*)workspace + quantized, workspace_bytes - quantized, call.s);
+        launch_i8_matmul(p, call.s);
     }
     call.done();
     Q3_API_END
@@ -169,7 +169,7 @@ int q3asr_i8_linear(q3asr_model* m, const void* x, int x_dtype, int64_t ldx, con
 
 int64_t q3asr_i8_workspace(q3asr_model* m, int M, int N, int K) {
     if (!m || M <= 0 || N <= 0 || K <= 0 || K > I8_MAX_K) return -1;
-    return quantized_bytes(M, K) + i8_matmul_scratch(M, N, K);
+    return quantized_bytes(M, K);
 }
 
 int q3asr_pages_status(q3asr_model* m, const q3asr_kv_pages* c, int32_t* out, int clear, void* stream) {

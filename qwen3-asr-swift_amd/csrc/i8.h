@@ -17,13 +17,9 @@ struct I8Params {
     int M = 0, N = 0, K = 0;
     void* out = nullptr; int64_t ldo = 0; int out_f32 = 0;
     int vec_out = 0;       // rows of out can take 16-byte stores
-    int* slab = nullptr;   // split K: [ksplit][M][N] partial sums
-    int ksplit = 1;
 };
 
 void launch_i8_quantize(const I8Source& src, int rows, int cols, int8_t* q, int64_t ldq, float* scales, hipStream_t s);
 // Both steps in one kernel where the rows are few; false: it does not apply.
 bool launch_i8_linear_few_rows(const I8Params& p, const I8Source& src, hipStream_t s);
-// bytes of scratch that launch_i8_matmul wants for split sums
-int64_t i8_matmul_scratch(int M, int N, int K);
-void launch_i8_matmul(I8Params p, void* scratch, int64_t scratch_bytes, hipStream_t s);
+void launch_i8_matmul(I8Params p, hipStream_t s);

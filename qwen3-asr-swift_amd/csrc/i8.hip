@@ -20,14 +20,18 @@ namespace {
 // exact in one fused multiply-add (r * scale and x are multiples of half an ulp of scale wherever r != 0, and the difference
 // is below scale), so comparing twice the remainder with scale decides.  Scales so small that 1 / scale overflows or that products
 // with it leave the normal range are lifted by 2^64 together with x, which is exact.
+// Rounding is bound by vector instructions, so eight values take a short way first: adding 1.5 * 2^23 in the multiply-add leaves
+// the rounded quotient in the low bits, from where bytes are picked.  It is right unless some remainder reaches half of scale
+// (about one value in 10^5 for arbitrary data), and then the long way is taken.
 struct RowScale {
     float scale, s, inv, lift;
+    __device__ RowScale() {}
     __device__ explicit RowScale(float amax) {
         scale = amax / 127.0f;
         const bool bad = !(amax < INFINITY);       // infinity or NaN somewhere in the row
         lift = scale < 7.8886090522101181e-31f ? 18446744073709551616.0f : 1.0f;   // 2^-100, 2^64
-        s = scale * lift;
-        inv = s > 0.f && !bad ? 1.0f / s : 0.f;
+        s = bad ? 0.f : scale * lift;
+        inv = s > 0.f ? 1.0f / s : 0.f;
         if (bad) scale = __builtin_nanf("");
     }
     __device__ int whole(float x) const {
@@ -36,6 +40,26 @@ struct RowScale {
         const float e2 = 2.0f * fabsf(fmaf(-r, s, v)), dir = copysignf(1.0f, fmaf(-r, s, v));
         if (e2 > s || (e2 == s && ((int)r & 1))) r += dir;
         return inv > 0.f ? (int)fminf(fmaxf(r, -127.0f), 127.0f) : 0;
+    }
+    __device__ uint2 pack8(const float* v) const {
+        uint32_t bits[8];
+        float far = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float t = fmaf(v[e], inv, 12582912.0f);
+            bits[e] = __float_as_uint(t);
+            far = fmaxf(far, fabsf(fmaf(12582912.0f - t, s, v[e])));
+        }
+        if (2.0f * far < s && lift == 1.0f) {   // false for rows of zeros and rows that are not finite as well
+            uint2 b;
+            b.x = __builtin_amdgcn_perm(__builtin_amdgcn_perm(bits[3], bits[2], 0x0c0c0400), __builtin_amdgcn_perm(bits[1], bits[0], 0x0c0c0400), 0x05040100);
+            b.y = __builtin_amdgcn_perm(__builtin_amdgcn_perm(bits[7], bits[6], 0x0c0c0400), __builtin_amdgcn_perm(bits[5], bits[4], 0x0c0c0400), 0x05040100);
+            return b;
+        }
+        uint32_t b[2] = {0, 0};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) b[e >> 2] |= (uint32_t)(whole(v[e]) & 255) << (8 * (e & 3));
+        return make_uint2(b[0], b[1]);
     }
 };
 
@@ -67,17 +91,17 @@ __device__ __forceinline__ void i8_load8(const void* row, int k, int cols, bool 
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = k + e < cols ? i8_load<F32>(row, k + e) : 0.f;
 }
-__device__ __forceinline__ uint2 i8_pack8(const RowScale& rs, const float* v) {
-    uint32_t b[2] = {0, 0};
-#pragma unroll
-    for (int e = 0; e < 8; ++e) b[e >> 2] |= (uint32_t)(rs.whole(v[e]) & 255) << (8 * (e & 3));
-    return make_uint2(b[0], b[1]);
-}
 // Magnitudes are compared as the bits of non-negative floats, an order in which a NaN lies above infinity.
 __device__ __forceinline__ uint32_t i8_max8(uint32_t m, const float* v) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(v[e]) & 0x7fffffffu);
     return m;
+}
+// Largest magnitude of four bf16 values, as the bits of a float.
+__device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    const u16x2 m = __builtin_elementwise_max(__builtin_bit_cast(u16x2, a & 0x7fff7fffu), __builtin_bit_cast(u16x2, b & 0x7fff7fffu));
+    return (uint32_t)max(m.x, m.y) << 16;
 }
 template <int CTRL>
 __device__ __forceinline__ uint32_t dpp_max_bits(uint32_t v) {
@@ -94,13 +118,24 @@ __device__ __forceinline__ uint32_t wave_max_bits(uint32_t v) {
     return max(max(a, b), max(c, d));
 }
 
-// One wave per row, 8 values per lane and step; rows of up to 512 * HELD values stay in registers between the maximum and the
-// rounding, longer ones are read twice.
-template <bool F32, int HELD>
+// One wave per row, or (WHOLE) a workgroup's four waves where the rows are few; 8 values per lane and step.  Rows of up to
+// 512 * HELD values (2048 * HELD) stay in registers between the maximum and the rounding, longer ones are read twice.
+template <bool F32, int HELD, bool WHOLE>
 __global__ __launch_bounds__(256) void i8_quantize_kernel(const void* x, int64_t ldx, int rows, int cols, int8_t* q, int64_t ldq, float* scales) {
-    const int lane = threadIdx.x & 63;
-    const int row = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= rows) return;
+    constexpr int STEP = WHOLE ? 256 : 64;
+    const int lane = WHOLE ? threadIdx.x : threadIdx.x & 63;
+    const int row = WHOLE ? blockIdx.x : blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= rows) return;   // WHOLE: never
+    __shared__ uint32_t top[4];
+    auto row_max = [&](uint32_t m) {
+        m = wave_max_bits(m);
+        if constexpr (WHOLE) {
+            if ((lane & 63) == 0) top[lane >> 6] = m;
+            __syncthreads();
+            m = max(max(top[0], top[1]), max(top[2], top[3]));
+        }
+        return __uint_as_float(m);
+    };
     const void* src = (const char*)x + (int64_t)row * ldx * (F32 ? 4 : 2);
     const bool vec = (uintptr_t)src % 16 == 0;
     int8_t* dst = q + (int64_t)row * ldq;
@@ -109,27 +144,27 @@ __global__ __launch_bounds__(256) void i8_quantize_kernel(const void* x, int64_t
     if constexpr (HELD > 0) {
         float v[HELD][8];
 #pragma unroll
-        for (int i = 0; i < HELD; ++i) i8_load8<F32>(src, (i * 64 + lane) * 8, cols, vec, v[i]);
+        for (int i = 0; i < HELD; ++i) i8_load8<F32>(src, (i * STEP + lane) * 8, cols, vec, v[i]);
 #pragma unroll
         for (int i = 0; i < HELD; ++i) m = i8_max8(m, v[i]);
-        const RowScale rs(__uint_as_float(wave_max_bits(m)));
+        const RowScale rs(row_max(m));
         if (lane == 0) scales[row] = rs.scale;
 #pragma unroll
         for (int i = 0; i < HELD; ++i) {
-            const int k = (i * 64 + lane) * 8;
-            if (k < k16) *(uint2*)(dst + k) = i8_pack8(rs, v[i]);
+            const int k = (i * STEP + lane) * 8;
+            if (k < k16) *(uint2*)(dst + k) = rs.pack8(v[i]);
         }
     } else {
         float v[8];
-        for (int k = lane * 8; k < cols; k += 512) {
+        for (int k = lane * 8; k < cols; k += 8 * STEP) {
             i8_load8<F32>(src, k, cols, vec, v);
             m = i8_max8(m, v);
         }
-        const RowScale rs(__uint_as_float(wave_max_bits(m)));
+        const RowScale rs(row_max(m));
         if (lane == 0) scales[row] = rs.scale;
-        for (int k = lane * 8; k < k16; k += 512) {
+        for (int k = lane * 8; k < k16; k += 8 * STEP) {
             i8_load8<F32>(src, k, cols, vec, v);
-            *(uint2*)(dst + k) = i8_pack8(rs, v);
+            *(uint2*)(dst + k) = rs.pack8(v);
         }
     }
 }
@@ -163,13 +198,37 @@ __device__ __forceinline__ void i8_store(const I8Params& p, int m, int c, const 
         }
 }
 
+// The same for rows that cannot take 16-byte stores: a wave's 16 rows x 4 * NC columns go through its own piece of LDS (16 rows of
+// 4 * NC + 1 words) so that a store instruction writes along rows instead of touching 64 lines.  Column q of the block is
+// column c + (q / NC) * step + q % NC of the matrix.
+template <int NC>
+__device__ __forceinline__ void i8_store_rows(const I8Params& p, int m, int c, int step, const float* y, float* piece) {
+    constexpr int W = 4 * NC;
+    const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int e = 0; e < NC; ++e) piece[li * (W + 1) + lg * NC + e] = y[e];
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+    for (int i = 0; i < W / 4; ++i) {
+        const int r = (i * 64 + lane) / W, q = (i * 64 + lane) % W, row = m + r, col = c + q / NC * step + q % NC;
+        const float v = piece[r * (W + 1) + q];
+        if (row < p.M && col < p.N) {
+            if (p.out_f32) ((float*)p.out)[(int64_t)row * p.ldo + col] = v;
+            else ((bf16_t*)p.out)[(int64_t)row * p.ldo + col] = f32_to_bf16(v);
+        }
+    }
+}
+
 // Tile BM x BN x 128 per 256-thread workgroup (4 waves as 2 x 2).  Operands are staged global -> LDS by 16-byte loads into a
 // ring of STAGES tiles (lane-linear image, XOR swizzle on the source chunk and on the fragment read); the weight fragment
 // is the MFMA "A" operand, with weight rows dealt to MFMA rows so that a lane owns 4 * NT consecutive output columns.
-template <int MT, int NT, int STAGES>
+template <int MT, int NT, int STAGES, int SUB>
 __global__ __launch_bounds__(256, 2) void i8_gemm_kernel(I8Params p) {
     constexpr int BM = 32 * MT, BN = 32 * NT;
-    constexpr int A_BYTES = BM * 128, W_BYTES = BN * 128, STAGE = A_BYTES + W_BYTES;
+    constexpr int A_BYTES = BM * 128, W_BYTES = BN * 128, PART = A_BYTES + W_BYTES, STAGE = SUB * PART;
     constexpr int AP = BM * 8 / 256, WP = BN * 8 / 256;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, lane = tid & 63;
@@ -188,9 +247,7 @@ __global__ __launch_bounds__(256, 2) void i8_gemm_kernel(I8Params p) {
     const int m0 = (first_m + (L % per_group) % gsz) * BM, n0 = (L % per_group) / gsz * BN;
 
     const int k16 = (p.K + 15) & ~15;
-    const int nk_total = (k16 + 127) >> 7;
-    const int per = (nk_total + p.ksplit - 1) / p.ksplit;
-    const int kt0 = blockIdx.z * per, kt1 = min(nk_total, kt0 + per);
+    const int nt = (k16 + 128 * SUB - 1) / (128 * SUB);
 
     constexpr int BUF_RANGE = 0x40000000, BUF_OOB = 0x7f000000;   // offsets at or beyond the range read as zero (K tail)
     const auto a_rsrc = uniform_buffer(p.A + (int64_t)m0 * p.lda, BUF_RANGE);
@@ -209,22 +266,38 @@ __global__ __launch_bounds__(256, 2) void i8_gemm_kernel(I8Params p) {
         w_koff[q] = sc * 16;
         w_voff[q] = (min(n0 + row, p.N - 1) - n0) * (int)p.ldw + sc * 16;
     }
-    auto stage = [&](int buf, int kt) {
-        char* sa = smem + buf * STAGE;
-        char* sw = sa + A_BYTES;
-        const int kbase = kt * 128;
-        const bool tail = kbase + 128 > k16;
+    auto stage = [&](int buf, int t) {
 #pragma unroll
-        for (int q = 0; q < AP; ++q) {
-            const int v = tail && kbase + a_koff[q] >= k16 ? BUF_OOB : a_voff[q];
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(a_rsrc, LDS_PTR(sa + (q * 256 + uwave * 64) * 16), 16, v, kbase, 0, 0);
-        }
+        for (int h = 0; h < SUB; ++h) {
+            char* sa = smem + buf * STAGE + h * PART;
+            char* sw = sa + A_BYTES;
+            const int kbase = (t * SUB + h) * 128;
+            const bool tail = kbase + 128 > k16;
 #pragma unroll
-        for (int q = 0; q < WP; ++q) {
-            const int v = tail && kbase + w_koff[q] >= k16 ? BUF_OOB : w_voff[q];
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(w_rsrc, LDS_PTR(sw + (q * 256 + uwave * 64) * 16), 16, v, kbase, 0, 0);
+            for (int q = 0; q < AP; ++q) {
+                const int v = tail && kbase + a_koff[q] >= k16 ? BUF_OOB : a_voff[q];
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(a_rsrc, LDS_PTR(sa + (q * 256 + uwave * 64) * 16), 16, v, kbase, 0, 0);
+            }
+#pragma unroll
+            for (int q = 0; q < WP; ++q) {
+                const int v = tail && kbase + w_koff[q] >= k16 ? BUF_OOB : w_voff[q];
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(w_rsrc, LDS_PTR(sw + (q * 256 + uwave * 64) * 16), 16, v, kbase, 0, 0);
+            }
         }
     };
+
+    // the epilogue's operands, ahead of everything else
+    const int c0 = n0 + wc * 16 * NT + lg * 4 * NT;
+    float scale_w[4 * NT], bias[4 * NT], scale_a[MT];
+#pragma unroll
+    for (int e = 0; e < 4 * NT; ++e) {
+        const int c = min(c0 + e, p.N - 1);
+        scale_w[e] = p.sw[c];
+        bias[e] = p.bias ? p.bias[c] : 0.f;
+    }
+#pragma unroll
+    for (int a = 0; a < MT; ++a) scale_a[a] = p.sa[min(m0 + wr * 16 * MT + a * 16 + li, p.M - 1)];
+    __builtin_amdgcn_sched_barrier(0);
 
     i32x4 acc[MT][NT];
 #pragma unroll
@@ -242,70 +315,53 @@ __global__ __launch_bounds__(256, 2) void i8_gemm_kernel(I8Params p) {
     }
     // Iteration t: wait until this wave's loads of tile t have landed (the STAGES - 2 younger tiles stay in flight), barrier,
     // refill the buffer of tile t - 1, compute tile t.
-    constexpr int INFLIGHT = (STAGES - 2) * (AP + WP);
+    constexpr int INFLIGHT = (STAGES - 2) * SUB * (AP + WP);
     static_assert(INFLIGHT <= 63, "vmcnt field overflow");
-    const int nt = kt1 - kt0;
 #pragma unroll
     for (int s = 0; s < STAGES - 1; ++s)
-        if (s < nt) stage(s, kt0 + s);
+        if (s < nt) stage(s, s);
     for (int t = 0; t < nt; ++t) {
         if (t + STAGES - 2 < nt) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(INFLIGHT) : "memory");
         else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
-        if (t + STAGES - 1 < nt) stage((t + STAGES - 1) % STAGES, kt0 + t + STAGES - 1);
+        if (t + STAGES - 1 < nt) stage((t + STAGES - 1) % STAGES, t + STAGES - 1);
         const char* sb = smem + (t % STAGES) * STAGE;
-        i32x4 wf[2][NT], af[2][MT];
+        i32x4 wf[SUB][2][NT], af[SUB][2][MT];
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
+        for (int h = 0; h < SUB; ++h)
 #pragma unroll
-            for (int b = 0; b < NT; ++b) wf[ks][b] = *(const i32x4*)(sb + w_rd[ks] + b * 4 * 128);
+            for (int ks = 0; ks < 2; ++ks) {
 #pragma unroll
-            for (int a = 0; a < MT; ++a) af[ks][a] = *(const i32x4*)(sb + a_rd[ks] + a * 16 * 128);
-        }
+                for (int b = 0; b < NT; ++b) wf[h][ks][b] = *(const i32x4*)(sb + h * PART + w_rd[ks] + b * 4 * 128);
+#pragma unroll
+                for (int a = 0; a < MT; ++a) af[h][ks][a] = *(const i32x4*)(sb + h * PART + a_rd[ks] + a * 16 * 128);
+            }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
+        for (int h = 0; h < SUB; ++h)
 #pragma unroll
-            for (int a = 0; a < MT; ++a)
+            for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-                for (int b = 0; b < NT; ++b) acc[a][b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[ks][b], af[ks][a], acc[a][b], 0, 0, 0);
+                for (int a = 0; a < MT; ++a)
+#pragma unroll
+                    for (int b = 0; b < NT; ++b)
+                        acc[a][b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[h][ks][b], af[h][ks][a], acc[a][b], 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
     }
 
     // epilogue: lane (li, lg) owns row m, columns c0 .. c0 + 4 * NT - 1
-    const int c0 = n0 + wc * 16 * NT + lg * 4 * NT;
-    if (p.ksplit > 1) {
-#pragma unroll
-        for (int a = 0; a < MT; ++a) {
-            const int m = m0 + wr * 16 * MT + a * 16 + li;
-            if (m >= p.M) continue;
-            int* o = p.slab + ((int64_t)blockIdx.z * p.M + m) * p.N;
-#pragma unroll
-            for (int b = 0; b < NT; ++b)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (c0 + b * 4 + r < p.N) o[c0 + b * 4 + r] = acc[a][b][r];
-        }
-        return;
-    }
-    float sw[4 * NT], bias[4 * NT];
-#pragma unroll
-    for (int e = 0; e < 4 * NT; ++e) {
-        const int c = min(c0 + e, p.N - 1);
-        sw[e] = p.sw[c];
-        bias[e] = p.bias ? p.bias[c] : 0.f;
-    }
+    float* const piece = (float*)smem + uwave * 16 * (16 * NT + 1);
+    if (!p.vec_out) __syncthreads();   // the tiles in LDS have been read by all waves
 #pragma unroll
     for (int a = 0; a < MT; ++a) {
-        const int m = m0 + wr * 16 * MT + a * 16 + li;
-        if (m >= p.M) continue;
-        const float sa = p.sa[m];
+        const int m = m0 + wr * 16 * MT + a * 16;
         float y[4 * NT];
 #pragma unroll
         for (int b = 0; b < NT; ++b)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) y[b * 4 + r] = i8_scaled(acc[a][b][r], sa, sw[b * 4 + r]) + bias[b * 4 + r];
-        i8_store<4 * NT>(p, m, c0, y);
+            for (int r = 0; r < 4; ++r) y[b * 4 + r] = i8_scaled(acc[a][b][r], scale_a[a], scale_w[b * 4 + r]) + bias[b * 4 + r];
+        if (!p.vec_out) i8_store_rows<4 * NT>(p, m, n0 + wc * 16 * NT, 4 * NT, y, piece);
+        else if (m + li < p.M) i8_store<4 * NT>(p, m + li, c0, y);
     }
 }
 
@@ -316,7 +372,9 @@ __global__ __launch_bounds__(256, 2) void i8_gemm_kernel(I8Params p) {
 // over byte for byte: a K tile is 128 bytes of a row, which are 64 bf16 or 128 int8 values, and a 16-byte fragment feeds one
 // 16x16x32 bf16 or one 16x16x64 int8 MFMA of the same length.  Twice the work per byte moved, so the phases are the same and
 // the rate doubles.
-constexpr int UNIT = 128 * 128, BUF = 4 * UNIT, LDS256 = 2 * BUF;   // A0 | A1 | W0 | W1, two K tiles
+constexpr int UNIT = 128 * 128, BUF = 4 * UNIT;   // A0 | A1 | W0 | W1, two K tiles
+constexpr int SCALES = 3 * 256 * 4, PIECE = 16 * 33 * 4;
+constexpr int LDS256 = 2 * BUF + 2 * SCALES + 8 * PIECE;   // scales of the tile's rows, columns, and the bias, for two tiles; a piece per wave
 
 __global__ __launch_bounds__(512, 2) void i8_gemm256_kernel(I8Params p) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -335,6 +393,7 @@ __global__ __launch_bounds__(512, 2) void i8_gemm256_kernel(I8Params p) {
     int m0 = 0, n0 = 0;
     int a_off[2][2], w_off[2][2];
     __amdgpu_buffer_rsrc_t a_rsrc, w_rsrc;
+    int parity = 0;
     auto setup = [&](int b) {
         const int q8 = total >> 3, r8 = total & 7, x = b & 7;
         const int L = (x < r8 ? x * (q8 + 1) : r8 * (q8 + 1) + (x - r8) * q8) + (b >> 3);
@@ -370,7 +429,18 @@ __global__ __launch_bounds__(512, 2) void i8_gemm256_kernel(I8Params p) {
     const int w_rd = (wc * 32 + li) * 128 + ((lg ^ (sw & 3)) << 4) + ((sw >> 2) << 6);
 
     i32x4 acc[2][4][2][2];
+    // The scales come first: 4 bytes per thread, waves 0-3 the rows', waves 4-7 the columns', waves 0-3 the bias.  What lies behind
+    // the last row or column reads as zero.
     auto prefetch = [&]() {
+        char* sc = smem + 2 * BUF + parity * SCALES + uwave * 256;
+        const bool rows = uwave < 4;
+        const int at = (tid & 255) * 4;
+        const auto rsrc = uniform_buffer(rows ? p.sa + m0 : p.sw + n0, min(256, rows ? p.M - m0 : p.N - n0) * 4);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, LDS_PTR(sc), 4, at, 0, 0, 0);
+        if (rows && p.bias) {
+            const auto brsrc = uniform_buffer(p.bias + n0, min(256, p.N - n0) * 4);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(brsrc, LDS_PTR(sc + 2048), 4, at, 0, 0, 0);
+        }
         stage(0, 2, 0); stage(0, 0, 0); stage(0, 3, 0); stage(0, 1, 0);
         stage(1, 2, 1); stage(1, 0, 1); stage(1, 3, 1);
     };
@@ -385,9 +455,8 @@ __global__ __launch_bounds__(512, 2) void i8_gemm256_kernel(I8Params p) {
                 for (int u = 0; u < 2; ++u)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) acc[a][f][u][j] = (i32x4){0, 0, 0, 0};
-        // first tile: only its own loads are out; later ones: the previous epilogue's stores as well
+        // first tile: its first K tile has landed; later ones: all of their loads have, before the previous tile's stores
         if (vb == (int)blockIdx.x) asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         if (wr == 1) __builtin_amdgcn_s_barrier();
         i32x4 af[4][2], w0f[2][2], w1f[2][2];
@@ -452,31 +521,52 @@ __global__ __launch_bounds__(512, 2) void i8_gemm256_kernel(I8Params p) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         if (wr == 0) __builtin_amdgcn_s_barrier();
 
-        // the next tile's first loads travel under this tile's epilogue
+        // The next tile's first loads travel while this tile's sums become results; they have landed before the first store is
+        // issued, so that the stores drain under the next tile's first phases.
         const int e_m0 = m0, e_n0 = n0;
+        const char* const sc = smem + 2 * BUF + parity * SCALES;
+        parity ^= 1;
         if (vb + (int)gridDim.x < total) {
             setup(vb + gridDim.x);
             prefetch();
         }
         // lane (li, lg) owns rows e_m0 + wr * 128 + a * 64 + f * 16 + li, columns c0 .. c0 + 15
-        const int c0 = e_n0 + wc * 64 + lg * 16;
-        float scale[16];
+        const int c0 = wc * 64 + lg * 16;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) scale[e] = p.sw[min(c0 + e, p.N - 1)];
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const float4 sw4 = *(const float4*)(sc + 1024 + (c0 + u * 8 + j * 4) * 4);
+                float4 bias = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (p.bias) bias = *(const float4*)(sc + 2048 + (c0 + u * 8 + j * 4) * 4);
+#pragma unroll
+                for (int a = 0; a < 2; ++a)
+#pragma unroll
+                    for (int f = 0; f < 4; ++f) {
+                        const float sa = *(const float*)(sc + (wr * 128 + a * 64 + f * 16 + li) * 4);
+                        i32x4& v = acc[a][f][u][j];
+                        v[0] = __float_as_int(i8_scaled(v[0], sa, sw4.x) + bias.x);
+                        v[1] = __float_as_int(i8_scaled(v[1], sa, sw4.y) + bias.y);
+                        v[2] = __float_as_int(i8_scaled(v[2], sa, sw4.z) + bias.z);
+                        v[3] = __float_as_int(i8_scaled(v[3], sa, sw4.w) + bias.w);
+                    }
+            }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
         for (int a = 0; a < 2; ++a)
 #pragma unroll
             for (int f = 0; f < 4; ++f) {
-                const int m = e_m0 + wr * 128 + a * 64 + f * 16 + li;
-                if (m >= p.M) continue;
-                const float sa = p.sa[m];
+                const int m = e_m0 + wr * 128 + a * 64 + f * 16;
                 float y[16];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    y[e] = i8_scaled(acc[a][f][e >> 3][(e >> 2) & 1][e & 3], sa, scale[e]);
-                    if (p.bias) y[e] += p.bias[min(c0 + e, p.N - 1)];
+                for (int e = 0; e < 16; ++e) y[e] = __int_as_float(acc[a][f][e >> 3][(e >> 2) & 1][e & 3]);
+                if (!p.vec_out) {
+                    float* const piece = (float*)(smem + 2 * BUF + 2 * SCALES + uwave * PIECE);
+                    i8_store_rows<8>(p, m, e_n0 + wc * 64, 16, y, piece);
+                    i8_store_rows<8>(p, m, e_n0 + wc * 64 + 8, 16, y + 8, piece);
+                } else if (m + li < p.M) {
+                    i8_store<16>(p, m + li, e_n0 + c0, y);
                 }
-                i8_store<16>(p, m, c0, y);
             }
     }
 }
@@ -500,7 +590,7 @@ void launch_gemm256(const I8Params& p, hipStream_t s) {
 // FROM: 0 bf16 rows, 1 fp32 rows, 2 rows that are rounded already.  HELD > 0: the rows are aligned to 16 bytes, K is a multiple
 // of 8 and a thread's share of the rows, at most HELD pieces of 8 values, is requested before the weights and held in registers, so
 // that nothing waits behind the weights; 0: rows of any alignment and number, read twice.
-constexpr int FEW_THREADS = 512, FEW_WAVES = 8, FEW_ROWS = 16, FEW_LDS = 100 * 1024;
+constexpr int FEW_THREADS = 512, FEW_WAVES = 8, FEW_ROWS = 6, FEW_LDS = 100 * 1024;
 constexpr int FEW_RED = FEW_WAVES * 256 * 4;
 __host__ __device__ inline int few_stride(int K) { return ((K + 63) & ~63) + 16; }   // rows 16 bytes apart modulo the banks
 
@@ -508,7 +598,7 @@ template <int FROM, int NS, int HELD>
 __global__ __launch_bounds__(FEW_THREADS, 2) void i8_few_rows_kernel(I8Params p, I8Source src) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     __shared__ uint32_t amax[FEW_ROWS];
-    __shared__ float scale[FEW_ROWS];
+    __shared__ RowScale scales[FEW_ROWS];
     constexpr bool F32 = FROM == 1;
     const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -518,13 +608,15 @@ __global__ __launch_bounds__(FEW_THREADS, 2) void i8_few_rows_kernel(I8Params p,
     char* const xq = smem + FEW_RED;             // [M][stride]
 
     i32x4 w[NS];
-    // steps i0 + wave, i0 + wave + 8, ... of 16 weight rows.  Loads are unconditional (one behind a branch would make the waits
+    // pairs of steps, so that a wave reads whole 128-byte lines
+    auto step_of = [&](int i0, int i) { return i0 + 2 * wave + (i & 1) + 2 * FEW_WAVES * (i >> 1); };
+    // a wave's steps of 16 weight rows.  Loads are unconditional (one behind a branch would make the waits
     // count as if it had not been issued): what lies behind a row's end is read from its last 16 bytes and meets zeros.
     auto request = [&](int n0, int i0) {
         const int8_t* row = p.W + (int64_t)min(n0 + li, p.N - 1) * p.ldw;
 #pragma unroll
         for (int i = 0; i < NS; ++i)
-            w[i] = __builtin_nontemporal_load((const i32x4*)(row + min((i0 + wave + FEW_WAVES * i) * 64 + lg * 16, k16 - 16)));
+            w[i] = __builtin_nontemporal_load((const i32x4*)(row + min(step_of(i0, i) * 64 + lg * 16, k16 - 16)));
     };
     int n0 = blockIdx.x * 16;
     if (tid < FEW_ROWS) amax[tid] = 0;
@@ -557,9 +649,15 @@ __global__ __launch_bounds__(FEW_THREADS, 2) void i8_few_rows_kernel(I8Params p,
         };
 #pragma unroll
         for (int i = 0; i < HELD; ++i) {
-            float v[8];
-            values(i, v);
-            const uint32_t top = i8_max8(0, v);
+            uint32_t top = 0;
+            if constexpr (F32) {
+                float v[8];
+                values(i, v);
+                top = i8_max8(0, v);
+            } else {
+                top = max(max_bf16x2(held[i][0].x, held[i][0].y), max_bf16x2(held[i][0].z, held[i][0].w));
+                top = k_of[i] < p.K ? top : 0;
+            }
             const int first = __builtin_amdgcn_readfirstlane(row_of[i]);
             if (first == __builtin_amdgcn_readlane(row_of[i], 63)) {   // the wave's pieces lie in one row
                 const uint32_t all = wave_max_bits(top);
@@ -569,15 +667,14 @@ __global__ __launch_bounds__(FEW_THREADS, 2) void i8_few_rows_kernel(I8Params p,
             }
         }
         __syncthreads();
+        if (tid < p.M) scales[tid] = RowScale(__uint_as_float(amax[tid]));
+        __syncthreads();
 #pragma unroll
         for (int i = 0; i < HELD; ++i) {
-            const RowScale rs(__uint_as_float(amax[row_of[i]]));
+            const RowScale rs = scales[row_of[i]];
             float v[8];
             values(i, v);
-            if (tid + FEW_THREADS * i < pieces) {
-                *(uint2*)(xq + row_of[i] * stride + k_of[i]) = i8_pack8(rs, v);
-                if (k_of[i] == 0) scale[row_of[i]] = rs.scale;
-            }
+            if (tid + FEW_THREADS * i < pieces) *(uint2*)(xq + row_of[i] * stride + k_of[i]) = rs.pack8(v);
         }
     } else if constexpr (FROM == 2) {
         request(n0, 0);
@@ -585,7 +682,7 @@ __global__ __launch_bounds__(FEW_THREADS, 2) void i8_few_rows_kernel(I8Params p,
             const int m = c / per_row, k = (c - m * per_row) * 8;
             *(uint2*)(xq + m * stride + k) = k < k16 ? *(const uint2*)(p.A + (int64_t)m * p.lda + k) : make_uint2(0, 0);
         }
-        if (tid < p.M) scale[tid] = p.sa[tid];
+        if (tid < p.M) scales[tid].scale = p.sa[tid];
     } else {
         __syncthreads();
         for (int c0 = 0; c0 < pieces; c0 += FEW_THREADS) {
@@ -603,14 +700,15 @@ __global__ __launch_bounds__(FEW_THREADS, 2) void i8_few_rows_kernel(I8Params p,
             }
         }
         __syncthreads();
+        if (tid < p.M) scales[tid] = RowScale(__uint_as_float(amax[tid]));
+        __syncthreads();
         for (int c = tid; c < pieces; c += FEW_THREADS) {
             const int m = c / per_row, k = (c - m * per_row) * 8;
-            const RowScale rs(__uint_as_float(amax[m]));
+            const RowScale rs = scales[m];
             const char* row = (const char*)src.x + (int64_t)m * src.ldx * (F32 ? 4 : 2);
             float v[8];
             i8_load8<F32>(row, k, p.K, (uintptr_t)row % 16 == 0, v);
-            *(uint2*)(xq + m * stride + k) = i8_pack8(rs, v);
-            if (k == 0) scale[m] = rs.scale;
+            *(uint2*)(xq + m * stride + k) = rs.pack8(v);
         }
         request(n0, 0);
     }
@@ -623,7 +721,7 @@ __global__ __launch_bounds__(FEW_THREADS, 2) void i8_few_rows_kernel(I8Params p,
             if (i0 > 0) request(n0, i0);
 #pragma unroll
             for (int i = 0; i < NS; ++i) {
-                const int step = i0 + wave + FEW_WAVES * i;
+                const int step = step_of(i0, i);
                 if (step < steps) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[i], *(const i32x4*)(xr + step * 64), acc, 0, 0, 0);
             }
         }
@@ -639,7 +737,7 @@ __global__ __launch_bounds__(FEW_THREADS, 2) void i8_few_rows_kernel(I8Params p,
                 int sum = 0;
 #pragma unroll
                 for (int v = 0; v < FEW_WAVES; ++v) sum += red[v * 256 + tid];
-                const float y = i8_scaled(sum, scale[m], p.sw[n]) + (p.bias ? p.bias[n] : 0.f);
+                const float y = i8_scaled(sum, scales[m].scale, p.sw[n]) + (p.bias ? p.bias[n] : 0.f);
                 if (p.out_f32) ((float*)p.out)[(int64_t)m * p.ldo + n] = y;
                 else ((bf16_t*)p.out)[(int64_t)m * p.ldo + n] = f32_to_bf16(y);
             }
@@ -666,91 +764,76 @@ void launch_few_steps(const I8Params& p, const I8Source& src, hipStream_t s) {
     if (per_wave <= 4) launch_few<FROM, 4, HELD>(p, src, s);
     else launch_few<FROM, 12, HELD>(p, src, s);
 }
-bool few_rows(int M, int K) { return M <= FEW_ROWS && M * (int64_t)few_stride(K) <= FEW_LDS; }
+// Whether rounding the rows in every workgroup is cheaper than a launch of its own (us, one kernel against two): 1 x 2048 -> 4096:
+// 4.9, 7.3; 5 x 2048 -> 4096: 7.1, 7.3; 8 x 2048 -> 4096: 7.6, 7.3; 5 x 6144 -> 2048: 11.7, 13.2; rows of any alignment, read
+// twice: 2 x 2048 -> 2048: 6.8, 7.4; 4: 9.3, 7.4.
 template <int FROM>
-void launch_few_rows(const I8Params& p, const I8Source& src, hipStream_t s) {
-    const int held = cdiv((int64_t)p.M * (few_stride(p.K) >> 3), FEW_THREADS);
+bool launch_few_rows(const I8Params& p, const I8Source& src, hipStream_t s) {
+    const int64_t held = cdiv((int64_t)p.M * (few_stride(p.K) >> 3), FEW_THREADS);
     const bool vec = p.K % 8 == 0 && (uintptr_t)src.x % 16 == 0 && src.ldx * (src.f32 ? 4 : 2) % 16 == 0;
+    if (p.M > FEW_ROWS || held > (vec ? 8 : 2)) return false;
     if (vec && held <= 2) launch_few_steps<FROM, 2>(p, src, s);
-    else if (vec && held <= 8) launch_few_steps<FROM, 8>(p, src, s);
+    else if (vec) launch_few_steps<FROM, 8>(p, src, s);
     else launch_few_steps<FROM, 0>(p, src, s);
+    return true;
 }
 
-// Sums of the parts of a split K.
-__global__ __launch_bounds__(256) void i8_reduce_kernel(I8Params p) {
-    const int64_t total = (int64_t)p.M * p.N;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int m = (int)(i / p.N), n = (int)(i - (int64_t)m * p.N);
-        int acc = 0;
-        for (int z = 0; z < p.ksplit; ++z) acc += p.slab[z * total + i];
-        const float y = i8_scaled(acc, p.sa[m], p.sw[n]) + (p.bias ? p.bias[n] : 0.f);
-        if (p.out_f32) ((float*)p.out)[(int64_t)m * p.ldo + n] = y;
-        else ((bf16_t*)p.out)[(int64_t)m * p.ldo + n] = f32_to_bf16(y);
-    }
-}
-
-template <int MT, int NT, int STAGES>
+template <int MT, int NT, int STAGES, int SUB>
 void launch_tile(const I8Params& p, hipStream_t s) {
-    constexpr int BM = 32 * MT, BN = 32 * NT, LDS = STAGES * (BM + BN) * 128;
+    constexpr int BM = 32 * MT, BN = 32 * NT, LDS = STAGES * SUB * (BM + BN) * 128;
     static PerDeviceOnce once;
     once.run([&] {
-        HIP_CHECK(hipFuncSetAttribute((const void*)i8_gemm_kernel<MT, NT, STAGES>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
+        HIP_CHECK(hipFuncSetAttribute((const void*)i8_gemm_kernel<MT, NT, STAGES, SUB>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
     });
     ProfScope ps("i8_gemm_kernel", 2.0 * p.M * p.N * p.K, s);
-    hipLaunchKernelGGL((i8_gemm_kernel<MT, NT, STAGES>), dim3(cdiv(p.M, BM) * cdiv(p.N, BN), 1, p.ksplit), dim3(256), LDS, s, p);
+    hipLaunchKernelGGL((i8_gemm_kernel<MT, NT, STAGES, SUB>), dim3(cdiv(p.M, BM) * cdiv(p.N, BN)), dim3(256), LDS, s, p);
     HIP_CHECK(hipGetLastError());
-}
-
-struct I8Plan {
-    int tile;     // 0: 128 x 128, 1: 64 x 64, 2: 256 x 256
-    int ksplit;
-};
-I8Plan i8_plan(int M, int N, int K) {
-    if ((int64_t)cdiv(M, 256) * cdiv(N, 256) >= 224) return {2, 1};
-    if ((int64_t)cdiv(M, 128) * cdiv(N, 128) >= 384) return {0, 1};
-    return {1, 1};
 }
 
 }  // namespace
 
 void launch_i8_quantize(const I8Source& src, int rows, int cols, int8_t* q, int64_t ldq, float* scales, hipStream_t s) {
     ProfScope ps("i8_quantize_kernel", (double)rows * cols * (src.f32 ? 5 : 3), s);
-    const dim3 grid(cdiv(rows, 4)), block(256);
-#define I8_QUANTIZE(F32, HELD) hipLaunchKernelGGL((i8_quantize_kernel<F32, HELD>), grid, block, 0, s, src.x, src.ldx, rows, cols, q, ldq, scales)
-    if (cols <= 2048) { if (src.f32) I8_QUANTIZE(true, 4); else I8_QUANTIZE(false, 4); }
-    else if (cols <= 6144) { if (src.f32) I8_QUANTIZE(true, 12); else I8_QUANTIZE(false, 12); }
-    else { if (src.f32) I8_QUANTIZE(true, 0); else I8_QUANTIZE(false, 0); }
+    const bool whole = rows <= 1024;
+    const dim3 grid(whole ? rows : cdiv(rows, 4)), block(256);
+#define I8_QUANTIZE(F32, HELD, WHOLE) \
+    hipLaunchKernelGGL((i8_quantize_kernel<F32, HELD, WHOLE>), grid, block, 0, s, src.x, src.ldx, rows, cols, q, ldq, scales)
+#define I8_QUANTIZE_TYPE(HELD, WHOLE) \
+    if (src.f32) I8_QUANTIZE(true, HELD, WHOLE); \
+    else I8_QUANTIZE(false, HELD, WHOLE)
+    if (whole) {
+        if (cols <= 2048) { I8_QUANTIZE_TYPE(1, true); }
+        else if (cols <= 8192) { I8_QUANTIZE_TYPE(4, true); }
+        else { I8_QUANTIZE_TYPE(0, true); }
+    } else {
+        if (cols <= 2048) { I8_QUANTIZE_TYPE(4, false); }
+        else if (cols <= 6144) { I8_QUANTIZE_TYPE(12, false); }
+        else { I8_QUANTIZE_TYPE(0, false); }
+    }
+#undef I8_QUANTIZE_TYPE
 #undef I8_QUANTIZE
     HIP_CHECK(hipGetLastError());
 }
 
 bool launch_i8_linear_few_rows(const I8Params& p, const I8Source& src, hipStream_t s) {
-    if (!few_rows(p.M, p.K)) return false;
-    if (src.f32) launch_few_rows<1>(p, src, s);
-    else launch_few_rows<0>(p, src, s);
-    return true;
+    return src.f32 ? launch_few_rows<1>(p, src, s) : launch_few_rows<0>(p, src, s);
 }
 
-int64_t i8_matmul_scratch(int M, int N, int K) {
-    const I8Plan plan = i8_plan(M, N, K);
-    return plan.ksplit > 1 ? (int64_t)plan.ksplit * M * N * 4 : 0;
-}
-
-void launch_i8_matmul(I8Params p, void* scratch, int64_t scratch_bytes, hipStream_t s) {
-    if (few_rows(p.M, p.K)) {
+void launch_i8_matmul(I8Params p, hipStream_t s) {
+    if (p.M <= FEW_ROWS && p.M * (int64_t)few_stride(p.K) <= FEW_LDS) {
         launch_few_steps<2, 0>(p, {}, s);
         return;
     }
-    const I8Plan plan = i8_plan(p.M, p.N, p.K);
-    Q3_REQUIRE(i8_matmul_scratch(p.M, p.N, p.K) <= scratch_bytes, "i8_matmul: workspace too small");
     p.vec_out = ((uintptr_t)p.out % 16 == 0) && p.ldo % (p.out_f32 ? 4 : 8) == 0;
-    p.ksplit = plan.ksplit;
-    p.slab = (int*)scratch;
-    if (plan.tile == 2) launch_gemm256(p, s);
-    else if (plan.tile == 0) launch_tile<4, 4, 2>(p, s);
-    else launch_tile<2, 2, 4>(p, s);
-    if (p.ksplit > 1) {
-        hipLaunchKernelGGL(i8_reduce_kernel, dim3((int)std::min<int64_t>(cdiv((int64_t)p.M * p.N, 256), 4096)), dim3(256), 0, s, p);
-        HIP_CHECK(hipGetLastError());
-    }
+    // The smallest tiles that still fit the device at once win while the sums are short of workgroups, because the walk along K
+    // is then all latency (us at K = 2048, and 6144 with *; 32 x 32 by 512 bytes of K, 32 x 64 by 512, by 256, 64 x 64, 128 x 128,
+    // 256 x 256):  64 x 4096: 5.0, 5.7, 5.9, 8.2, 13.8, 24;  128 x 2048*: 8.7, 11.1, 12.6, 18, 37, 58;  256 x 4096: 14, 9.8, 7.7, 8.3,
+    // 14, 26;  512 x 4096: 26, 18, 13, 9.3, 14.6, 26;  2000 x 4096: 98, 65, 47, 32, 22.4, 30;  1000 x 12288: 147, 98, 70, 47, 34, 32.
+    const auto tiles = [&](int bm, int bn) { return (int64_t)cdiv(p.M, bm) * cdiv(p.N, bn); };
+    if (tiles(32, 32) <= 256) launch_tile<1, 1, 3, 4>(p, s);
+    else if (tiles(32, 64) <= 256) launch_tile<1, 2, 3, 4>(p, s);
+    else if (tiles(32, 64) <= 512) launch_tile<1, 2, 3, 2>(p, s);
+    else if (tiles(64, 64) <= 512 || p.M <= 64) launch_tile<2, 2, 2, 2>(p, s);
+    else if (tiles(256, 256) >= 192 && p.M > 128) launch_gemm256(p, s);
+    else launch_tile<4, 4, 2, 1>(p, s);
 }
