@@ -1,15 +1,18 @@
 // Attention over the paged KV cache for sequences that share prefixes (gfx950).
 //
 // o = sum_j p_j v_j, p = softmax_j(scale q . k_j).  The keys of a sequence are cut into its group's shared pages and its own
-// pages, and both into chunks; a workgroup takes one chunk for one KV head and all query rows that read it -- of every
-// sequence of the group for a shared chunk, so that a shared key crosses HBM once per group -- and leaves (max, sum, weighted
-// sum of values) per row.  A second kernel joins the parts of a row.  Both softmax statistics and the sums stay in fp32; the
-// probabilities are rounded to bf16 for the matrix cores (2^-9 relative each, which averages out over the keys of a row).
+// pages, and both into chunks; a work item is one chunk for one KV head and up to 16 * QT of the query rows that read it -- of
+// every sequence of the group for a shared chunk, so that a shared key crosses HBM once per group -- and leaves (max, sum,
+// weighted sum of values) per row.  Three launches: one workgroup plans the items from the lengths and tables on the device,
+// sorted by size; a grid that fills the device once works them off; a last one joins the parts of the rows that have several.
+// Both softmax statistics and the sums stay in fp32; the probabilities are rounded to bf16 for the matrix cores (2^-9 relative
+// each on average, which averages out over the keys of a row).
 //
 // HBM-bound: with G query heads per KV head and H hypotheses a shared chunk is 16 * QT columns of a matrix product against
 // 2 * head_dim * 2 bytes per key.  Four waves take tiles of 32 keys in turn, each with its own statistics: S^T = K Q^T with the K
 // rows loaded from memory as MFMA A fragments, then O^T = V^T P^T, where the exponentiated scores are as they stand the B
-// fragment and the V rows reach the A fragments through transposing reads of a wave's own LDS tile.
+// fragment and the V rows reach the A fragments through transposing reads of a wave's own LDS tile.  A workgroup requests the
+// next item's first tile before it joins its waves' results, and that item's page numbers an item ahead.
 #include "paged.h"
 #include "prof.h"
 #include <algorithm>
@@ -21,8 +24,11 @@ typedef __attribute__((ext_vector_type(4))) short s16x4;
 
 namespace {
 
-constexpr int WAVES = 4;
-constexpr int CHUNK = 512;        // keys of a workgroup; at most 1024, a page number per lane and 16 keys
+constexpr int WAVES = 4, PLAN = 1024;
+constexpr int CHUNK_MAX = 1024;                   // keys: one page number per lane and 16 keys
+constexpr int BUCKETS = CHUNK_MAX / 32 + 1;       // items by their number of 32-key tiles
+constexpr int BATCH = 64;                         // items whose descriptions a workgroup holds at a time
+constexpr int CUS = 256;
 
 union Frag {
     bf16x8 v;
@@ -44,6 +50,23 @@ __device__ __forceinline__ float rows_sum(float x) {
     return __uint_as_float(h[0]) + __uint_as_float(h[1]);
 }
 
+// LDS written by some lanes of a wave is read by others behind this.
+__device__ __forceinline__ void wave_lds_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// A chunk of keys for up to 16 * QT query rows: row r of M is row r0 + r / group of the step, head kvh * group + r % group, and
+// sees keys below `limit` + r / group of an own chunk, all keys of a shared one.
+struct __attribute__((aligned(16))) Item {
+    int r0, M, first;   // first: the lowest r
+    int seq, k0, k1;    // keys [k0, k1) of the pages of sequence seq
+    int limit;          // SHARED: a shared chunk
+    int slot;           // where the part goes; DIRECT: it is the rows' only one and goes to the output
+};
+constexpr int SHARED = 0x7fffffff, DIRECT = -1;
+
 struct AttnParams {
     const bf16_t* q; int64_t q_ld;
     bf16_t* out; int64_t o_ld;
@@ -56,18 +79,15 @@ struct AttnParams {
     int n, rows, n_groups, heads, kv_heads, group;
     int max_rows, max_group_rows, max_len, max_own, max_shared;
     float scale_log2;
-    // shared chunks first, then own ones
-    int chunk_p, chunks_p, tiles_p, chunk_s, chunks_s, tiles_s, blocks_p, slots;
-    float* part_o;                             // [rows][heads][slots][D]
+    int chunk, chunks_p, chunks_s, slots, rows_p, rows_s;   // shared chunks' slots first, then own ones'; query rows of an item
+    int* count;                                // [1] items
+    int* parts;                                // [rows] parts of a row: shared | own << 16
+    Item* items;
     float2* part_ml;                           // [rows][heads][slots]: maximum (base 2), sum
+    float* part_o;                             // [rows][heads][slots][D]
 };
 
-// The query rows of a workgroup: row r of M is row r0 + r / group of the step, head kvh * group + r % group.
-struct Queries {
-    int r0, M, first;      // first: this workgroup's lowest r
-    int limit0, limit_t;   // row r sees keys below limit0 + limit_t * (r / group)
-};
-
+// ---- plan ----
 struct Entry {             // a sequence of the step
     int seq, r0, T, len;
     bool ok;
@@ -76,93 +96,203 @@ __device__ __forceinline__ Entry entry_of(const AttnParams& p, int i) {
     Entry e;
     e.seq = p.seqs[i];
     const int a = p.cu_rows[i], b = p.cu_rows[i + 1];
-    const bool ok = (unsigned)e.seq < (unsigned)p.max_seqs && a >= 0 && b >= a && b <= p.rows && b - a <= p.max_rows;
+    const bool in = (unsigned)e.seq < (unsigned)p.max_seqs, ok = in && a >= 0 && b >= a && b <= p.rows && b - a <= p.max_rows;
     e.r0 = ok ? a : 0;
     e.T = ok ? b - a : 0;
     e.len = ok ? p.lens[e.seq] : 0;
     e.ok = ok && e.len >= 0 && e.len <= p.max_len;
     if (!e.ok) {
-        if (threadIdx.x == 0) pages_error(p.status, (unsigned)e.seq < (unsigned)p.max_seqs ? Q3ASR_PAGES_BAD_BATCH : Q3ASR_PAGES_BAD_INDEX, i);
-        e.seq = ok ? e.seq : 0;
+        pages_error(p.status, in ? Q3ASR_PAGES_BAD_BATCH : Q3ASR_PAGES_BAD_INDEX, i);
+        e.seq = in ? e.seq : 0;
         e.len = min(max(e.len, 0), p.max_len);
     }
     return e;
 }
-// Tokens that a group reads from the pages of its first sequence.
+// Tokens that group g reads from the pages of its first sequence.
 __device__ __forceinline__ int shared_of(const AttnParams& p, int g, const Entry& first) {
-    return max(0, min(p.shared[g], first.len - first.T)) >> p.pt_shift << p.pt_shift;
+    return max(0, min(min(p.shared[g], p.max_shared), first.len - first.T)) >> p.pt_shift << p.pt_shift;
+}
+
+__global__ __launch_bounds__(PLAN) void paged_attn_plan_kernel(AttnParams p) {
+    __shared__ int bucket[BUCKETS];
+    const int tid = threadIdx.x;
+    for (int b = tid; b < BUCKETS; b += PLAN) bucket[b] = 0;
+    for (int r = tid; r < p.rows; r += PLAN) p.parts[r] = 0;
+    __syncthreads();
+    // The items of group g or sequence i, in any order: f(item).
+    auto items_of = [&](int which, bool report, auto f) {
+        Item it;
+        if (which < p.n_groups) {
+            const int g = which, i0 = p.cu_groups[g], i1 = p.cu_groups[g + 1];
+            if (i0 < 0 || i1 <= i0 || i1 > p.n) {
+                if (report && i1 != i0) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, g);
+                return;
+            }
+            const Entry first = entry_of(p, i0);
+            const int end = p.cu_rows[i1], keys = shared_of(p, g, first);
+            if (end < first.r0 || end > p.rows || end - first.r0 > p.max_group_rows || p.shared[g] > p.max_shared) {
+                if (report) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, i0);
+                if (end < first.r0 || end > p.rows) return;
+            }
+            it.r0 = first.r0;
+            it.M = (end - first.r0) * p.group;
+            it.seq = first.seq;
+            it.limit = SHARED;
+            for (int ch = 0; ch * p.chunk < keys; ++ch)
+                for (it.first = 0; it.first < it.M; it.first += p.rows_p) {
+                    it.k0 = ch * p.chunk;
+                    it.k1 = min(keys, it.k0 + p.chunk);
+                    it.slot = ch;
+                    f(it);
+                }
+            return;
+        }
+        const int i = which - p.n_groups;
+        const Entry e = entry_of(p, i);
+        int from = 0;      // keys before it are read by the group
+        bool ok = e.ok;
+        if (p.n_groups > 0) {
+            int lo = 0, hi = p.n_groups;   // the last group that begins at or before entry i
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (p.cu_groups[mid] <= i) lo = mid;
+                else hi = mid;
+            }
+            const int i0 = p.cu_groups[lo], i1 = p.cu_groups[lo + 1];
+            if (i0 >= 0 && i >= i0 && i < i1 && i1 <= p.n) {
+                const Entry first = i0 == i ? e : entry_of(p, i0);
+                from = shared_of(p, lo, first);
+                ok = ok && first.ok;
+            } else if (report) {
+                pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, i);
+            }
+        }
+        if (report && ok && (from > max(0, e.len - e.T) || e.len - from > p.max_own)) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, i);
+        const int own = min(max(0, e.len - from), p.chunks_s * p.chunk), parts_p = (from + p.chunk - 1) / p.chunk;
+        const int parts_s = max((own + p.chunk - 1) / p.chunk, parts_p ? 0 : 1);   // a row without keys has one empty part
+        it.r0 = e.r0;
+        it.M = e.T * p.group;
+        it.seq = e.seq;
+        it.limit = e.len - e.T + 1;
+        if (report)
+            for (int t = 0; t < e.T; ++t) p.parts[e.r0 + t] = parts_p | parts_s << 16;
+        for (int ch = 0; ch < parts_s; ++ch)
+            for (it.first = 0; it.first < it.M; it.first += p.rows_s) {
+                it.k0 = from + ch * p.chunk;
+                it.k1 = min(from + own, it.k0 + p.chunk);
+                it.slot = parts_p + parts_s == 1 ? DIRECT : p.chunks_p + ch;
+                f(it);
+            }
+    };
+    const int all = p.n_groups + p.n;
+    for (int w = tid; w < all; w += PLAN) items_of(w, true, [&](const Item& it) { atomicAdd(&bucket[(it.k1 - it.k0 + 31) >> 5], 1); });
+    __syncthreads();
+    if (tid == 0) {        // the largest first, so that the last items to be taken up are small
+        int at = 0;
+        for (int b = BUCKETS - 1; b >= 0; --b) {
+            const int n = bucket[b];
+            bucket[b] = at;
+            at += n;
+        }
+        *p.count = at;
+    }
+    __syncthreads();
+    for (int w = tid; w < all; w += PLAN) items_of(w, false, [&](const Item& it) { p.items[atomicAdd(&bucket[(it.k1 - it.k0 + 31) >> 5], 1)] = it; });
 }
 
 template <int D>
 struct Lds {
-    static constexpr int VROW = 2 * D + 32, OROW = D + 4;
+    static constexpr int KROW = 2 * D + 16, VROW = 2 * D + 32, OROW = D + 4;   // padded: fragment and transposing reads meet all banks
     static constexpr int V_BYTES = WAVES * 32 * VROW, O_BYTES = WAVES * 16 * OROW * 4;
     static constexpr int BYTES = V_BYTES > O_BYTES ? V_BYTES : O_BYTES;
 };
 
-// One workgroup's part: keys [k0, k1) of the sequence whose page numbers are in `pages`, for 16 * QT of the queries.
-template <int D, int QT>
-__device__ __forceinline__ void attend(const AttnParams& p, const int* pages, int kvh, int k0, int k1, const Queries& qs, int slot,
-                                       char* lds, float (*sm_m)[64], float (*sm_l)[64]) {
-    constexpr int NKS = D / 32, NDT = D / 16, LPR = D / 8, RPI = 64 / LPR, IV = 16 / RPI, VROW = Lds<D>::VROW, OROW = Lds<D>::OROW;
-    const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int nsub = (k1 - k0 + 15) >> 4, ntiles = (nsub + 1) >> 1;
+// A wave's registers that carry over from one item to the next.
+template <int D, int QMAX>
+struct Stream {
+    static constexpr int NKS = D / 32, LPR = D / 8, RPI = 64 / LPR, IV = 16 / RPI, NQ = (16 * QMAX * LPR + 255) / 256;
+    Frag kf[2][IV], vf[2][IV];    // a tile of 32 keys, as rows
+    uint4 qv[NQ];                 // the thread's pieces of the item's query rows, on their way to LDS
+    int ids;                      // page numbers of the item's chunk, 16 keys per lane
 
-    // page numbers of the chunk, 16 keys per lane
-    int ids = 0;
-    if (lane < nsub) {
-        ids = pages[(k0 + 16 * lane) >> p.pt_shift];
+    const AttnParams& p;
+    const int lane, li, lg;
+    int k0, nsub;
+    int64_t head;
+    __device__ Stream(const AttnParams& p_, int lane_) : p(p_), lane(lane_), li(lane_ & 15), lg(lane_ >> 4) {}
+
+    __device__ int page_numbers(int seq, int k0_, int k1_) const {
+        const int n = (k1_ - k0_ + 15) >> 4;
+        if (n <= 0) return 0;
+        return p.table[(int64_t)seq * p.max_seq_pages + ((k0_ + 16 * min(lane, n - 1)) >> p.pt_shift)];
+    }
+    __device__ void begin(int ids_, int kvh, int k0_, int k1_) {
+        k0 = k0_;
+        nsub = (k1_ - k0_ + 15) >> 4;
+        head = (int64_t)kvh * p.head_stride;
+        ids = ids_;
         if ((unsigned)ids >= (unsigned)p.pages) {
-            pages_error(p.status, Q3ASR_PAGES_BAD_INDEX, 0);
+            if (nsub > 0) pages_error(p.status, Q3ASR_PAGES_BAD_INDEX, 0);
             ids = 0;
         }
     }
-    const int64_t head = (int64_t)kvh * p.head_stride;
-    const int in_page = (1 << p.pt_shift) - 1;
-
-    Frag kf[2][NKS], vf[2][IV];
-    auto base_of = [&](int t, int h) -> int64_t {   // first value of 16 keys; those behind the last are read from the last's
+    __device__ void load_q(const Item& it, int kvh, int most) {
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+            const int idx = threadIdx.x + 256 * i, in = idx / LPR, r = it.first + in;
+            qv[i] = make_uint4(0, 0, 0, 0);
+            if (in < most && r < it.M) {
+                const int tok = r / p.group;
+                qv[i] = *(const uint4*)(p.q + (int64_t)(it.r0 + tok) * p.q_ld + (kvh * p.group + r - tok * p.group) * D + 8 * (idx % LPR));
+            }
+        }
+    }
+    __device__ void store_q(char* sq) const {
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+            const int idx = threadIdx.x + 256 * i, in = idx / LPR;
+            if (in < 16 * QMAX) *(uint4*)(sq + in * (2 * D + 16) + 16 * (idx % LPR)) = qv[i];
+        }
+    }
+    __device__ int64_t base_of(int t, int h) const {   // first value of 16 keys; those behind the last are read from the last's
         const int sub = min(2 * t + h, nsub - 1);
         const int64_t page = __builtin_amdgcn_readlane(ids, sub);
-        return page * p.page_stride + head + (int64_t)((k0 + 16 * sub) & in_page) * D;
-    };
-    auto load_k = [&](int t) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const bf16_t* src = p.K + base_of(t, h) + li * D + 8 * lg;
-#pragma unroll
-            for (int ks = 0; ks < NKS; ++ks) kf[h][ks].v = __builtin_nontemporal_load((const bf16x8*)(src + 32 * ks));
-        }
-    };
-    auto load_v = [&](int t) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const bf16_t* src = p.V + base_of(t, h) + (lane / LPR) * D + 8 * (lane % LPR);
-#pragma unroll
-            for (int i = 0; i < IV; ++i) vf[h][i].v = __builtin_nontemporal_load((const bf16x8*)(src + i * RPI * D));
-        }
-    };
-    int t = wave;
-    if (t < ntiles) {
-        load_k(t);
-        load_v(t);
+        return page * p.page_stride + head + (int64_t)((k0 + 16 * sub) & ((1 << p.pt_shift) - 1)) * D;
     }
+    // 32 keys of K or V as whole rows, RPI of them per instruction
+    __device__ void load(const bf16_t* pool, Frag (&x)[2][IV], int t) const {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const bf16_t* src = pool + base_of(t, h) + (lane / LPR) * D + 8 * (lane % LPR);
+#pragma unroll
+            for (int i = 0; i < IV; ++i) x[h][i].v = __builtin_nontemporal_load((const bf16x8*)(src + i * RPI * D));
+        }
+    }
+    __device__ void load_k(int t) { load(p.K, kf, t); }
+    __device__ void load_v(int t) { load(p.V, vf, t); }
+};
 
-    // queries as B fragments: lane (li, lg) holds values 32 ks + 8 lg .. of query li
-    Frag qf[QT][NKS];
-    int limit[QT], lowest = k1;
+// One item for one KV head; its first tile has been requested.  request_next: the same for the next one, which a single group of
+// queries leaves registers for before the join.
+template <int D, int QT, int QMAX, class F>
+__device__ __forceinline__ void attend(const AttnParams& p, const Item& it, int kvh, Stream<D, QMAX>& st, char* lds, char* sq, float (*sm_m)[64],
+                                       float (*sm_l)[64], F request_next) {
+    constexpr int NKS = D / 32, NDT = D / 16, LPR = D / 8, RPI = 64 / LPR, IV = 16 / RPI;
+    constexpr int KROW = Lds<D>::KROW, VROW = Lds<D>::VROW, OROW = Lds<D>::OROW;
+    const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int k0 = it.k0, k1 = it.k1, ntiles = (k1 - k0 + 31) >> 5;
+    int t = wave;
+
+    int limit[QT];
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
-        const int r = qs.first + 16 * qt + li;
-        const bool ok = r < qs.M;
-        const int rr = ok ? r : 0, tok = rr / p.group;
-        limit[qt] = ok ? min(k1, qs.limit0 + qs.limit_t * tok) : 0;
-        const bf16_t* src = p.q + (int64_t)(qs.r0 + tok) * p.q_ld + (kvh * p.group + rr - tok * p.group) * D + 8 * lg;
-#pragma unroll
-        for (int ks = 0; ks < NKS; ++ks) qf[qt][ks].u = ok ? *(const uint4*)(src + 32 * ks) : make_uint4(0, 0, 0, 0);
+        const int r = it.first + 16 * qt + li;
+        limit[qt] = r >= it.M ? 0 : it.limit == SHARED ? k1 : min(k1, it.limit + r / p.group);
     }
-    lowest = min(k1, qs.limit0);   // keys below it are seen by all rows
+    // queries as B fragments: lane (li, lg) reads values 32 ks + 8 lg .. of query li
+    const char* const qr = sq + li * (2 * D + 16) + 16 * lg;
+    const int lowest = min(k1, it.limit);   // keys below it are seen by all rows
 
     float m[QT], l[QT];
     f32x4 o[QT][NDT];
@@ -174,31 +304,44 @@ __device__ __forceinline__ void attend(const AttnParams& p, const int* pages, in
         for (int dt = 0; dt < NDT; ++dt) o[qt][dt] = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
     char* const vt = lds + wave * 32 * VROW;
+    char* const kw = vt + (lane / LPR) * KROW + 16 * (lane % LPR);
     char* const vw = vt + (lane / LPR) * VROW + 16 * (lane % LPR);
+    const char* const kr = vt + li * KROW + 16 * lg;
     // transposing reads: per 16 lanes a block of 4 keys x 16 dims, lane 4 a + b addresses key a, dims 4 b .. 4 b + 3
     const char* const vr = vt + (4 * lg + (li >> 2)) * VROW + (li & 3) * 8;
 
     auto tile = [&](auto last) {
         constexpr bool LAST = decltype(last)::value;
         const int kv0 = k0 + 32 * t;
-        f32x4 s[QT][2];
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                s[qt][h] = (f32x4){0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < IV; ++i) *(uint4*)(kw + (16 * h + i * RPI) * KROW) = st.kf[h][i].u;
+        if constexpr (!LAST) st.load_k(t + WAVES);
+        wave_lds_fence();
+        Frag ka[2][NKS];   // K rows as A fragments: lane (li, lg) reads values 32 ks + 8 lg .. of key li
 #pragma unroll
-                for (int ks = 0; ks < NKS; ++ks) s[qt][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[h][ks].v, qf[qt][ks].v, s[qt][h], 0, 0, 0);
-            }
-        if constexpr (!LAST) load_k(t + WAVES);
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int ks = 0; ks < NKS; ++ks) ka[h][ks].u = *(const uint4*)(kr + 16 * h * KROW + 64 * ks);
         Frag pf[QT];
         float alpha[QT];
         bool moved = false;
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) {
+            Frag qf[NKS];
+#pragma unroll
+            for (int ks = 0; ks < NKS; ++ks) qf[ks].u = *(const uint4*)(qr + qt * 16 * (2 * D + 16) + 64 * ks);
+            f32x4 s[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                s[h] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int ks = 0; ks < NKS; ++ks) s[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka[h][ks].v, qf[ks].v, s[h], 0, 0, 0);
+            }
             float sv[8], top = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) sv[j] = s[qt][j >> 2][j & 3] * p.scale_log2;
+            for (int j = 0; j < 8; ++j) sv[j] = s[j >> 2][j & 3] * p.scale_log2;
             if (kv0 + 32 > lowest) {   // the same for the whole workgroup's tile
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
@@ -219,19 +362,19 @@ __device__ __forceinline__ void attend(const AttnParams& p, const int* pages, in
             moved |= m_new != m[qt];
             m[qt] = m_new;
             pf[qt].u = make_uint4(pack_bf16x2(pe[0], pe[1]), pack_bf16x2(pe[2], pe[3]), pack_bf16x2(pe[4], pe[5]), pack_bf16x2(pe[6], pe[7]));
+            if constexpr (QT > 1) __builtin_amdgcn_sched_barrier(0);   // one group of queries' fragments in registers at a time
         }
+        __builtin_amdgcn_wave_barrier();   // the V rows go where the K rows were
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int i = 0; i < IV; ++i) {
                 // what lies behind the last key may be anything: a NaN there would survive its zero weight
                 const bool keep = !LAST || kv0 + 16 * h + i * RPI + lane / LPR < k1;
-                *(uint4*)(vw + (16 * h + i * RPI) * VROW) = keep ? vf[h][i].u : make_uint4(0, 0, 0, 0);
+                *(uint4*)(vw + (16 * h + i * RPI) * VROW) = keep ? st.vf[h][i].u : make_uint4(0, 0, 0, 0);
             }
-        if constexpr (!LAST) load_v(t + WAVES);
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        if constexpr (!LAST) st.load_v(t + WAVES);
+        wave_lds_fence();
         if (__builtin_amdgcn_ballot_w64(moved) != 0) {
 #pragma unroll
             for (int qt = 0; qt < QT; ++qt)
@@ -257,6 +400,7 @@ __device__ __forceinline__ void attend(const AttnParams& p, const int* pages, in
         tile(std::true_type{});
     }
 
+    if constexpr (QT == 1) request_next();
     // join the four waves, 16 queries at a time
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
@@ -270,12 +414,13 @@ __device__ __forceinline__ void attend(const AttnParams& p, const int* pages, in
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
         __syncthreads();
+        if (QT == 1) st.store_q(sq);   // the next item's: all waves are done with this one's
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) *(f32x4*)(so + (wave * 16 + li) * OROW + 16 * dt + 4 * lg) = o[qt][dt];
         __syncthreads();
         constexpr int PER = D / 16;   // values per thread
-        const int qi = tid >> 4, d0 = (tid & 15) * PER, r = qs.first + 16 * qt + qi;
-        if (r < qs.M) {
+        const int qi = tid >> 4, d0 = (tid & 15) * PER, r = it.first + 16 * qt + qi;
+        if (r < it.M) {
             float M = -INFINITY, L = 0.f, acc[PER];
 #pragma unroll
             for (int w = 0; w < WAVES; ++w) M = fmaxf(M, sm_m[w][16 * qt + qi]);
@@ -289,8 +434,8 @@ __device__ __forceinline__ void attend(const AttnParams& p, const int* pages, in
 #pragma unroll
                 for (int e = 0; e < PER; ++e) acc[e] += so[(w * 16 + qi) * OROW + d0 + e] * f;
             }
-            const int tok = r / p.group, row = qs.r0 + tok, hq = kvh * p.group + r - tok * p.group;
-            if (p.slots == 1) {
+            const int tok = r / p.group, row = it.r0 + tok, hq = kvh * p.group + r - tok * p.group;
+            if (it.slot == DIRECT) {
                 const float inv = L > 0.f || L != L ? 1.0f / L : 0.f;
                 uint32_t w[PER / 2];
 #pragma unroll
@@ -300,129 +445,107 @@ __device__ __forceinline__ void attend(const AttnParams& p, const int* pages, in
                 else *(uint2*)dst = make_uint2(w[0], w[1]);
                 if (p.lse && d0 == 0) p.lse[(int64_t)row * p.heads + hq] = (use + __builtin_amdgcn_logf(L)) * 0.69314718055994530942f;
             } else {
-                const int64_t at = ((int64_t)row * p.heads + hq) * p.slots + slot;
+                const int64_t at = ((int64_t)row * p.heads + hq) * p.slots + it.slot;
 #pragma unroll
                 for (int e = 0; e < PER; e += 4) *(float4*)(p.part_o + at * D + d0 + e) = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
                 if (d0 == 0) p.part_ml[at] = make_float2(M, L);
             }
         }
     }
+    if constexpr (QT > 1) {
+        request_next();
+        st.store_q(sq);
+    }
+    __syncthreads();   // the next item's tiles go where these results were
 }
 
 template <int D, int QP, int QS>
-__global__ __launch_bounds__(256, QP == 4 || QS == 4 ? 1 : 2) void paged_attn_kernel(AttnParams p) {
+__global__ __launch_bounds__(256, D == 64 || QP == 1 ? 3 : 2) void paged_attn_kernel(AttnParams p) {
     __shared__ __attribute__((aligned(16))) char lds[Lds<D>::BYTES];
+    __shared__ __attribute__((aligned(16))) char sq[16 * QP * (2 * D + 16)];
     __shared__ float sm_m[WAVES][64], sm_l[WAVES][64];
-    int b = blockIdx.x;
-    Queries qs;
-    if (b < p.blocks_p) {
-        const int kvh = b % p.kv_heads;
-        b /= p.kv_heads;
-        const int g = b % p.n_groups;
-        b /= p.n_groups;
-        const int tile = b % p.tiles_p, ch = b / p.tiles_p;
-        const int i0 = p.cu_groups[g], i1 = p.cu_groups[g + 1];
-        if (i0 < 0 || i1 <= i0 || i1 > p.n) {
-            if (threadIdx.x == 0 && (i0 < 0 || i1 < i0 || i1 > p.n)) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, g);
-            return;
+    __shared__ Item items[BATCH];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int total = *p.count * p.kv_heads;
+    Stream<D, QP> st(p, tid & 63);
+    auto item_at = [&](int j) {
+        Item it;
+        const int* src = (const int*)&items[j];
+        int* dst = (int*)&it;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dst[e] = __builtin_amdgcn_readfirstlane(src[e]);
+        return it;
+    };
+    for (int w0 = blockIdx.x; w0 < total; w0 += BATCH * gridDim.x) {
+        const int n = min(BATCH, (total - w0 + (int)gridDim.x - 1) / (int)gridDim.x);
+        __syncthreads();
+        if (tid < n) {
+            const uint4* src = (const uint4*)&p.items[(w0 + tid * (int)gridDim.x) / p.kv_heads];
+            uint4* dst = (uint4*)&items[tid];
+            dst[0] = src[0];
+            dst[1] = src[1];
         }
-        const Entry first = entry_of(p, i0);
-        const int end = p.cu_rows[i1], keys = shared_of(p, g, first);
-        if (end < first.r0 || end > p.rows || end - first.r0 > p.max_group_rows) {
-            if (threadIdx.x == 0) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, i0);
-            return;
-        }
-        qs.r0 = first.r0;
-        qs.M = (end - first.r0) * p.group;
-        qs.first = tile * 16 * QP;
-        qs.limit0 = 0x7fffffff;
-        qs.limit_t = 0;
-        if (qs.first >= qs.M) return;
-        const int k0 = ch * p.chunk_p, k1 = min(keys, k0 + p.chunk_p);
-        if (keys > p.max_shared && threadIdx.x == 0) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, i0);
-        if (k1 <= k0) {
-            for (int r = qs.first + threadIdx.x; r < min(qs.M, qs.first + 16 * QP); r += 256) {
-                const int tok = r / p.group, hq = kvh * p.group + r - tok * p.group;
-                p.part_ml[((int64_t)(qs.r0 + tok) * p.heads + hq) * p.slots + ch] = make_float2(-INFINITY, 0.f);
+        __syncthreads();
+        Item it = item_at(0);
+        auto request = [&](const Item& x, int kvh, int ids) {
+            st.begin(ids, kvh, x.k0, x.k1);
+            st.load_q(x, kvh, x.limit == SHARED ? 16 * QP : 16 * QS);
+            if (wave < (x.k1 - x.k0 + 31) >> 5) {
+                st.load_k(wave);
+                st.load_v(wave);
             }
-            return;
+        };
+        request(it, w0 % p.kv_heads, st.page_numbers(it.seq, it.k0, it.k1));
+        st.store_q(sq);
+        __syncthreads();
+        for (int j = 0; j < n; ++j) {
+            const int w = w0 + j * (int)gridDim.x, kvh = w % p.kv_heads, next_kvh = (w + (int)gridDim.x) % p.kv_heads;
+            const Item next = item_at(min(j + 1, n - 1));
+            const int next_ids = st.page_numbers(next.seq, next.k0, next.k1);
+            auto request_next = [&] { if (j + 1 < n) request(next, next_kvh, next_ids); };
+            if (QP != QS && it.limit == SHARED) attend<D, QP, QP>(p, it, kvh, st, lds, sq, sm_m, sm_l, request_next);
+            else attend<D, QS, QP>(p, it, kvh, st, lds, sq, sm_m, sm_l, request_next);
+            it = next;
         }
-        attend<D, QP>(p, p.table + (int64_t)first.seq * p.max_seq_pages, kvh, k0, k1, qs, ch, lds, sm_m, sm_l);
-        return;
     }
-    b -= p.blocks_p;
-    const int kvh = b % p.kv_heads;
-    b /= p.kv_heads;
-    const int i = b % p.n;
-    b /= p.n;
-    const int tile = b % p.tiles_s, ch = b / p.tiles_s;
-    const Entry e = entry_of(p, i);
-    int from = 0;   // keys before it are read by the group
-    bool ok = e.ok;
-    if (p.n_groups > 0) {
-        int g = -1;   // the last group that begins at or before entry i
-        for (int g0 = 0; g0 < p.n_groups; g0 += 64) {
-            const int at = g0 + (threadIdx.x & 63);
-            const unsigned long long below = __ballot(at < p.n_groups && p.cu_groups[at] <= i);
-            g += __popcll(below);
-            if (below != ~0ull) break;
-        }
-        if (g >= 0) {
-            const int i0 = p.cu_groups[g], i1 = p.cu_groups[g + 1];
-            if (i0 >= 0 && i >= i0 && i < i1 && i1 <= p.n) {
-                const Entry first = i0 == i ? e : entry_of(p, i0);
-                from = shared_of(p, g, first);
-                ok = ok && first.ok;
-            } else {
-                g = -1;
-            }
-        }
-        if (g < 0 && threadIdx.x == 0) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, i);
-    }
-    qs.r0 = e.r0;
-    qs.M = e.T * p.group;
-    qs.first = tile * 16 * QS;
-    qs.limit0 = e.len - e.T + 1;
-    qs.limit_t = 1;
-    if (qs.first >= qs.M) return;
-    const int k0 = from + ch * p.chunk_s, k1 = min(e.len, k0 + p.chunk_s);
-    if (threadIdx.x == 0 && ok && (from > max(0, e.len - e.T) || e.len - from > p.max_own)) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, i);
-    const int slot = p.chunks_p + ch;
-    if (k1 <= k0 && p.slots > 1) {
-        for (int r = qs.first + threadIdx.x; r < min(qs.M, qs.first + 16 * QS); r += 256) {
-            const int tok = r / p.group, hq = kvh * p.group + r - tok * p.group;
-            p.part_ml[((int64_t)(qs.r0 + tok) * p.heads + hq) * p.slots + slot] = make_float2(-INFINITY, 0.f);
-        }
-        return;
-    }
-    attend<D, QS>(p, p.table + (int64_t)e.seq * p.max_seq_pages, kvh, k0, max(k0, k1), qs, slot, lds, sm_m, sm_l);
 }
 
-// Joins the parts of a row: one wave per (row, head).
+// Joins the parts of a row that has several: one wave per (row, head).
 template <int D>
 __global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnParams p) {
+    constexpr int PER = D / 64, AHEAD = 8;
     const int lane = threadIdx.x & 63;
-    const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int64_t item = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (item >= (int64_t)p.rows * p.heads) return;
     const int row = (int)(item / p.heads), hq = (int)(item - (int64_t)row * p.heads);
-    if (row >= p.cu_rows[p.n]) return;
+    const int parts = p.parts[row], np = parts & 0xffff, n = np + (parts >> 16);
+    if (n <= 1) return;   // written already, or not a row of this step
+    auto slot_of = [&](int i) { return item * p.slots + (i < np ? i : p.chunks_p + i - np); };
     float M = -INFINITY;
-    for (int s = lane; s < p.slots; s += 64) M = fmaxf(M, p.part_ml[item * p.slots + s].x);
+    for (int i = lane; i < n; i += 64) M = fmaxf(M, p.part_ml[slot_of(i)].x);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
     const float use = M == -INFINITY ? 0.f : M;
-    constexpr int PER = D / 64;
     float L = 0.f, acc[PER];
 #pragma unroll
     for (int e = 0; e < PER; ++e) acc[e] = 0.f;
-    for (int s = 0; s < p.slots; ++s) {
-        const float2 ml = p.part_ml[item * p.slots + s];
-        if (ml.x == -INFINITY) continue;   // nothing seen: its sums were not written
-        const float f = __builtin_amdgcn_exp2f(ml.x - use);
-        L += ml.y * f;
-        const float* src = p.part_o + (item * p.slots + s) * D + lane * PER;
+    for (int i0 = 0; i0 < n; i0 += AHEAD) {   // the parts of a turn are requested together
+        float2 ml[AHEAD];
+        float v[AHEAD][PER];
 #pragma unroll
-        for (int e = 0; e < PER; ++e) acc[e] += src[e] * f;
+        for (int a = 0; a < AHEAD; ++a) {
+            const int64_t at = slot_of(min(i0 + a, n - 1));
+            ml[a] = p.part_ml[at];
+#pragma unroll
+            for (int e = 0; e < PER; ++e) v[a][e] = p.part_o[at * D + lane * PER + e];
+        }
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+            const float f = i0 + a < n ? __builtin_amdgcn_exp2f(ml[a].x - use) : 0.f;
+            L += ml[a].y * f;
+#pragma unroll
+            for (int e = 0; e < PER; ++e) acc[e] += v[a][e] * f;
+        }
     }
     const float inv = L > 0.f || L != L ? 1.0f / L : 0.f;
     bf16_t* dst = p.out + (int64_t)row * p.o_ld + hq * D + lane * PER;
@@ -432,45 +555,47 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnParams p) {
 }
 
 struct Plan {
-    int qp, qs;   // 16-query tiles per workgroup
-    int chunk_p, chunks_p, tiles_p, chunk_s, chunks_s, tiles_s, slots;
+    int qp, qs;           // 16-row tiles of a shared and of an own item
+    int chunk, chunks_p, chunks_s, slots;
+    int64_t items;        // at most
+    int64_t at_parts, at_items, at_ml, at_o, bytes;
 };
-int tiles_for(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
+int tiles_for(int64_t rows) { return rows <= 16 ? 1 : 2; }
 Plan plan_for(const q3asr_kv_pages& c, const q3asr_attn_batch& b, int heads) {
     Plan r{};
     const int group = heads / c.kv_heads;
     const bool shares = b.n_groups > 0 && b.max_shared >= c.page_tokens;
-    r.qs = tiles_for(b.max_rows * group);
-    r.qp = shares ? std::max(r.qs, tiles_for(std::min(b.max_group_rows, 64) * group)) : r.qs;
-    r.tiles_s = cdiv((int64_t)b.max_rows * group, 16 * r.qs);
-    r.chunk_s = CHUNK;
     const int own = shares ? b.max_own : b.max_len;
-    r.chunks_s = std::max(1, cdiv(own, r.chunk_s));
-    if (shares) {
-        r.tiles_p = cdiv((int64_t)b.max_group_rows * group, 16 * r.qp);
-        r.chunk_p = CHUNK;
-        r.chunks_p = cdiv(b.max_shared, r.chunk_p);
-    } else {
-        r.tiles_p = 1;
-        r.chunk_p = CHUNK;
-    }
+    r.qs = tiles_for((int64_t)b.max_rows * group);
+    r.qp = shares ? std::max(r.qs, tiles_for((int64_t)b.max_group_rows * group)) : r.qs;
+    // About three items per workgroup of a full device: fewer and larger items have less to join and less that begins and ends, more
+    // and smaller ones spread a few long sequences over the device.
+    const int64_t keys = (shares ? (int64_t)b.n_groups * b.max_shared : 0) + (int64_t)b.n * own;
+    r.chunk = (int)std::min<int64_t>(CHUNK_MAX, std::max<int64_t>(128, (keys * c.kv_heads / (CUS * 9) + 127) / 128 * 128));
+    r.chunks_p = shares ? cdiv(b.max_shared, r.chunk) : 0;
+    r.chunks_s = std::max(1, cdiv(own, r.chunk));
     r.slots = r.chunks_p + r.chunks_s;
+    r.items = (shares ? (int64_t)b.n_groups * r.chunks_p * cdiv((int64_t)b.max_group_rows * group, 16 * r.qp) : 0) +
+              (int64_t)b.n * r.chunks_s * cdiv((int64_t)b.max_rows * group, 16 * r.qs);
+    auto round = [](int64_t x) { return (x + 255) & ~255ll; };
+    r.at_parts = 256;
+    r.at_items = r.at_parts + round((int64_t)b.rows * 4);
+    r.at_ml = r.at_items + round(r.items * (int64_t)sizeof(Item));
+    r.at_o = r.at_ml + (r.slots > 1 ? round((int64_t)b.rows * heads * r.slots * 8) : 0);
+    r.bytes = r.at_o + (r.slots > 1 ? round((int64_t)b.rows * heads * r.slots * c.head_dim * 4) : 0);
     return r;
-}
-int64_t part_bytes(const q3asr_kv_pages& c, const q3asr_attn_batch& b, int heads, const Plan& r) {
-    return r.slots > 1 ? (((int64_t)b.rows * heads * r.slots * 8 + 255) & ~255ll) + (int64_t)b.rows * heads * r.slots * c.head_dim * 4 : 0;
 }
 
 template <int D>
-void launch_d(const AttnParams& p, const Plan& r, int blocks, hipStream_t s) {
-    const dim3 grid(blocks), block(256);
+void launch_d(const AttnParams& p, const Plan& r, hipStream_t s) {
+    const dim3 block(256);
+    hipLaunchKernelGGL(paged_attn_plan_kernel, dim3(1), dim3(PLAN), 0, s, p);
+    HIP_CHECK(hipGetLastError());
+    const dim3 grid((int)std::min<int64_t>(r.items * p.kv_heads, CUS * (D == 64 || r.qp == 1 ? 3 : 2)));
     switch (r.qp * 10 + r.qs) {
         case 11: hipLaunchKernelGGL((paged_attn_kernel<D, 1, 1>), grid, block, 0, s, p); break;
         case 21: hipLaunchKernelGGL((paged_attn_kernel<D, 2, 1>), grid, block, 0, s, p); break;
-        case 41: hipLaunchKernelGGL((paged_attn_kernel<D, 4, 1>), grid, block, 0, s, p); break;
-        case 22: hipLaunchKernelGGL((paged_attn_kernel<D, 2, 2>), grid, block, 0, s, p); break;
-        case 42: hipLaunchKernelGGL((paged_attn_kernel<D, 4, 2>), grid, block, 0, s, p); break;
-        default: hipLaunchKernelGGL((paged_attn_kernel<D, 4, 4>), grid, block, 0, s, p); break;
+        default: hipLaunchKernelGGL((paged_attn_kernel<D, 2, 2>), grid, block, 0, s, p); break;
     }
     HIP_CHECK(hipGetLastError());
     if (p.slots > 1) {
@@ -481,9 +606,7 @@ void launch_d(const AttnParams& p, const Plan& r, int blocks, hipStream_t s) {
 
 }  // namespace
 
-int64_t paged_attention_workspace(const q3asr_kv_pages& c, const q3asr_attn_batch& b, int heads) {
-    return part_bytes(c, b, heads, plan_for(c, b, heads));
-}
+int64_t paged_attention_workspace(const q3asr_kv_pages& c, const q3asr_attn_batch& b, int heads) { return plan_for(c, b, heads).bytes; }
 
 void launch_paged_attention(const q3asr_kv_pages& c, int layer, const bf16_t* q, int64_t q_ld, int heads, float scale,
                             const q3asr_attn_batch& b, bf16_t* out, int64_t o_ld, float* lse, void* workspace, hipStream_t s) {
@@ -498,21 +621,23 @@ void launch_paged_attention(const q3asr_kv_pages& c, int layer, const bf16_t* q,
     p.seqs = b.seqs; p.cu_rows = b.cu_rows; p.cu_groups = b.cu_groups; p.shared = b.shared;
     p.max_seqs = c.max_seqs; p.max_seq_pages = c.max_seq_pages; p.pages = c.pages;
     while ((1 << p.pt_shift) < c.page_tokens) ++p.pt_shift;
-    p.n = b.n; p.rows = b.rows; p.n_groups = r.chunks_p > 0 ? b.n_groups : 0;
+    const bool shares = r.chunks_p > 0;
+    p.n = b.n; p.rows = b.rows; p.n_groups = shares ? b.n_groups : 0;
     p.heads = heads; p.kv_heads = c.kv_heads; p.group = heads / c.kv_heads;
     p.max_rows = b.max_rows; p.max_group_rows = b.max_group_rows; p.max_len = b.max_len;
-    p.max_own = r.chunks_p > 0 ? b.max_own : b.max_len;
+    p.max_own = shares ? b.max_own : b.max_len;
     p.max_shared = b.max_shared;
     p.scale_log2 = scale * 1.44269504088896340736f;
-    p.chunk_p = r.chunk_p; p.chunks_p = r.chunks_p; p.tiles_p = r.tiles_p;
-    p.chunk_s = r.chunk_s; p.chunks_s = r.chunks_s; p.tiles_s = r.tiles_s; p.slots = r.slots;
-    const int64_t ml = ((int64_t)b.rows * heads * r.slots * 8 + 255) & ~255ll;
-    p.part_ml = (float2*)workspace;
-    p.part_o = (float*)((char*)workspace + ml);
-    const int64_t bp = (int64_t)p.n_groups * c.kv_heads * r.tiles_p * r.chunks_p, bs = (int64_t)b.n * c.kv_heads * r.tiles_s * r.chunks_s;
-    Q3_REQUIRE(bp + bs < (1ll << 31), "paged_attention: too many workgroups (smaller bounds in the batch make fewer)");
-    p.blocks_p = (int)bp;
+    p.chunk = r.chunk; p.chunks_p = r.chunks_p; p.chunks_s = r.chunks_s; p.slots = r.slots;
+    p.rows_p = 16 * r.qp; p.rows_s = 16 * r.qs;
+    char* ws = (char*)workspace;
+    p.count = (int*)ws;
+    p.parts = (int*)(ws + r.at_parts);
+    p.items = (Item*)(ws + r.at_items);
+    p.part_ml = (float2*)(ws + r.at_ml);
+    p.part_o = (float*)(ws + r.at_o);
+    Q3_REQUIRE(r.items * c.kv_heads < (1ll << 30) && r.slots < (1 << 15), "paged_attention: too much work for one call (smaller bounds in the batch make less)");
     ProfScope ps("paged_attn_kernel", 4.0 * b.rows * heads * (double)b.max_len * c.head_dim, s);
-    if (c.head_dim == 64) launch_d<64>(p, r, (int)(bp + bs), s);
-    else launch_d<128>(p, r, (int)(bp + bs), s);
+    if (c.head_dim == 64) launch_d<64>(p, r, s);
+    else launch_d<128>(p, r, s);
 }
