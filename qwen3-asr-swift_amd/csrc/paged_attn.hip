@@ -26,9 +26,9 @@ namespace {
 
 constexpr int WAVES = 4, PLAN = 1024;
 constexpr int CHUNK_MAX = 1024;                   // keys: one page number per lane and 16 keys
-constexpr int BUCKETS = CHUNK_MAX / 32 + 1;       // items by their number of 32-key tiles
+constexpr int BUCKETS = CHUNK_MAX / 32 + 1;       // items by their number of 32-key tiles; at most 64
 constexpr int BATCH = 64;                         // items whose descriptions a workgroup holds at a time
-constexpr int CUS = 256;
+constexpr int CUS = 256, PLAIN_ITEMS = 512;
 
 union Frag {
     bf16x8 v;
@@ -80,6 +80,9 @@ struct AttnParams {
     int max_rows, max_group_rows, max_len, max_own, max_shared;
     float scale_log2;
     int chunk, chunks_p, chunks_s, slots, rows_p, rows_s;   // shared chunks' slots first, then own ones'; query rows of an item
+    int plain;                                 // no plan: own items of whole sequences, tiles_s each
+    int tiles_s;
+    void* plan_ws;                             // what of a plan does not fit LDS
     int* count;                                // [1] items
     int* parts;                                // [rows] parts of a row: shared | own << 16
     Item* items;
@@ -92,7 +95,7 @@ struct Entry {             // a sequence of the step
     int seq, r0, T, len;
     bool ok;
 };
-__device__ __forceinline__ Entry entry_of(const AttnParams& p, int i) {
+__device__ __forceinline__ Entry entry_of(const AttnParams& p, int i, bool report) {
     Entry e;
     e.seq = p.seqs[i];
     const int a = p.cu_rows[i], b = p.cu_rows[i + 1];
@@ -102,40 +105,54 @@ __device__ __forceinline__ Entry entry_of(const AttnParams& p, int i) {
     e.len = ok ? p.lens[e.seq] : 0;
     e.ok = ok && e.len >= 0 && e.len <= p.max_len;
     if (!e.ok) {
-        pages_error(p.status, in ? Q3ASR_PAGES_BAD_BATCH : Q3ASR_PAGES_BAD_INDEX, i);
+        if (report) pages_error(p.status, in ? Q3ASR_PAGES_BAD_BATCH : Q3ASR_PAGES_BAD_INDEX, i);
         e.seq = in ? e.seq : 0;
         e.len = min(max(e.len, 0), p.max_len);
     }
     return e;
 }
-// Tokens that group g reads from the pages of its first sequence.
-__device__ __forceinline__ int shared_of(const AttnParams& p, int g, const Entry& first) {
-    return max(0, min(min(p.shared[g], p.max_shared), first.len - first.T)) >> p.pt_shift << p.pt_shift;
-}
 
+// Two dependent loads per sequence (its number, its length), everything else from LDS: with one workgroup nothing covers latency.
+// Lists beyond HELD entries or groups stay in the workspace.
+constexpr int HELD = 1024;
 __global__ __launch_bounds__(PLAN) void paged_attn_plan_kernel(AttnParams p) {
-    __shared__ int bucket[BUCKETS];
+    __shared__ int bucket[64];
+    __shared__ Entry held[HELD];
+    __shared__ int held_cu[HELD + 1], held_from[HELD];
     const int tid = threadIdx.x;
-    for (int b = tid; b < BUCKETS; b += PLAN) bucket[b] = 0;
+    Entry* const entry = p.n <= HELD ? held : (Entry*)p.plan_ws;
+    int* const from = p.n_groups <= HELD ? held_from : (int*)((Entry*)p.plan_ws + p.n);   // tokens that a group shares
+    const int* const cu = p.n_groups <= HELD ? held_cu : p.cu_groups;
+    if (tid < 64) bucket[tid] = 0;
     for (int r = tid; r < p.rows; r += PLAN) p.parts[r] = 0;
+    for (int i = tid; i < p.n; i += PLAN) entry[i] = entry_of(p, i, true);
+    if (p.n_groups > 0 && p.n_groups <= HELD)
+        for (int g = tid; g <= p.n_groups; g += PLAN) held_cu[g] = p.cu_groups[g];
     __syncthreads();
-    // The items of group g or sequence i, in any order: f(item).
+    for (int g = tid; g < p.n_groups; g += PLAN) {
+        const int i0 = cu[g], i1 = cu[g + 1], shared = p.shared[g];
+        from[g] = 0;
+        if (i0 < 0 || i1 < i0 || i1 > p.n) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, g);
+        else if (i1 > i0) {
+            const Entry first = entry[i0];
+            const int end = p.cu_rows[i1];
+            if (shared > p.max_shared || (first.ok && (end < first.r0 || end > p.rows || end - first.r0 > p.max_group_rows)))
+                pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, i0);
+            from[g] = max(0, min(min(shared, p.max_shared), first.len - first.T)) >> p.pt_shift << p.pt_shift;
+        }
+    }
+    __syncthreads();
+    // the items of group g (which = g) or sequence i (which = n_groups + i), in any order: f(item)
     auto items_of = [&](int which, bool report, auto f) {
         Item it;
         if (which < p.n_groups) {
-            const int g = which, i0 = p.cu_groups[g], i1 = p.cu_groups[g + 1];
-            if (i0 < 0 || i1 <= i0 || i1 > p.n) {
-                if (report && i1 != i0) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, g);
-                return;
-            }
-            const Entry first = entry_of(p, i0);
-            const int end = p.cu_rows[i1], keys = shared_of(p, g, first);
-            if (end < first.r0 || end > p.rows || end - first.r0 > p.max_group_rows || p.shared[g] > p.max_shared) {
-                if (report) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, i0);
-                if (end < first.r0 || end > p.rows) return;
-            }
+            const int i0 = cu[which], i1 = cu[which + 1], keys = from[which];
+            if (i0 < 0 || i1 <= i0 || i1 > p.n) return;
+            const Entry first = entry[i0];
+            const int end = min(p.cu_rows[i1], first.r0 + p.max_group_rows);
+            if (!first.ok || end > p.rows) return;
             it.r0 = first.r0;
-            it.M = (end - first.r0) * p.group;
+            it.M = max(0, end - first.r0) * p.group;
             it.seq = first.seq;
             it.limit = SHARED;
             for (int ch = 0; ch * p.chunk < keys; ++ch)
@@ -148,27 +165,26 @@ __global__ __launch_bounds__(PLAN) void paged_attn_plan_kernel(AttnParams p) {
             return;
         }
         const int i = which - p.n_groups;
-        const Entry e = entry_of(p, i);
-        int from = 0;      // keys before it are read by the group
+        const Entry e = entry[i];
+        int behind = 0;    // keys before it are read by the group
         bool ok = e.ok;
         if (p.n_groups > 0) {
             int lo = 0, hi = p.n_groups;   // the last group that begins at or before entry i
             while (hi - lo > 1) {
                 const int mid = (lo + hi) >> 1;
-                if (p.cu_groups[mid] <= i) lo = mid;
+                if (cu[mid] <= i) lo = mid;
                 else hi = mid;
             }
-            const int i0 = p.cu_groups[lo], i1 = p.cu_groups[lo + 1];
+            const int i0 = cu[lo], i1 = cu[lo + 1];
             if (i0 >= 0 && i >= i0 && i < i1 && i1 <= p.n) {
-                const Entry first = i0 == i ? e : entry_of(p, i0);
-                from = shared_of(p, lo, first);
-                ok = ok && first.ok;
+                behind = from[lo];
+                ok = ok && entry[i0].ok;
             } else if (report) {
                 pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, i);
             }
         }
-        if (report && ok && (from > max(0, e.len - e.T) || e.len - from > p.max_own)) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, i);
-        const int own = min(max(0, e.len - from), p.chunks_s * p.chunk), parts_p = (from + p.chunk - 1) / p.chunk;
+        if (report && ok && (behind > max(0, e.len - e.T) || e.len - behind > p.max_own)) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, i);
+        const int own = min(max(0, e.len - behind), p.chunks_s * p.chunk), parts_p = (behind + p.chunk - 1) / p.chunk;
         const int parts_s = max((own + p.chunk - 1) / p.chunk, parts_p ? 0 : 1);   // a row without keys has one empty part
         it.r0 = e.r0;
         it.M = e.T * p.group;
@@ -178,26 +194,50 @@ __global__ __launch_bounds__(PLAN) void paged_attn_plan_kernel(AttnParams p) {
             for (int t = 0; t < e.T; ++t) p.parts[e.r0 + t] = parts_p | parts_s << 16;
         for (int ch = 0; ch < parts_s; ++ch)
             for (it.first = 0; it.first < it.M; it.first += p.rows_s) {
-                it.k0 = from + ch * p.chunk;
-                it.k1 = min(from + own, it.k0 + p.chunk);
+                it.k0 = behind + ch * p.chunk;
+                it.k1 = min(behind + own, it.k0 + p.chunk);
                 it.slot = parts_p + parts_s == 1 ? DIRECT : p.chunks_p + ch;
                 f(it);
             }
     };
+    // the largest first, so that the last items to be taken up are small
+    auto bucket_of = [](const Item& it) { return BUCKETS - 1 - ((it.k1 - it.k0 + 31) >> 5); };
     const int all = p.n_groups + p.n;
-    for (int w = tid; w < all; w += PLAN) items_of(w, true, [&](const Item& it) { atomicAdd(&bucket[(it.k1 - it.k0 + 31) >> 5], 1); });
+    for (int w = tid; w < all; w += PLAN) items_of(w, true, [&](const Item& it) { atomicAdd(&bucket[bucket_of(it)], 1); });
     __syncthreads();
-    if (tid == 0) {        // the largest first, so that the last items to be taken up are small
-        int at = 0;
-        for (int b = BUCKETS - 1; b >= 0; --b) {
-            const int n = bucket[b];
-            bucket[b] = at;
-            at += n;
+    if (tid < 64) {
+        const int n = bucket[tid];
+        int x = n;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int t = __shfl_up(x, o, 64);
+            if (tid >= o) x += t;
         }
-        *p.count = at;
+        bucket[tid] = x - n;
+        if (tid == 63) *p.count = x;
     }
     __syncthreads();
-    for (int w = tid; w < all; w += PLAN) items_of(w, false, [&](const Item& it) { p.items[atomicAdd(&bucket[(it.k1 - it.k0 + 31) >> 5], 1)] = it; });
+    for (int w = tid; w < all; w += PLAN) items_of(w, false, [&](const Item& it) { p.items[atomicAdd(&bucket[bucket_of(it)], 1)] = it; });
+}
+
+// Without a plan the groups are not used; a workgroup of its own checks them all the same.
+__device__ void check_groups(const AttnParams& p) {
+    if (threadIdx.x == 0 && (p.cu_groups[0] != 0 || p.cu_groups[p.n_groups] != p.n)) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, 0);
+    for (int g = threadIdx.x; g < p.n_groups; g += 256) {
+        const int i0 = p.cu_groups[g], i1 = p.cu_groups[g + 1], shared = p.shared[g];
+        if (i0 < 0 || i1 < i0 || i1 > p.n) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, g);
+        else if (i1 > i0) {
+            const Entry first = entry_of(p, i0, false);
+            const int end = p.cu_rows[i1], behind = max(0, min(shared, first.len - first.T)) >> p.pt_shift << p.pt_shift;
+            if (!first.ok) continue;
+            if (shared > p.max_shared || end < first.r0 || end > p.rows || end - first.r0 > p.max_group_rows)
+                pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, i0);
+            for (int i = i0; i < i1; ++i) {
+                const Entry e = entry_of(p, i, false);
+                if (e.ok && (behind > max(0, e.len - e.T) || e.len - behind > p.max_own)) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, i);
+            }
+        }
+    }
 }
 
 template <int D>
@@ -466,7 +506,12 @@ __global__ __launch_bounds__(256, D == 64 || QP == 1 ? 3 : 2) void paged_attn_ke
     __shared__ float sm_m[WAVES][64], sm_l[WAVES][64];
     __shared__ Item items[BATCH];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int total = *p.count * p.kv_heads;
+    const int total = (p.plain ? p.n * p.tiles_s : *p.count) * p.kv_heads;
+    const int grid = (int)gridDim.x - (p.plain && p.n_groups > 0);
+    if ((int)blockIdx.x == grid) {
+        check_groups(p);
+        return;
+    }
     Stream<D, QP> st(p, tid & 63);
     auto item_at = [&](int j) {
         Item it;
@@ -476,11 +521,15 @@ __global__ __launch_bounds__(256, D == 64 || QP == 1 ? 3 : 2) void paged_attn_ke
         for (int e = 0; e < 8; ++e) dst[e] = __builtin_amdgcn_readfirstlane(src[e]);
         return it;
     };
-    for (int w0 = blockIdx.x; w0 < total; w0 += BATCH * gridDim.x) {
-        const int n = min(BATCH, (total - w0 + (int)gridDim.x - 1) / (int)gridDim.x);
+    for (int w0 = blockIdx.x; w0 < total; w0 += BATCH * grid) {
+        const int n = min(BATCH, (total - w0 + grid - 1) / grid);
         __syncthreads();
-        if (tid < n) {
-            const uint4* src = (const uint4*)&p.items[(w0 + tid * (int)gridDim.x) / p.kv_heads];
+        if (p.plain && tid < n) {
+            const int x = (w0 + tid * grid) / p.kv_heads, i = x / p.tiles_s;
+            const Entry e = entry_of(p, i, true);
+            items[tid] = Item{e.r0, e.T * p.group, (x - i * p.tiles_s) * 16 * QS, e.seq, 0, min(e.len, CHUNK_MAX), e.len - e.T + 1, DIRECT};
+        } else if (tid < n) {
+            const uint4* src = (const uint4*)&p.items[(w0 + tid * grid) / p.kv_heads];
             uint4* dst = (uint4*)&items[tid];
             dst[0] = src[0];
             dst[1] = src[1];
@@ -499,7 +548,7 @@ __global__ __launch_bounds__(256, D == 64 || QP == 1 ? 3 : 2) void paged_attn_ke
         st.store_q(sq);
         __syncthreads();
         for (int j = 0; j < n; ++j) {
-            const int w = w0 + j * (int)gridDim.x, kvh = w % p.kv_heads, next_kvh = (w + (int)gridDim.x) % p.kv_heads;
+            const int w = w0 + j * grid, kvh = w % p.kv_heads, next_kvh = (w + grid) % p.kv_heads;
             const Item next = item_at(min(j + 1, n - 1));
             const int next_ids = st.page_numbers(next.seq, next.k0, next.k1);
             auto request_next = [&] { if (j + 1 < n) request(next, next_kvh, next_ids); };
@@ -513,40 +562,49 @@ __global__ __launch_bounds__(256, D == 64 || QP == 1 ? 3 : 2) void paged_attn_ke
 // Joins the parts of a row that has several: one wave per (row, head).
 template <int D>
 __global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnParams p) {
-    constexpr int PER = D / 64, AHEAD = 8;
+    constexpr int PER = D / 64;
     const int lane = threadIdx.x & 63;
     const int64_t item = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (item >= (int64_t)p.rows * p.heads) return;
     const int row = (int)(item / p.heads), hq = (int)(item - (int64_t)row * p.heads);
-    const int parts = p.parts[row], np = parts & 0xffff, n = np + (parts >> 16);
+    const int parts = __builtin_amdgcn_readfirstlane(p.parts[row]), np = parts & 0xffff, n = np + (parts >> 16);
     if (n <= 1) return;   // written already, or not a row of this step
     auto slot_of = [&](int i) { return item * p.slots + (i < np ? i : p.chunks_p + i - np); };
-    float M = -INFINITY;
-    for (int i = lane; i < n; i += 64) M = fmaxf(M, p.part_ml[slot_of(i)].x);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
-    const float use = M == -INFINITY ? 0.f : M;
-    float L = 0.f, acc[PER];
+    float M = -INFINITY, L = 0.f, acc[PER];
 #pragma unroll
     for (int e = 0; e < PER; ++e) acc[e] = 0.f;
-    for (int i0 = 0; i0 < n; i0 += AHEAD) {   // the parts of a turn are requested together
-        float2 ml[AHEAD];
-        float v[AHEAD][PER];
+    // parts are requested several at a time, behind the last one the last again
+    auto turn = [&](int i0, auto ahead, bool maximum_known) {
+        constexpr int A = decltype(ahead)::value;
+        float2 ml[A];
+        float v[A][PER];
 #pragma unroll
-        for (int a = 0; a < AHEAD; ++a) {
+        for (int a = 0; a < A; ++a) {
             const int64_t at = slot_of(min(i0 + a, n - 1));
             ml[a] = p.part_ml[at];
 #pragma unroll
             for (int e = 0; e < PER; ++e) v[a][e] = p.part_o[at * D + lane * PER + e];
         }
+        if (!maximum_known) {
 #pragma unroll
-        for (int a = 0; a < AHEAD; ++a) {
+            for (int a = 0; a < A; ++a) M = fmaxf(M, ml[a].x);
+        }
+        const float use = M == -INFINITY ? 0.f : M;
+#pragma unroll
+        for (int a = 0; a < A; ++a) {
             const float f = i0 + a < n ? __builtin_amdgcn_exp2f(ml[a].x - use) : 0.f;
             L += ml[a].y * f;
 #pragma unroll
             for (int e = 0; e < PER; ++e) acc[e] += v[a][e] * f;
         }
+    };
+    if (n <= 2) turn(0, std::integral_constant<int, 2>{}, false);
+    else {
+        for (int i = lane; i < n; i += 64) M = fmaxf(M, p.part_ml[slot_of(i)].x);
+        M = wave_max(M);
+        for (int i0 = 0; i0 < n; i0 += 8) turn(i0, std::integral_constant<int, 8>{}, true);
     }
+    const float use = M == -INFINITY ? 0.f : M;
     const float inv = L > 0.f || L != L ? 1.0f / L : 0.f;
     bf16_t* dst = p.out + (int64_t)row * p.o_ld + hq * D + lane * PER;
     if constexpr (PER == 2) *(uint32_t*)dst = pack_bf16x2(acc[0] * inv, acc[1] * inv);
@@ -558,15 +616,20 @@ struct Plan {
     int qp, qs;           // 16-row tiles of a shared and of an own item
     int chunk, chunks_p, chunks_s, slots;
     int64_t items;        // at most
-    int64_t at_parts, at_items, at_ml, at_o, bytes;
+    int64_t at_parts, at_plan, at_items, at_ml, at_o, bytes;
+    bool plain;
+    int tiles_s;
 };
 int tiles_for(int64_t rows) { return rows <= 16 ? 1 : 2; }
 Plan plan_for(const q3asr_kv_pages& c, const q3asr_attn_batch& b, int heads) {
     Plan r{};
     const int group = heads / c.kv_heads;
-    const bool shares = b.n_groups > 0 && b.max_shared >= c.page_tokens;
-    const int own = shares ? b.max_own : b.max_len;
     r.qs = tiles_for((int64_t)b.max_rows * group);
+    r.tiles_s = cdiv((int64_t)b.max_rows * group, 16 * r.qs);
+    // A small step is all latency: whole sequences as items that fit the device at once, shared or not, in one launch.
+    r.plain = b.max_len <= CHUNK_MAX && (int64_t)b.n * r.tiles_s * c.kv_heads <= PLAIN_ITEMS;
+    const bool shares = !r.plain && b.n_groups > 0 && b.max_shared >= c.page_tokens;
+    const int own = shares ? b.max_own : b.max_len;
     r.qp = shares ? std::max(r.qs, tiles_for((int64_t)b.max_group_rows * group)) : r.qs;
     // About three items per workgroup of a full device: fewer and larger items have less to join and less that begins and ends, more
     // and smaller ones spread a few long sequences over the device.
@@ -577,9 +640,18 @@ Plan plan_for(const q3asr_kv_pages& c, const q3asr_attn_batch& b, int heads) {
     r.slots = r.chunks_p + r.chunks_s;
     r.items = (shares ? (int64_t)b.n_groups * r.chunks_p * cdiv((int64_t)b.max_group_rows * group, 16 * r.qp) : 0) +
               (int64_t)b.n * r.chunks_s * cdiv((int64_t)b.max_rows * group, 16 * r.qs);
+    if (r.plain) {
+        r.chunk = CHUNK_MAX;
+        r.chunks_p = 0;
+        r.chunks_s = r.slots = 1;
+        r.qp = r.qs;
+        r.items = (int64_t)b.n * r.tiles_s;
+        return r;
+    }
     auto round = [](int64_t x) { return (x + 255) & ~255ll; };
     r.at_parts = 256;
-    r.at_items = r.at_parts + round((int64_t)b.rows * 4);
+    r.at_plan = r.at_parts + round((int64_t)b.rows * 4);
+    r.at_items = r.at_plan + (b.n > HELD || b.n_groups > HELD ? round((int64_t)b.n * (int64_t)sizeof(Entry) + (int64_t)b.n_groups * 4) : 0);
     r.at_ml = r.at_items + round(r.items * (int64_t)sizeof(Item));
     r.at_o = r.at_ml + (r.slots > 1 ? round((int64_t)b.rows * heads * r.slots * 8) : 0);
     r.bytes = r.at_o + (r.slots > 1 ? round((int64_t)b.rows * heads * r.slots * c.head_dim * 4) : 0);
@@ -589,9 +661,11 @@ Plan plan_for(const q3asr_kv_pages& c, const q3asr_attn_batch& b, int heads) {
 template <int D>
 void launch_d(const AttnParams& p, const Plan& r, hipStream_t s) {
     const dim3 block(256);
-    hipLaunchKernelGGL(paged_attn_plan_kernel, dim3(1), dim3(PLAN), 0, s, p);
-    HIP_CHECK(hipGetLastError());
-    const dim3 grid((int)std::min<int64_t>(r.items * p.kv_heads, CUS * (D == 64 || r.qp == 1 ? 3 : 2)));
+    if (!r.plain) {
+        hipLaunchKernelGGL(paged_attn_plan_kernel, dim3(1), dim3(PLAN), 0, s, p);
+        HIP_CHECK(hipGetLastError());
+    }
+    const dim3 grid((int)std::min<int64_t>(r.items * p.kv_heads, CUS * (D == 64 || r.qp == 1 ? 3 : 2)) + (r.plain && p.n_groups > 0));
     switch (r.qp * 10 + r.qs) {
         case 11: hipLaunchKernelGGL((paged_attn_kernel<D, 1, 1>), grid, block, 0, s, p); break;
         case 21: hipLaunchKernelGGL((paged_attn_kernel<D, 2, 1>), grid, block, 0, s, p); break;
@@ -621,7 +695,7 @@ void launch_paged_attention(const q3asr_kv_pages& c, int layer, const bf16_t* q,
     p.seqs = b.seqs; p.cu_rows = b.cu_rows; p.cu_groups = b.cu_groups; p.shared = b.shared;
     p.max_seqs = c.max_seqs; p.max_seq_pages = c.max_seq_pages; p.pages = c.pages;
     while ((1 << p.pt_shift) < c.page_tokens) ++p.pt_shift;
-    const bool shares = r.chunks_p > 0;
+    const bool shares = b.n_groups > 0 && b.max_shared >= c.page_tokens;
     p.n = b.n; p.rows = b.rows; p.n_groups = shares ? b.n_groups : 0;
     p.heads = heads; p.kv_heads = c.kv_heads; p.group = heads / c.kv_heads;
     p.max_rows = b.max_rows; p.max_group_rows = b.max_group_rows; p.max_len = b.max_len;
@@ -631,7 +705,10 @@ void launch_paged_attention(const q3asr_kv_pages& c, int layer, const bf16_t* q,
     p.chunk = r.chunk; p.chunks_p = r.chunks_p; p.chunks_s = r.chunks_s; p.slots = r.slots;
     p.rows_p = 16 * r.qp; p.rows_s = 16 * r.qs;
     char* ws = (char*)workspace;
+    p.plain = r.plain;
+    p.tiles_s = r.tiles_s;
     p.count = (int*)ws;
+    p.plan_ws = ws + r.at_plan;
     p.parts = (int*)(ws + r.at_parts);
     p.items = (Item*)(ws + r.at_items);
     p.part_ml = (float2*)(ws + r.at_ml);

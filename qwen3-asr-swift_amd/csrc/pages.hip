@@ -356,14 +356,19 @@ __global__ __launch_bounds__(256) void pages_copy_kernel(Pages p) {
 __global__ __launch_bounds__(256) void pages_write_kernel(Pages p, int layer, const bf16_t* k, int64_t k_ld, const bf16_t* v, int64_t v_ld,
                                                           const int* seqs, const int* cu_rows, int n, int rows) {
     const int row = blockIdx.x, tid = threadIdx.x;
-    // the entry of the list that the row belongs to
-    int lo = 0, hi = n;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (cu_rows[mid] <= row) lo = mid;
-        else hi = mid;
+    // the entry of the list that the row belongs to: the row's own number where every sequence has one row, else by halving
+    int lo = min(row, n - 1), r0 = cu_rows[lo], r1 = cu_rows[lo + 1];
+    if (row < r0 || row >= r1) {
+        lo = 0;
+        int hi = n;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (cu_rows[mid] <= row) lo = mid;
+            else hi = mid;
+        }
+        r0 = cu_rows[lo];
+        r1 = cu_rows[lo + 1];
     }
-    const int r0 = cu_rows[lo], r1 = cu_rows[lo + 1];
     if (row < r0 || row >= r1 || r1 > rows) {
         if (tid == 0) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, lo);
         return;

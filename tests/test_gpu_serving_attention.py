@@ -19,7 +19,7 @@ class Step:
         members = [m for _, ms in groups for m in ms]
         n = len(members)
         lens = [s + own for s, ms in groups for own, _ in ms]
-        width = max(1, -(-max(lens) // pg)) + 1
+        width = max(1, -(-max(max(lens), 1040) // pg)) + 1
         pages = sum(-(-x // pg) + 1 for x in lens) + sum(s // pg + 2 for s, _ in groups) + 3
         self.c = c = Cache(dev, model, seqs=n + len(groups), width=width, pages=pages, layers=layers, heads=kv, dim=dim, pg=pg, seed=seed, poison=poison)
         # every group grows from a base sequence, pages scattered over the pool by a few that come and go
@@ -117,6 +117,9 @@ def test_attention_matches_fp64(tiny_model, g, heads, kv, dim, pg):
         s = Step(dev, tiny_model[0], GROUPS[g], heads, kv, dim, pg, seed=g)
         s.check(*s.run(s.batch(), pad=8 * (g % 2), extra_rows=1))
         s.check(*s.run(s.batch(grouped=False)))
+        # a bound above 1024 tokens takes small steps, too, through the plan and the parts
+        s.check(*s.run(s.batch(max_len=max(1040, max(s.lens))), pad=8, extra_rows=2))
+        s.check(*s.run(s.batch(grouped=False, max_len=max(1040, max(s.lens)))))
         if g in (2, 5):      # bounds above what the batch needs, another scale, sharp rows, no lse
             m = (s.c.width - 1) * s.c.book.pg
             s.check(*s.run(s.batch(max_len=m, max_shared=m, max_own=m, max_group_rows=s.cu[-1])))
@@ -133,7 +136,7 @@ def test_rows_without_keys_are_zero(tiny_model):
         # sequence 0: no token, one row; sequence 1: no token, two rows
         s.rows, s.cu = [1, 2, 1], [0, 1, 3, 4]
         s.q = bf16_bits(s.rng.standard_normal((4, 512)))
-        for b in (s.batch(), s.batch(grouped=False)):
+        for b in (s.batch(), s.batch(grouped=False), s.batch(max_len=1040), s.batch(grouped=False, max_len=1040)):
             out, lse = s.run(b)
             s.check(out, lse)
             assert (out[:3] == 0).all() and (lse[:3] == -np.inf).all()
@@ -143,9 +146,11 @@ def test_extreme_scores(tiny_model):
     """One key far above the others in the last and in the first place, equal scores everywhere, scores of thousands."""
     with Device() as dev:
         s = Step(dev, tiny_model[0], [(100, [(60, 2), (9, 1)])], 4, 2, 128, 16, seed=4, spread=30.0)
-        s.check(*s.run(s.batch()))
+        for b in (s.batch(), s.batch(max_len=1040)):
+            s.check(*s.run(b))
         s.q[:] = 0                       # a flat softmax
-        s.check(*s.run(s.batch()))
+        for b in (s.batch(), s.batch(max_len=1040)):
+            s.check(*s.run(b))
 
 
 @pytest.mark.parametrize("dim,kv", [(128, 8), (64, 2)])
@@ -195,11 +200,14 @@ def test_wrong_batches_are_reported(tiny_model):
                 over = {}
             if over.get("max_len") == 80:
                 over.update(max_shared=64, max_own=80)
-            with pytest.raises(Q3Error):
-                s.run(s.batch(**over))
-            st = dev.stream()
-            s.run(s.batch(**over), stream=st)
-            assert s.c.c.status(stream=st)[0] == code, over
+            for planned in ({}, dict(max_len=1040)):
+                if "max_len" in over and planned:
+                    continue
+                with pytest.raises(Q3Error):
+                    s.run(s.batch(**over, **planned))
+                st = dev.stream()
+                s.run(s.batch(**over, **planned), stream=st)
+                assert s.c.c.status(stream=st)[0] == code, (over, planned)
         s.c.put()
         s.check(*s.run(s.batch()))
         b = s.batch(max_rows=0)
