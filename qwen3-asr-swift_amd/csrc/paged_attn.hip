@@ -1,18 +1,22 @@
 // Attention over the paged KV cache for sequences that share prefixes (gfx950).
 //
-// o = sum_j p_j v_j, p = softmax_j(scale q . k_j).  The keys of a sequence are cut into its group's shared pages and its own
-// pages, and both into chunks; a work item is one chunk for one KV head and up to 16 * QT of the query rows that read it -- of
-// every sequence of the group for a shared chunk, so that a shared key crosses HBM once per group -- and leaves (max, sum,
-// weighted sum of values) per row.  Three launches: one workgroup plans the items from the lengths and tables on the device,
-// sorted by size; a grid that fills the device once works them off; a last one joins the parts of the rows that have several.
-// Both softmax statistics and the sums stay in fp32; the probabilities are rounded to bf16 for the matrix cores (2^-9 relative
-// each on average, which averages out over the keys of a row).
+// o = sum_j p_j v_j, p = softmax_j(scale q . k_j).  The keys of a sequence are its group's shared pages and its own pages; all query
+// rows that read a shared key -- of every sequence of the group, with all query heads of the KV head -- are columns of one matrix
+// product, so that a shared key crosses HBM once per group.  Partial results (max, sum, weighted sum of values) are joined per
+// row.  Both softmax statistics and the sums stay in fp32; the probabilities are rounded to bf16 for the matrix cores (at most
+// 2^-8 relative each, which averages out over the keys of a row).
 //
-// HBM-bound: with G query heads per KV head and H hypotheses a shared chunk is 16 * QT columns of a matrix product against
-// 2 * head_dim * 2 bytes per key.  Four waves take tiles of 32 keys in turn, each with its own statistics: S^T = K Q^T with the K
-// rows loaded from memory as MFMA A fragments, then O^T = V^T P^T, where the exponentiated scores are as they stand the B
-// fragment and the V rows reach the A fragments through transposing reads of a wave's own LDS tile.  A workgroup requests the
-// next item's first tile before it joins its waves' results, and that item's page numbers an item ahead.
+// HBM-bound: 2 * head_dim * 2 bytes per key and KV head against 16 * QT columns.  A wave works on tiles of 32 keys: the K rows,
+// loaded whole, become MFMA A fragments of S^T = K Q^T through an LDS tile of the wave's own; the exponentiated scores are as
+// they stand the B fragment of O^T = V^T P^T, whose A fragments are transposing reads of the V rows in the same LDS tile.  The
+// next tile's rows are requested as soon as this one's have left their registers.
+//
+//   plain   few rows: a workgroup per sequence and KV head, its four waves taking tiles in turn; one launch, nothing shared
+//   stream  the tiles of all sequences and groups in one row, cut into equal parts, one per wave of a full device: no wave waits for
+//           another, and each has a tile in flight all the time.  Three launches: a plan (one workgroup: lengths -> where every
+//           sequence's tiles begin), the waves, and the join of what was cut.
+// Measured against 4-wave work items of up to 1024 keys, sorted by size: rounding to four tiles and joining cost 1.2 to 1.4 times
+// the mean load there.
 #include "paged.h"
 #include "prof.h"
 #include <algorithm>
@@ -24,11 +28,9 @@ typedef __attribute__((ext_vector_type(4))) short s16x4;
 
 namespace {
 
-constexpr int WAVES = 4, PLAN = 1024;
-constexpr int CHUNK_MAX = 1024;                   // keys: one page number per lane and 16 keys
-constexpr int BUCKETS = CHUNK_MAX / 32 + 1;       // items by their number of 32-key tiles; at most 64
-constexpr int BATCH = 64;                         // items whose descriptions a workgroup holds at a time
-constexpr int CUS = 256, PLAIN_ITEMS = 512;
+constexpr int WAVES = 4, PLAN = 1024, CUS = 256;
+constexpr int STREAM_WAVES = CUS * 2 * WAVES;     // two workgroups per CU
+constexpr int PLAIN_ITEMS = 512, PLAIN_KEYS = 1024;
 
 union Frag {
     bf16x8 v;
@@ -49,7 +51,6 @@ __device__ __forceinline__ float rows_sum(float x) {
     const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return __uint_as_float(h[0]) + __uint_as_float(h[1]);
 }
-
 // LDS written by some lanes of a wave is read by others behind this.
 __device__ __forceinline__ void wave_lds_fence() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -57,15 +58,22 @@ __device__ __forceinline__ void wave_lds_fence() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// A chunk of keys for up to 16 * QT query rows: row r of M is row r0 + r / group of the step, head kvh * group + r % group, and
-// sees keys below `limit` + r / group of an own chunk, all keys of a shared one.
-struct __attribute__((aligned(16))) Item {
-    int r0, M, first;   // first: the lowest r
-    int seq, k0, k1;    // keys [k0, k1) of the pages of sequence seq
-    int limit;          // SHARED: a shared chunk
-    int slot;           // where the part goes; DIRECT: it is the rows' only one and goes to the output
+// Query rows that read the same keys: row r of M is row r0 + r / group of the step, head kvh * group + r % group.  They read keys
+// [k0, k1) of the pages of sequence seq, row r those below limit + r / group (SHARED: all of them).
+struct __attribute__((aligned(16))) Segment {
+    int r0, M, seq, k0, k1, limit;
+    int start;    // first tile in the row of all tiles; tile t of query tile q and KV head h is start + (q * kv_heads + h) * ntiles + t
+    int whole;    // 1: its rows read nothing else
 };
-constexpr int SHARED = 0x7fffffff, DIRECT = -1;
+constexpr int SHARED = 0x7fffffff;
+// Where a row's parts are: tiles of its group's and of its own segment (0: none), their starts and first rows.
+struct __attribute__((aligned(16))) RowParts {
+    int start[2], tiles[2], r0[2];
+    int known, pad;
+};
+struct __attribute__((aligned(16))) Total {
+    int tiles, per, segments, pad;   // per: tiles of a wave
+};
 
 struct AttnParams {
     const bf16_t* q; int64_t q_ld;
@@ -79,18 +87,17 @@ struct AttnParams {
     int n, rows, n_groups, heads, kv_heads, group;
     int max_rows, max_group_rows, max_len, max_own, max_shared;
     float scale_log2;
-    int chunk, chunks_p, chunks_s, slots, rows_p, rows_s;   // shared chunks' slots first, then own ones'; query rows of an item
-    int plain;                                 // no plan: own items of whole sequences, tiles_s each
-    int tiles_s;
+    int rows_q;                                // query rows of a wave: 16 * QT
+    int tiles_q;                               // plain: query tiles of a sequence
+    int per_min, slots_p, slots;               // parts of a row at most: of its group's segment first
+    Total* total;
     void* plan_ws;                             // what of a plan does not fit LDS
-    int* count;                                // [1] items
-    int* parts;                                // [rows] parts of a row: shared | own << 16
-    Item* items;
+    Segment* segments;
+    RowParts* parts;                           // [rows]
     float2* part_ml;                           // [rows][heads][slots]: maximum (base 2), sum
     float* part_o;                             // [rows][heads][slots][D]
 };
 
-// ---- plan ----
 struct Entry {             // a sequence of the step
     int seq, r0, T, len;
     bool ok;
@@ -112,112 +119,112 @@ __device__ __forceinline__ Entry entry_of(const AttnParams& p, int i, bool repor
     return e;
 }
 
+// ---- plan ----
 // Two dependent loads per sequence (its number, its length), everything else from LDS: with one workgroup nothing covers latency.
 // Lists beyond HELD entries or groups stay in the workspace.
 constexpr int HELD = 1024;
 __global__ __launch_bounds__(PLAN) void paged_attn_plan_kernel(AttnParams p) {
-    __shared__ int bucket[64];
     __shared__ Entry held[HELD];
-    __shared__ int held_cu[HELD + 1], held_from[HELD];
+    __shared__ int held_cu[HELD + 1], held_from[HELD], held_rows[HELD + 1], scan[PLAN / 64];
     const int tid = threadIdx.x;
     Entry* const entry = p.n <= HELD ? held : (Entry*)p.plan_ws;
     int* const from = p.n_groups <= HELD ? held_from : (int*)((Entry*)p.plan_ws + p.n);   // tokens that a group shares
     const int* const cu = p.n_groups <= HELD ? held_cu : p.cu_groups;
-    if (tid < 64) bucket[tid] = 0;
-    for (int r = tid; r < p.rows; r += PLAN) p.parts[r] = 0;
-    for (int i = tid; i < p.n; i += PLAN) entry[i] = entry_of(p, i, true);
+    const int* const cu_rows = p.n <= HELD ? held_rows : p.cu_rows;
+    for (int r = tid; r < p.rows; r += PLAN) p.parts[r].known = 0;
     if (p.n_groups > 0 && p.n_groups <= HELD)
         for (int g = tid; g <= p.n_groups; g += PLAN) held_cu[g] = p.cu_groups[g];
+    for (int g = tid; g < p.n_groups; g += PLAN) from[g] = p.shared[g];
+    if (p.n <= HELD)
+        for (int i = tid; i <= p.n; i += PLAN) held_rows[i] = p.cu_rows[i];
+    for (int i = tid; i < p.n; i += PLAN) entry[i] = entry_of(p, i, true);
     __syncthreads();
     for (int g = tid; g < p.n_groups; g += PLAN) {
-        const int i0 = cu[g], i1 = cu[g + 1], shared = p.shared[g];
+        const int i0 = cu[g], i1 = cu[g + 1], shared = from[g];
         from[g] = 0;
         if (i0 < 0 || i1 < i0 || i1 > p.n) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, g);
         else if (i1 > i0) {
             const Entry first = entry[i0];
-            const int end = p.cu_rows[i1];
-            if (shared > p.max_shared || (first.ok && (end < first.r0 || end > p.rows || end - first.r0 > p.max_group_rows)))
-                pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, i0);
-            from[g] = max(0, min(min(shared, p.max_shared), first.len - first.T)) >> p.pt_shift << p.pt_shift;
+            const int end = cu_rows[i1];
+            const bool fits = end >= first.r0 && end <= p.rows && end - first.r0 <= p.max_group_rows;
+            if (shared > p.max_shared || (first.ok && !fits)) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, i0);
+            if (first.ok && fits) from[g] = max(0, min(min(shared, p.max_shared), first.len - first.T)) >> p.pt_shift << p.pt_shift;
         }
     }
     __syncthreads();
-    // the items of group g (which = g) or sequence i (which = n_groups + i), in any order: f(item)
-    auto items_of = [&](int which, bool report, auto f) {
-        Item it;
-        if (which < p.n_groups) {
-            const int i0 = cu[which], i1 = cu[which + 1], keys = from[which];
-            if (i0 < 0 || i1 <= i0 || i1 > p.n) return;
-            const Entry first = entry[i0];
-            const int end = min(p.cu_rows[i1], first.r0 + p.max_group_rows);
-            if (!first.ok || end > p.rows) return;
-            it.r0 = first.r0;
-            it.M = max(0, end - first.r0) * p.group;
-            it.seq = first.seq;
-            it.limit = SHARED;
-            for (int ch = 0; ch * p.chunk < keys; ++ch)
-                for (it.first = 0; it.first < it.M; it.first += p.rows_p) {
-                    it.k0 = ch * p.chunk;
-                    it.k1 = min(keys, it.k0 + p.chunk);
-                    it.slot = ch;
-                    f(it);
-                }
-            return;
-        }
-        const int i = which - p.n_groups;
-        const Entry e = entry[i];
-        int behind = 0;    // keys before it are read by the group
-        bool ok = e.ok;
-        if (p.n_groups > 0) {
-            int lo = 0, hi = p.n_groups;   // the last group that begins at or before entry i
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (cu[mid] <= i) lo = mid;
-                else hi = mid;
-            }
-            const int i0 = cu[lo], i1 = cu[lo + 1];
-            if (i0 >= 0 && i >= i0 && i < i1 && i1 <= p.n) {
-                behind = from[lo];
-                ok = ok && entry[i0].ok;
-            } else if (report) {
-                pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, i);
-            }
-        }
-        if (report && ok && (behind > max(0, e.len - e.T) || e.len - behind > p.max_own)) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, i);
-        const int own = min(max(0, e.len - behind), p.chunks_s * p.chunk), parts_p = (behind + p.chunk - 1) / p.chunk;
-        const int parts_s = max((own + p.chunk - 1) / p.chunk, parts_p ? 0 : 1);   // a row without keys has one empty part
-        it.r0 = e.r0;
-        it.M = e.T * p.group;
-        it.seq = e.seq;
-        it.limit = e.len - e.T + 1;
-        if (report)
-            for (int t = 0; t < e.T; ++t) p.parts[e.r0 + t] = parts_p | parts_s << 16;
-        for (int ch = 0; ch < parts_s; ++ch)
-            for (it.first = 0; it.first < it.M; it.first += p.rows_s) {
-                it.k0 = behind + ch * p.chunk;
-                it.k1 = min(behind + own, it.k0 + p.chunk);
-                it.slot = parts_p + parts_s == 1 ? DIRECT : p.chunks_p + ch;
-                f(it);
-            }
-    };
-    // the largest first, so that the last items to be taken up are small
-    auto bucket_of = [](const Item& it) { return BUCKETS - 1 - ((it.k1 - it.k0 + 31) >> 5); };
+    // segments: the groups', then the sequences'
     const int all = p.n_groups + p.n;
-    for (int w = tid; w < all; w += PLAN) items_of(w, true, [&](const Item& it) { atomicAdd(&bucket[bucket_of(it)], 1); });
-    __syncthreads();
-    if (tid < 64) {
-        const int n = bucket[tid];
-        int x = n;
+    int carry = 0;
+    for (int w0 = 0; w0 < all; w0 += PLAN) {
+        const int w = w0 + tid;
+        Segment sg{};
+        int g = -1, count = 0;
+        Entry e{};
+        if (w < p.n_groups) {
+            if (from[w] > 0) {   // a group without sequences or with wrong ones shares nothing
+                const Entry first = entry[cu[w]];
+                sg = Segment{first.r0, (cu_rows[cu[w + 1]] - first.r0) * p.group, first.seq, 0, from[w], SHARED, 0, 0};
+            }
+        } else if (w < all) {
+            const int i = w - p.n_groups;
+            e = entry[i];
+            int behind = 0;      // keys before it are read by the group
+            bool ok = e.ok;
+            if (p.n_groups > 0) {
+                int lo = 0, hi = p.n_groups;   // the last group that begins at or before entry i
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) >> 1;
+                    if (cu[mid] <= i) lo = mid;
+                    else hi = mid;
+                }
+                const int i0 = cu[lo], i1 = cu[lo + 1];
+                if (i0 >= 0 && i >= i0 && i < i1 && i1 <= p.n) {
+                    g = lo;
+                    behind = from[lo];
+                    ok = ok && entry[i0].ok;
+                } else {
+                    pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, i);
+                }
+            }
+            if (ok && (behind > max(0, e.len - e.T) || e.len - behind > p.max_own)) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, i);
+            sg = Segment{e.r0, e.T * p.group, e.seq, behind, behind + min(max(0, e.len - behind), p.max_own), e.len - e.T + 1, 0, behind == 0};
+        }
+        const int tiles = (sg.k1 - sg.k0 + 31) >> 5;
+        count = tiles * ((sg.M + p.rows_q - 1) / p.rows_q) * p.kv_heads;
+        // exclusive prefix sum
+        const int lane = tid & 63, wave = tid >> 6;
+        int x = count;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
             const int t = __shfl_up(x, o, 64);
-            if (tid >= o) x += t;
+            if (lane >= o) x += t;
         }
-        bucket[tid] = x - n;
-        if (tid == 63) *p.count = x;
+        if (lane == 63) scan[wave] = x;
+        __syncthreads();
+        int before = carry;
+        for (int v = 0; v < PLAN / 64; ++v) {
+            before += v < wave ? scan[v] : 0;
+            carry += scan[v];
+        }
+        sg.start = before + x - count;
+        if (w < all) p.segments[w] = sg;
+        __syncthreads();   // scan is written again; the groups' segments are read below
+        if (w >= p.n_groups && w < all) {
+            RowParts rp{};
+            if (g >= 0 && from[g] > 0) {
+                const Segment& sh = p.segments[g];
+                rp.start[0] = sh.start;
+                rp.tiles[0] = (sh.k1 - sh.k0 + 31) >> 5;
+                rp.r0[0] = sh.r0;
+            }
+            rp.start[1] = sg.start;
+            rp.tiles[1] = tiles;
+            rp.r0[1] = sg.r0;
+            rp.known = 1;
+            for (int t = 0; t < e.T; ++t) p.parts[e.r0 + t] = rp;
+        }
     }
-    __syncthreads();
-    for (int w = tid; w < all; w += PLAN) items_of(w, false, [&](const Item& it) { p.items[atomicAdd(&bucket[bucket_of(it)], 1)] = it; });
+    if (tid == 0) *p.total = Total{carry, max(p.per_min, (carry + STREAM_WAVES - 1) / STREAM_WAVES), all, 0};
 }
 
 // Without a plan the groups are not used; a workgroup of its own checks them all the same.
@@ -240,124 +247,81 @@ __device__ void check_groups(const AttnParams& p) {
     }
 }
 
+// ---- a wave's work ----
 template <int D>
-struct Lds {
-    static constexpr int KROW = 2 * D + 16, VROW = 2 * D + 32, OROW = D + 4;   // padded: fragment and transposing reads meet all banks
-    static constexpr int V_BYTES = WAVES * 32 * VROW, O_BYTES = WAVES * 16 * OROW * 4;
-    static constexpr int BYTES = V_BYTES > O_BYTES ? V_BYTES : O_BYTES;
+struct Rows {
+    static constexpr int KROW = 2 * D + 16, VROW = 2 * D + 32;   // padded: fragment and transposing reads meet all banks
+    static constexpr int TILE = 32 * VROW;
 };
 
-// A wave's registers that carry over from one item to the next.
-template <int D, int QMAX>
-struct Stream {
-    static constexpr int NKS = D / 32, LPR = D / 8, RPI = 64 / LPR, IV = 16 / RPI, NQ = (16 * QMAX * LPR + 255) / 256;
-    Frag kf[2][IV], vf[2][IV];    // a tile of 32 keys, as rows
-    uint4 qv[NQ];                 // the thread's pieces of the item's query rows, on their way to LDS
-    int ids;                      // page numbers of the item's chunk, 16 keys per lane
-
+template <int D, int QT>
+struct Wave {
+    static constexpr int NKS = D / 32, NDT = D / 16, LPR = D / 8, RPI = 64 / LPR, IV = 16 / RPI;
+    static constexpr int KROW = Rows<D>::KROW, VROW = Rows<D>::VROW;
     const AttnParams& p;
     const int lane, li, lg;
-    int k0, nsub;
-    int64_t head;
-    __device__ Stream(const AttnParams& p_, int lane_) : p(p_), lane(lane_), li(lane_ & 15), lg(lane_ >> 4) {}
+    char* const tile;             // the wave's LDS
+    Frag kf[2][IV], vf[2][IV];    // 32 keys, as rows
+    Frag qf[QT][NKS];             // queries as B fragments: lane (li, lg) holds values 32 ks + 8 lg .. of query 16 qt + li
+    int limit[QT];                // the lane's queries see keys below
+    int lowest;                   // keys below it are seen by all of them
+    float m[QT], l[QT];           // l: of this lane's keys only, until the end
+    f32x4 o[QT][NDT];             // lane (li, lg) holds values 16 dt + 4 lg .. of query 16 qt + li
+    int ids, id_base;             // page numbers of 64 times 16 keys from key id_base on, one per lane
+    __device__ Wave(const AttnParams& p_, char* tile_) : p(p_), lane(threadIdx.x & 63), li(threadIdx.x & 15), lg((threadIdx.x & 63) >> 4), tile(tile_) {}
 
-    __device__ int page_numbers(int seq, int k0_, int k1_) const {
-        const int n = (k1_ - k0_ + 15) >> 4;
-        if (n <= 0) return 0;
-        return p.table[(int64_t)seq * p.max_seq_pages + ((k0_ + 16 * min(lane, n - 1)) >> p.pt_shift)];
-    }
-    __device__ void begin(int ids_, int kvh, int k0_, int k1_) {
-        k0 = k0_;
-        nsub = (k1_ - k0_ + 15) >> 4;
-        head = (int64_t)kvh * p.head_stride;
-        ids = ids_;
+    __device__ void page_numbers(int seq, int base, int k1) {
+        id_base = base;
+        const int key = min(base + 16 * lane, k1 - 1);
+        ids = p.table[(int64_t)seq * p.max_seq_pages + (key >> p.pt_shift)];
         if ((unsigned)ids >= (unsigned)p.pages) {
-            if (nsub > 0) pages_error(p.status, Q3ASR_PAGES_BAD_INDEX, 0);
+            pages_error(p.status, Q3ASR_PAGES_BAD_INDEX, 0);
             ids = 0;
         }
     }
-    __device__ void load_q(const Item& it, int kvh, int most) {
-#pragma unroll
-        for (int i = 0; i < NQ; ++i) {
-            const int idx = threadIdx.x + 256 * i, in = idx / LPR, r = it.first + in;
-            qv[i] = make_uint4(0, 0, 0, 0);
-            if (in < most && r < it.M) {
-                const int tok = r / p.group;
-                qv[i] = *(const uint4*)(p.q + (int64_t)(it.r0 + tok) * p.q_ld + (kvh * p.group + r - tok * p.group) * D + 8 * (idx % LPR));
-            }
-        }
+    __device__ int64_t base_of(int64_t head, int key, int k1) const {   // 16 keys; those behind the last 16 are read from these
+        const int at = min(key, (k1 - 1) & ~15);
+        const int64_t page = __builtin_amdgcn_readlane(ids, (at - id_base) >> 4);
+        return page * p.page_stride + head + (int64_t)(at & ((1 << p.pt_shift) - 1)) * D;
     }
-    __device__ void store_q(char* sq) const {
-#pragma unroll
-        for (int i = 0; i < NQ; ++i) {
-            const int idx = threadIdx.x + 256 * i, in = idx / LPR;
-            if (in < 16 * QMAX) *(uint4*)(sq + in * (2 * D + 16) + 16 * (idx % LPR)) = qv[i];
-        }
-    }
-    __device__ int64_t base_of(int t, int h) const {   // first value of 16 keys; those behind the last are read from the last's
-        const int sub = min(2 * t + h, nsub - 1);
-        const int64_t page = __builtin_amdgcn_readlane(ids, sub);
-        return page * p.page_stride + head + (int64_t)((k0 + 16 * sub) & ((1 << p.pt_shift) - 1)) * D;
-    }
-    // 32 keys of K or V as whole rows, RPI of them per instruction
-    __device__ void load(const bf16_t* pool, Frag (&x)[2][IV], int t) const {
+    __device__ void load(const bf16_t* pool, Frag (&x)[2][IV], int64_t head, int kv0, int k1) const {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const bf16_t* src = pool + base_of(t, h) + (lane / LPR) * D + 8 * (lane % LPR);
+            const bf16_t* src = pool + base_of(head, kv0 + 16 * h, k1) + (lane / LPR) * D + 8 * (lane % LPR);
 #pragma unroll
             for (int i = 0; i < IV; ++i) x[h][i].v = __builtin_nontemporal_load((const bf16x8*)(src + i * RPI * D));
         }
     }
-    __device__ void load_k(int t) { load(p.K, kf, t); }
-    __device__ void load_v(int t) { load(p.V, vf, t); }
-};
-
-// One item for one KV head; its first tile has been requested.  request_next: the same for the next one, which a single group of
-// queries leaves registers for before the join.
-template <int D, int QT, int QMAX, class F>
-__device__ __forceinline__ void attend(const AttnParams& p, const Item& it, int kvh, Stream<D, QMAX>& st, char* lds, char* sq, float (*sm_m)[64],
-                                       float (*sm_l)[64], F request_next) {
-    constexpr int NKS = D / 32, NDT = D / 16, LPR = D / 8, RPI = 64 / LPR, IV = 16 / RPI;
-    constexpr int KROW = Lds<D>::KROW, VROW = Lds<D>::VROW, OROW = Lds<D>::OROW;
-    const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int k0 = it.k0, k1 = it.k1, ntiles = (k1 - k0 + 31) >> 5;
-    int t = wave;
-
-    int limit[QT];
+    __device__ void queries(const Segment& sg, int first, int kvh) {
 #pragma unroll
-    for (int qt = 0; qt < QT; ++qt) {
-        const int r = it.first + 16 * qt + li;
-        limit[qt] = r >= it.M ? 0 : it.limit == SHARED ? k1 : min(k1, it.limit + r / p.group);
+        for (int qt = 0; qt < QT; ++qt) {
+            const int r = first + 16 * qt + li;
+            const bool ok = r < sg.M;
+            const int tok = (ok ? r : 0) / p.group;
+            limit[qt] = !ok ? 0 : sg.limit == SHARED ? sg.k1 : min(sg.k1, sg.limit + tok);
+            const bf16_t* src = p.q + (int64_t)(sg.r0 + tok) * p.q_ld + (kvh * p.group + (ok ? r - tok * p.group : 0)) * D + 8 * lg;
+#pragma unroll
+            for (int ks = 0; ks < NKS; ++ks) qf[qt][ks].u = *(const uint4*)(src + 32 * ks);
+            m[qt] = -INFINITY;
+            l[qt] = 0.f;
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt) o[qt][dt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        }
+        lowest = min(sg.k1, sg.limit);
     }
-    // queries as B fragments: lane (li, lg) reads values 32 ks + 8 lg .. of query li
-    const char* const qr = sq + li * (2 * D + 16) + 16 * lg;
-    const int lowest = min(k1, it.limit);   // keys below it are seen by all rows
-
-    float m[QT], l[QT];
-    f32x4 o[QT][NDT];
-#pragma unroll
-    for (int qt = 0; qt < QT; ++qt) {
-        m[qt] = -INFINITY;
-        l[qt] = 0.f;
-#pragma unroll
-        for (int dt = 0; dt < NDT; ++dt) o[qt][dt] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    }
-    char* const vt = lds + wave * 32 * VROW;
-    char* const kw = vt + (lane / LPR) * KROW + 16 * (lane % LPR);
-    char* const vw = vt + (lane / LPR) * VROW + 16 * (lane % LPR);
-    const char* const kr = vt + li * KROW + 16 * lg;
-    // transposing reads: per 16 lanes a block of 4 keys x 16 dims, lane 4 a + b addresses key a, dims 4 b .. 4 b + 3
-    const char* const vr = vt + (4 * lg + (li >> 2)) * VROW + (li & 3) * 8;
-
-    auto tile = [&](auto last) {
-        constexpr bool LAST = decltype(last)::value;
-        const int kv0 = k0 + 32 * t;
+    // The tile of keys kv0 .. whose rows are in kf and vf; next_k and next_v request the next tile's once these are free.
+    template <class NK, class NV>
+    __device__ void step(int kv0, int k1, NK next_k, NV next_v) {
+        char* const kw = tile + (lane / LPR) * KROW + 16 * (lane % LPR);
+        char* const vw = tile + (lane / LPR) * VROW + 16 * (lane % LPR);
+        const char* const kr = tile + li * KROW + 16 * lg;
+        // transposing reads: per 16 lanes a block of 4 keys x 16 dims, lane 4 a + b addresses key a, dims 4 b .. 4 b + 3
+        const char* const vr = tile + (4 * lg + (li >> 2)) * VROW + (li & 3) * 8;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int i = 0; i < IV; ++i) *(uint4*)(kw + (16 * h + i * RPI) * KROW) = st.kf[h][i].u;
-        if constexpr (!LAST) st.load_k(t + WAVES);
+            for (int i = 0; i < IV; ++i) *(uint4*)(kw + (16 * h + i * RPI) * KROW) = kf[h][i].u;
+        next_k();
         wave_lds_fence();
         Frag ka[2][NKS];   // K rows as A fragments: lane (li, lg) reads values 32 ks + 8 lg .. of key li
 #pragma unroll
@@ -369,20 +333,17 @@ __device__ __forceinline__ void attend(const AttnParams& p, const Item& it, int 
         bool moved = false;
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) {
-            Frag qf[NKS];
-#pragma unroll
-            for (int ks = 0; ks < NKS; ++ks) qf[ks].u = *(const uint4*)(qr + qt * 16 * (2 * D + 16) + 64 * ks);
             f32x4 s[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 s[h] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int ks = 0; ks < NKS; ++ks) s[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka[h][ks].v, qf[ks].v, s[h], 0, 0, 0);
+                for (int ks = 0; ks < NKS; ++ks) s[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka[h][ks].v, qf[qt][ks].v, s[h], 0, 0, 0);
             }
             float sv[8], top = -INFINITY;
 #pragma unroll
             for (int j = 0; j < 8; ++j) sv[j] = s[j >> 2][j & 3] * p.scale_log2;
-            if (kv0 + 32 > lowest) {   // the same for the whole workgroup's tile
+            if (kv0 + 32 > lowest) {   // wave-uniform
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                     if (kv0 + 16 * (j >> 2) + 4 * lg + (j & 3) >= limit[qt]) sv[j] = -INFINITY;
@@ -398,22 +359,25 @@ __device__ __forceinline__ void attend(const AttnParams& p, const Item& it, int 
                 pe[j] = __builtin_amdgcn_exp2f(sv[j] - m_use);
                 ps += pe[j];
             }
-            l[qt] = l[qt] * alpha[qt] + ps;   // this lane's keys only: the four rows of lanes are added at the end
+            l[qt] = l[qt] * alpha[qt] + ps;
             moved |= m_new != m[qt];
             m[qt] = m_new;
             pf[qt].u = make_uint4(pack_bf16x2(pe[0], pe[1]), pack_bf16x2(pe[2], pe[3]), pack_bf16x2(pe[4], pe[5]), pack_bf16x2(pe[6], pe[7]));
-            if constexpr (QT > 1) __builtin_amdgcn_sched_barrier(0);   // one group of queries' fragments in registers at a time
         }
         __builtin_amdgcn_wave_barrier();   // the V rows go where the K rows were
+        if (kv0 + 32 > k1) {
+            // what lies behind the last key may be anything: a NaN there would survive its zero weight
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < IV; ++i)
+                    if (kv0 + 16 * h + i * RPI + lane / LPR >= k1) vf[h][i].u = make_uint4(0, 0, 0, 0);
+        }
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int i = 0; i < IV; ++i) {
-                // what lies behind the last key may be anything: a NaN there would survive its zero weight
-                const bool keep = !LAST || kv0 + 16 * h + i * RPI + lane / LPR < k1;
-                *(uint4*)(vw + (16 * h + i * RPI) * VROW) = keep ? st.vf[h][i].u : make_uint4(0, 0, 0, 0);
-            }
-        if constexpr (!LAST) st.load_v(t + WAVES);
+            for (int i = 0; i < IV; ++i) *(uint4*)(vw + (16 * h + i * RPI) * VROW) = vf[h][i].u;
+        next_v();
         wave_lds_fence();
         if (__builtin_amdgcn_ballot_w64(moved) != 0) {
 #pragma unroll
@@ -433,143 +397,147 @@ __device__ __forceinline__ void attend(const AttnParams& p, const Item& it, int 
             for (int qt = 0; qt < QT; ++qt) o[qt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va.v, pf[qt].v, o[qt][dt], 0, 0, 0);
         }
         __builtin_amdgcn_wave_barrier();   // the next tile's rows are written after these reads
-    };
-    // a tile with a successor is full, and its loads of that successor are unconditional
-    if (t < ntiles) {
-        for (; t + WAVES < ntiles; t += WAVES) tile(std::false_type{});
-        tile(std::true_type{});
     }
+};
 
-    if constexpr (QT == 1) request_next();
-    // join the four waves, 16 queries at a time
-#pragma unroll
-    for (int qt = 0; qt < QT; ++qt) {
-        const float lt = rows_sum(l[qt]);
-        if (lg == 0) {
-            sm_m[wave][16 * qt + li] = m[qt];
-            sm_l[wave][16 * qt + li] = lt;
-        }
-    }
-    float* const so = (float*)lds;
-#pragma unroll
-    for (int qt = 0; qt < QT; ++qt) {
-        __syncthreads();
-        if (QT == 1) st.store_q(sq);   // the next item's: all waves are done with this one's
-#pragma unroll
-        for (int dt = 0; dt < NDT; ++dt) *(f32x4*)(so + (wave * 16 + li) * OROW + 16 * dt + 4 * lg) = o[qt][dt];
-        __syncthreads();
-        constexpr int PER = D / 16;   // values per thread
-        const int qi = tid >> 4, d0 = (tid & 15) * PER, r = it.first + 16 * qt + qi;
-        if (r < it.M) {
-            float M = -INFINITY, L = 0.f, acc[PER];
-#pragma unroll
-            for (int w = 0; w < WAVES; ++w) M = fmaxf(M, sm_m[w][16 * qt + qi]);
-            const float use = M == -INFINITY ? 0.f : M;
-#pragma unroll
-            for (int e = 0; e < PER; ++e) acc[e] = 0.f;
-#pragma unroll
-            for (int w = 0; w < WAVES; ++w) {
-                const float f = __builtin_amdgcn_exp2f(sm_m[w][16 * qt + qi] - use);
-                L += sm_l[w][16 * qt + qi] * f;
-#pragma unroll
-                for (int e = 0; e < PER; ++e) acc[e] += so[(w * 16 + qi) * OROW + d0 + e] * f;
-            }
-            const int tok = r / p.group, row = it.r0 + tok, hq = kvh * p.group + r - tok * p.group;
-            if (it.slot == DIRECT) {
-                const float inv = L > 0.f || L != L ? 1.0f / L : 0.f;
-                uint32_t w[PER / 2];
-#pragma unroll
-                for (int e = 0; e < PER; e += 2) w[e / 2] = pack_bf16x2(acc[e] * inv, acc[e + 1] * inv);
-                bf16_t* dst = p.out + (int64_t)row * p.o_ld + hq * D + d0;
-                if constexpr (PER == 8) *(uint4*)dst = make_uint4(w[0], w[1], w[2], w[3]);
-                else *(uint2*)dst = make_uint2(w[0], w[1]);
-                if (p.lse && d0 == 0) p.lse[(int64_t)row * p.heads + hq] = (use + __builtin_amdgcn_logf(L)) * 0.69314718055994530942f;
-            } else {
-                const int64_t at = ((int64_t)row * p.heads + hq) * p.slots + it.slot;
-#pragma unroll
-                for (int e = 0; e < PER; e += 4) *(float4*)(p.part_o + at * D + d0 + e) = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
-                if (d0 == 0) p.part_ml[at] = make_float2(M, L);
-            }
-        }
-    }
-    if constexpr (QT > 1) {
-        request_next();
-        st.store_q(sq);
-    }
-    __syncthreads();   // the next item's tiles go where these results were
-}
+__device__ __forceinline__ float lse_of(float m, float l) { return (m + __builtin_amdgcn_logf(l)) * 0.69314718055994530942f; }
+__device__ __forceinline__ float inverse_of(float l) { return l > 0.f || l != l ? 1.0f / l : 0.f; }   // no keys: zeros
 
-template <int D, int QP, int QS>
-__global__ __launch_bounds__(256, D == 64 || QP == 1 ? 3 : 2) void paged_attn_kernel(AttnParams p) {
-    __shared__ __attribute__((aligned(16))) char lds[Lds<D>::BYTES];
-    __shared__ __attribute__((aligned(16))) char sq[16 * QP * (2 * D + 16)];
-    __shared__ float sm_m[WAVES][64], sm_l[WAVES][64];
-    __shared__ Item items[BATCH];
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int total = (p.plain ? p.n * p.tiles_s : *p.count) * p.kv_heads;
-    const int grid = (int)gridDim.x - (p.plain && p.n_groups > 0);
-    if ((int)blockIdx.x == grid) {
-        check_groups(p);
-        return;
+// ---- stream ----
+template <int D, int QT>
+__global__ __launch_bounds__(256, 2) void paged_attn_stream_kernel(AttnParams p) {
+    __shared__ __attribute__((aligned(16))) char lds[WAVES * Rows<D>::TILE];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const Total total = *p.total;
+    int pos = (blockIdx.x * WAVES + wave) * total.per;
+    const int end = min(total.tiles, pos + total.per);
+    if (pos >= end) return;
+    Wave<D, QT> w(p, lds + wave * Rows<D>::TILE);
+
+    // the last segment that begins at or before pos: 64 probes at a time
+    int lo = 0, hi = total.segments;
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 63) >> 6, at = lo + lane * step;
+        const unsigned long long before = __ballot(at < hi && p.segments[at].start <= pos);
+        lo += (__popcll(before) - 1) * step;
+        hi = min(hi, lo + step);
     }
-    Stream<D, QP> st(p, tid & 63);
-    auto item_at = [&](int j) {
-        Item it;
-        const int* src = (const int*)&items[j];
-        int* dst = (int*)&it;
+    int which = lo;
+    Segment sg;
+    int ntiles, rel, kvh, first;   // rel: tile within the segment's query tile and KV head
+    auto fetch = [&] {             // wave-uniform
+        const int* src = (const int*)&p.segments[which];
+        int* dst = (int*)&sg;
 #pragma unroll
         for (int e = 0; e < 8; ++e) dst[e] = __builtin_amdgcn_readfirstlane(src[e]);
-        return it;
+        ntiles = (sg.k1 - sg.k0 + 31) >> 5;
     };
-    for (int w0 = blockIdx.x; w0 < total; w0 += BATCH * grid) {
-        const int n = min(BATCH, (total - w0 + grid - 1) / grid);
-        __syncthreads();
-        if (p.plain && tid < n) {
-            const int x = (w0 + tid * grid) / p.kv_heads, i = x / p.tiles_s;
-            const Entry e = entry_of(p, i, true);
-            items[tid] = Item{e.r0, e.T * p.group, (x - i * p.tiles_s) * 16 * QS, e.seq, 0, min(e.len, CHUNK_MAX), e.len - e.T + 1, DIRECT};
-        } else if (tid < n) {
-            const uint4* src = (const uint4*)&p.items[(w0 + tid * grid) / p.kv_heads];
-            uint4* dst = (uint4*)&items[tid];
-            dst[0] = src[0];
-            dst[1] = src[1];
-        }
-        __syncthreads();
-        Item it = item_at(0);
-        auto request = [&](const Item& x, int kvh, int ids) {
-            st.begin(ids, kvh, x.k0, x.k1);
-            st.load_q(x, kvh, x.limit == SHARED ? 16 * QP : 16 * QS);
-            if (wave < (x.k1 - x.k0 + 31) >> 5) {
-                st.load_k(wave);
-                st.load_v(wave);
-            }
-        };
-        request(it, w0 % p.kv_heads, st.page_numbers(it.seq, it.k0, it.k1));
-        st.store_q(sq);
-        __syncthreads();
-        for (int j = 0; j < n; ++j) {
-            const int w = w0 + j * grid, kvh = w % p.kv_heads, next_kvh = (w + grid) % p.kv_heads;
-            const Item next = item_at(min(j + 1, n - 1));
-            const int next_ids = st.page_numbers(next.seq, next.k0, next.k1);
-            auto request_next = [&] { if (j + 1 < n) request(next, next_kvh, next_ids); };
-            if (QP != QS && it.limit == SHARED) attend<D, QP, QP>(p, it, kvh, st, lds, sq, sm_m, sm_l, request_next);
-            else attend<D, QS, QP>(p, it, kvh, st, lds, sq, sm_m, sm_l, request_next);
-            it = next;
-        }
+    fetch();
+    {
+        const int at = pos - sg.start, stream = at / ntiles;   // segments without tiles are never the last one before a tile
+        rel = at - stream * ntiles;
+        kvh = stream % p.kv_heads;
+        first = stream / p.kv_heads * (16 * QT);
     }
+    int64_t head = (int64_t)kvh * p.head_stride;
+    auto window = [&] { w.page_numbers(sg.seq, sg.k0 + 32 * rel, sg.k1); };
+    window();
+    w.load(p.K, w.kf, head, sg.k0 + 32 * rel, sg.k1);
+    w.load(p.V, w.vf, head, sg.k0 + 32 * rel, sg.k1);
+    w.queries(sg, first, kvh);
+
+    // A tile, and the request of the next one.  That is unconditional where there is one (the wave's last tile has code of its own): a
+    // load behind a branch would make the waits count as if it had not been issued.
+    auto tile = [&](auto is_last) {
+        constexpr bool LAST = decltype(is_last)::value;
+        const Segment now = sg;
+        const int now_kvh = kvh, now_first = first, now_tiles = ntiles, kv0 = sg.k0 + 32 * rel;
+        const bool over = rel + 1 == ntiles;
+        auto next_k = [&] {
+            if constexpr (LAST) return;
+            if (!over) {
+                ++rel;
+                if (sg.k0 + 32 * rel - w.id_base >= 1024) window();
+            } else {
+                rel = 0;
+                if (++kvh == p.kv_heads) {
+                    kvh = 0;
+                    first += 16 * QT;
+                    if (first >= sg.M) {
+                        first = 0;
+                        do {
+                            ++which;
+                            fetch();
+                        } while (ntiles == 0 || sg.M == 0);   // there is a tile left, so there is such a segment
+                    }
+                    window();
+                } else if (w.id_base != sg.k0) {
+                    window();
+                }
+                head = (int64_t)kvh * p.head_stride;
+            }
+            w.load(p.K, w.kf, head, sg.k0 + 32 * rel, sg.k1);
+        };
+        auto next_v = [&] {
+            if constexpr (!LAST) w.load(p.V, w.vf, head, sg.k0 + 32 * rel, sg.k1);
+        };
+        w.step(kv0, now.k1, next_k, next_v);
+        if (over || LAST) {
+            // a part, or all there is for these rows
+            const int begin = now.start + (now_first / (16 * QT) * p.kv_heads + now_kvh) * now_tiles;   // first tile of these rows
+            const int before = begin / total.per, piece = pos / total.per - before;
+            const bool direct = now.whole && (begin + now_tiles - 1) / total.per == before;
+            const int slot = (now.limit == SHARED ? 0 : p.slots_p) + piece;
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) {
+                const int r = now_first + 16 * qt + w.li;
+                const float L = rows_sum(w.l[qt]);
+                if (r < now.M) {
+                    const int tok = r / p.group, row = now.r0 + tok, hq = now_kvh * p.group + r - tok * p.group;
+                    if (direct) {
+                        const float inv = inverse_of(L);
+                        bf16_t* dst = p.out + (int64_t)row * p.o_ld + hq * D + 4 * w.lg;
+#pragma unroll
+                        for (int dt = 0; dt < D / 16; ++dt)
+                            *(uint2*)(dst + 16 * dt) = make_uint2(pack_bf16x2(w.o[qt][dt][0] * inv, w.o[qt][dt][1] * inv),
+                                                                  pack_bf16x2(w.o[qt][dt][2] * inv, w.o[qt][dt][3] * inv));
+                        if (p.lse && w.lg == 0) p.lse[(int64_t)row * p.heads + hq] = lse_of(w.m[qt] == -INFINITY ? 0.f : w.m[qt], L);
+                    } else {
+                        const int64_t at = ((int64_t)row * p.heads + hq) * p.slots + slot;
+#pragma unroll
+                        for (int dt = 0; dt < D / 16; ++dt) *(f32x4*)(p.part_o + at * D + 16 * dt + 4 * w.lg) = w.o[qt][dt];
+                        if (w.lg == 0) p.part_ml[at] = make_float2(w.m[qt], L);
+                    }
+                }
+            }
+            if constexpr (!LAST) w.queries(sg, first, kvh);
+        }
+    };
+    for (; pos + 1 < end; ++pos) tile(std::false_type{});
+    tile(std::true_type{});
 }
 
-// Joins the parts of a row that has several: one wave per (row, head).
+// Joins the parts of a row that has several, and writes rows without keys: one wave per (row, head).
 template <int D>
 __global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnParams p) {
     constexpr int PER = D / 64;
     const int lane = threadIdx.x & 63;
     const int64_t item = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (item >= (int64_t)p.rows * p.heads) return;
-    const int row = (int)(item / p.heads), hq = (int)(item - (int64_t)row * p.heads);
-    const int parts = __builtin_amdgcn_readfirstlane(p.parts[row]), np = parts & 0xffff, n = np + (parts >> 16);
-    if (n <= 1) return;   // written already, or not a row of this step
-    auto slot_of = [&](int i) { return item * p.slots + (i < np ? i : p.chunks_p + i - np); };
+    const int row = (int)(item / p.heads), hq = (int)(item - (int64_t)row * p.heads), kvh = hq / p.group;
+    const RowParts rp = p.parts[row];
+    if (!rp.known) return;
+    const int per = p.total->per;
+    int count[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int r = (row - rp.r0[k]) * p.group + hq - kvh * p.group;
+        const int begin = rp.start[k] + (r / p.rows_q * p.kv_heads + kvh) * rp.tiles[k];
+        count[k] = rp.tiles[k] > 0 ? (begin + rp.tiles[k] - 1) / per - begin / per + 1 : 0;
+    }
+    const int np = min(count[0], p.slots_p), n = np + min(count[1], p.slots - p.slots_p);
+    if (np == 0 && n == 1) return;   // written already
+    auto slot_of = [&](int i) { return item * p.slots + (i < np ? i : p.slots_p + i - np); };
     float M = -INFINITY, L = 0.f, acc[PER];
 #pragma unroll
     for (int e = 0; e < PER; ++e) acc[e] = 0.f;
@@ -598,84 +566,146 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnParams p) {
             for (int e = 0; e < PER; ++e) acc[e] += v[a][e] * f;
         }
     };
-    if (n <= 2) turn(0, std::integral_constant<int, 2>{}, false);
-    else {
+    if (n > 0 && n <= 2) turn(0, std::integral_constant<int, 2>{}, false);
+    else if (n <= 4 && n > 0) turn(0, std::integral_constant<int, 4>{}, false);
+    else if (n > 0) {
         for (int i = lane; i < n; i += 64) M = fmaxf(M, p.part_ml[slot_of(i)].x);
         M = wave_max(M);
         for (int i0 = 0; i0 < n; i0 += 8) turn(i0, std::integral_constant<int, 8>{}, true);
     }
-    const float use = M == -INFINITY ? 0.f : M;
-    const float inv = L > 0.f || L != L ? 1.0f / L : 0.f;
+    const float inv = inverse_of(L);
     bf16_t* dst = p.out + (int64_t)row * p.o_ld + hq * D + lane * PER;
     if constexpr (PER == 2) *(uint32_t*)dst = pack_bf16x2(acc[0] * inv, acc[1] * inv);
     else *dst = f32_to_bf16(acc[0] * inv);
-    if (p.lse && lane == 0) p.lse[item] = (use + __builtin_amdgcn_logf(L)) * 0.69314718055994530942f;
+    if (p.lse && lane == 0) p.lse[item] = lse_of(M == -INFINITY ? 0.f : M, L);
+}
+
+// ---- plain ----
+template <int D, int QT>
+__global__ __launch_bounds__(256, 2) void paged_attn_plain_kernel(AttnParams p) {
+    constexpr int OROW = D + 4, PER = D / 16;
+    __shared__ __attribute__((aligned(16))) char lds[WAVES * Rows<D>::TILE];
+    __shared__ float sm_m[WAVES][16], sm_l[WAVES][16];
+    static_assert(WAVES * Rows<D>::TILE >= WAVES * 16 * OROW * 4, "the waves' results fit where their tiles were");
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int kvh = blockIdx.x % p.kv_heads, x = blockIdx.x / p.kv_heads, i = x / p.tiles_q;
+    if (i == p.n) {
+        check_groups(p);
+        return;
+    }
+    const Entry e = entry_of(p, i, true);
+    const Segment sg{e.r0, e.T * p.group, e.seq, 0, min(e.len, PLAIN_KEYS), e.len - e.T + 1, 0, 1};
+    const int first = (x - i * p.tiles_q) * 16 * QT, ntiles = (sg.k1 + 31) >> 5;
+    if (first >= sg.M) return;
+    Wave<D, QT> w(p, lds + wave * Rows<D>::TILE);
+    const int64_t head = (int64_t)kvh * p.head_stride;
+    int t = wave;
+    if (t < ntiles) {
+        w.page_numbers(sg.seq, 0, sg.k1);
+        w.load(p.K, w.kf, head, 32 * t, sg.k1);
+        w.load(p.V, w.vf, head, 32 * t, sg.k1);
+    }
+    w.queries(sg, first, kvh);
+    // a tile with a successor requests it unconditionally: a load behind a branch would make the waits count as if it had not been issued
+    if (t < ntiles) {
+        for (; t + WAVES < ntiles; t += WAVES)
+            w.step(32 * t, sg.k1, [&] { w.load(p.K, w.kf, head, 32 * (t + WAVES), sg.k1); }, [&] { w.load(p.V, w.vf, head, 32 * (t + WAVES), sg.k1); });
+        w.step(32 * t, sg.k1, [] {}, [] {});
+    }
+    // join the four waves, 16 queries at a time
+    float* const so = (float*)lds;
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+        const float lt = rows_sum(w.l[qt]);
+        __syncthreads();
+        if (w.lg == 0) {
+            sm_m[wave][w.li] = w.m[qt];
+            sm_l[wave][w.li] = lt;
+        }
+#pragma unroll
+        for (int dt = 0; dt < D / 16; ++dt) *(f32x4*)(so + (wave * 16 + w.li) * OROW + 16 * dt + 4 * w.lg) = w.o[qt][dt];
+        __syncthreads();
+        const int qi = tid >> 4, d0 = (tid & 15) * PER, r = first + 16 * qt + qi;
+        if (r < sg.M) {
+            float M = -INFINITY, L = 0.f, acc[PER];
+#pragma unroll
+            for (int v = 0; v < WAVES; ++v) M = fmaxf(M, sm_m[v][qi]);
+            const float use = M == -INFINITY ? 0.f : M;
+#pragma unroll
+            for (int d = 0; d < PER; ++d) acc[d] = 0.f;
+#pragma unroll
+            for (int v = 0; v < WAVES; ++v) {
+                const float f = __builtin_amdgcn_exp2f(sm_m[v][qi] - use);
+                L += sm_l[v][qi] * f;
+#pragma unroll
+                for (int d = 0; d < PER; ++d) acc[d] += so[(v * 16 + qi) * OROW + d0 + d] * f;
+            }
+            const int tok = r / p.group, row = sg.r0 + tok, hq = kvh * p.group + r - tok * p.group;
+            const float inv = inverse_of(L);
+            uint32_t b[PER / 2];
+#pragma unroll
+            for (int d = 0; d < PER; d += 2) b[d / 2] = pack_bf16x2(acc[d] * inv, acc[d + 1] * inv);
+            bf16_t* dst = p.out + (int64_t)row * p.o_ld + hq * D + d0;
+            if constexpr (PER == 8) *(uint4*)dst = make_uint4(b[0], b[1], b[2], b[3]);
+            else *(uint2*)dst = make_uint2(b[0], b[1]);
+            if (p.lse && d0 == 0) p.lse[(int64_t)row * p.heads + hq] = lse_of(use, L);
+        }
+    }
 }
 
 struct Plan {
-    int qp, qs;           // 16-row tiles of a shared and of an own item
-    int chunk, chunks_p, chunks_s, slots;
-    int64_t items;        // at most
-    int64_t at_parts, at_plan, at_items, at_ml, at_o, bytes;
     bool plain;
-    int tiles_s;
+    int qt, tiles_q, per_min, slots_p, slots;
+    int64_t at_plan, at_segments, at_parts, at_ml, at_o, bytes;
 };
-int tiles_for(int64_t rows) { return rows <= 16 ? 1 : 2; }
+bool groups_count(const q3asr_kv_pages& c, const q3asr_attn_batch& b) { return b.n_groups > 0 && b.max_shared >= c.page_tokens; }
 Plan plan_for(const q3asr_kv_pages& c, const q3asr_attn_batch& b, int heads) {
     Plan r{};
     const int group = heads / c.kv_heads;
-    r.qs = tiles_for((int64_t)b.max_rows * group);
-    r.tiles_s = cdiv((int64_t)b.max_rows * group, 16 * r.qs);
-    // A small step is all latency: whole sequences as items that fit the device at once, shared or not, in one launch.
-    r.plain = b.max_len <= CHUNK_MAX && (int64_t)b.n * r.tiles_s * c.kv_heads <= PLAIN_ITEMS;
-    const bool shares = !r.plain && b.n_groups > 0 && b.max_shared >= c.page_tokens;
-    const int own = shares ? b.max_own : b.max_len;
-    r.qp = shares ? std::max(r.qs, tiles_for((int64_t)b.max_group_rows * group)) : r.qs;
-    // About three items per workgroup of a full device: fewer and larger items have less to join and less that begins and ends, more
-    // and smaller ones spread a few long sequences over the device.
-    const int64_t keys = (shares ? (int64_t)b.n_groups * b.max_shared : 0) + (int64_t)b.n * own;
-    r.chunk = (int)std::min<int64_t>(CHUNK_MAX, std::max<int64_t>(128, (keys * c.kv_heads / (CUS * 9) + 127) / 128 * 128));
-    r.chunks_p = shares ? cdiv(b.max_shared, r.chunk) : 0;
-    r.chunks_s = std::max(1, cdiv(own, r.chunk));
-    r.slots = r.chunks_p + r.chunks_s;
-    r.items = (shares ? (int64_t)b.n_groups * r.chunks_p * cdiv((int64_t)b.max_group_rows * group, 16 * r.qp) : 0) +
-              (int64_t)b.n * r.chunks_s * cdiv((int64_t)b.max_rows * group, 16 * r.qs);
-    if (r.plain) {
-        r.chunk = CHUNK_MAX;
-        r.chunks_p = 0;
-        r.chunks_s = r.slots = 1;
-        r.qp = r.qs;
-        r.items = (int64_t)b.n * r.tiles_s;
-        return r;
-    }
+    // A small step is all latency: whole sequences that fit the device at once, shared or not, in one launch.
+    r.qt = (int64_t)b.max_rows * group <= 16 ? 1 : 2;
+    r.tiles_q = cdiv((int64_t)b.max_rows * group, 16 * r.qt);
+    r.plain = b.max_len <= PLAIN_KEYS && (int64_t)b.n * r.tiles_q * c.kv_heads <= PLAIN_ITEMS;
+    if (r.plain) return r;
+    const bool shares = groups_count(c, b);
+    if (shares && (int64_t)b.max_group_rows * group > 16) r.qt = 2;
+    // Parts of a row: tiles of its longest segment by the least tiles of a wave, and one for where it begins.  More parts spread a few
+    // long sequences over the device; their memory is kept to 64 MB (but 16 parts).
+    const int64_t part = (int64_t)b.rows * heads * (c.head_dim * 4 + 8);
+    const int most = (int)std::max<int64_t>(16, std::min<int64_t>(1024, (64ll << 20) / part));
+    const int own = shares ? b.max_own : b.max_len, longest = std::max({own, shares ? b.max_shared : 0, 1});
+    r.per_min = std::max(2, cdiv(cdiv(longest, 32), most));
+    r.slots_p = shares ? cdiv(cdiv(b.max_shared, 32), r.per_min) + 1 : 0;
+    r.slots = r.slots_p + cdiv(cdiv(own, 32), r.per_min) + 1;
     auto round = [](int64_t x) { return (x + 255) & ~255ll; };
-    r.at_parts = 256;
-    r.at_plan = r.at_parts + round((int64_t)b.rows * 4);
-    r.at_items = r.at_plan + (b.n > HELD || b.n_groups > HELD ? round((int64_t)b.n * (int64_t)sizeof(Entry) + (int64_t)b.n_groups * 4) : 0);
-    r.at_ml = r.at_items + round(r.items * (int64_t)sizeof(Item));
-    r.at_o = r.at_ml + (r.slots > 1 ? round((int64_t)b.rows * heads * r.slots * 8) : 0);
-    r.bytes = r.at_o + (r.slots > 1 ? round((int64_t)b.rows * heads * r.slots * c.head_dim * 4) : 0);
+    const int64_t groups = shares ? b.n_groups : 0;
+    r.at_plan = 256;
+    r.at_segments = r.at_plan + (b.n > HELD || groups > HELD ? round((int64_t)b.n * (int64_t)sizeof(Entry) + groups * 4) : 0);
+    r.at_parts = r.at_segments + round((b.n + groups) * (int64_t)sizeof(Segment));
+    r.at_ml = r.at_parts + round((int64_t)b.rows * (int64_t)sizeof(RowParts));
+    r.at_o = r.at_ml + round((int64_t)b.rows * heads * r.slots * 8);
+    r.bytes = r.at_o + round((int64_t)b.rows * heads * r.slots * c.head_dim * 4);
     return r;
 }
 
 template <int D>
 void launch_d(const AttnParams& p, const Plan& r, hipStream_t s) {
     const dim3 block(256);
-    if (!r.plain) {
-        hipLaunchKernelGGL(paged_attn_plan_kernel, dim3(1), dim3(PLAN), 0, s, p);
+    if (r.plain) {
+        const dim3 grid(p.n * r.tiles_q * p.kv_heads + (p.n_groups > 0));
+        if (r.qt == 1) hipLaunchKernelGGL((paged_attn_plain_kernel<D, 1>), grid, block, 0, s, p);
+        else hipLaunchKernelGGL((paged_attn_plain_kernel<D, 2>), grid, block, 0, s, p);
         HIP_CHECK(hipGetLastError());
+        return;
     }
-    const dim3 grid((int)std::min<int64_t>(r.items * p.kv_heads, CUS * (D == 64 || r.qp == 1 ? 3 : 2)) + (r.plain && p.n_groups > 0));
-    switch (r.qp * 10 + r.qs) {
-        case 11: hipLaunchKernelGGL((paged_attn_kernel<D, 1, 1>), grid, block, 0, s, p); break;
-        case 21: hipLaunchKernelGGL((paged_attn_kernel<D, 2, 1>), grid, block, 0, s, p); break;
-        default: hipLaunchKernelGGL((paged_attn_kernel<D, 2, 2>), grid, block, 0, s, p); break;
-    }
+    hipLaunchKernelGGL(paged_attn_plan_kernel, dim3(1), dim3(PLAN), 0, s, p);
     HIP_CHECK(hipGetLastError());
-    if (p.slots > 1) {
-        hipLaunchKernelGGL((paged_attn_join_kernel<D>), dim3(cdiv((int64_t)p.rows * p.heads, 4)), block, 0, s, p);
-        HIP_CHECK(hipGetLastError());
-    }
+    const dim3 grid(STREAM_WAVES / WAVES);
+    if (r.qt == 1) hipLaunchKernelGGL((paged_attn_stream_kernel<D, 1>), grid, block, 0, s, p);
+    else hipLaunchKernelGGL((paged_attn_stream_kernel<D, 2>), grid, block, 0, s, p);
+    HIP_CHECK(hipGetLastError());
+    hipLaunchKernelGGL((paged_attn_join_kernel<D>), dim3(cdiv((int64_t)p.rows * p.heads, 4)), block, 0, s, p);
+    HIP_CHECK(hipGetLastError());
 }
 
 }  // namespace
@@ -695,25 +725,26 @@ void launch_paged_attention(const q3asr_kv_pages& c, int layer, const bf16_t* q,
     p.seqs = b.seqs; p.cu_rows = b.cu_rows; p.cu_groups = b.cu_groups; p.shared = b.shared;
     p.max_seqs = c.max_seqs; p.max_seq_pages = c.max_seq_pages; p.pages = c.pages;
     while ((1 << p.pt_shift) < c.page_tokens) ++p.pt_shift;
-    const bool shares = b.n_groups > 0 && b.max_shared >= c.page_tokens;
+    const bool shares = groups_count(c, b);
     p.n = b.n; p.rows = b.rows; p.n_groups = shares ? b.n_groups : 0;
     p.heads = heads; p.kv_heads = c.kv_heads; p.group = heads / c.kv_heads;
     p.max_rows = b.max_rows; p.max_group_rows = b.max_group_rows; p.max_len = b.max_len;
     p.max_own = shares ? b.max_own : b.max_len;
     p.max_shared = b.max_shared;
     p.scale_log2 = scale * 1.44269504088896340736f;
-    p.chunk = r.chunk; p.chunks_p = r.chunks_p; p.chunks_s = r.chunks_s; p.slots = r.slots;
-    p.rows_p = 16 * r.qp; p.rows_s = 16 * r.qs;
+    p.rows_q = 16 * r.qt; p.tiles_q = r.tiles_q; p.per_min = r.per_min; p.slots_p = r.slots_p; p.slots = r.slots;
     char* ws = (char*)workspace;
-    p.plain = r.plain;
-    p.tiles_s = r.tiles_s;
-    p.count = (int*)ws;
+    p.total = (Total*)ws;
     p.plan_ws = ws + r.at_plan;
-    p.parts = (int*)(ws + r.at_parts);
-    p.items = (Item*)(ws + r.at_items);
+    p.segments = (Segment*)(ws + r.at_segments);
+    p.parts = (RowParts*)(ws + r.at_parts);
     p.part_ml = (float2*)(ws + r.at_ml);
     p.part_o = (float*)(ws + r.at_o);
-    Q3_REQUIRE(r.items * c.kv_heads < (1ll << 30) && r.slots < (1 << 15), "paged_attention: too much work for one call (smaller bounds in the batch make less)");
+    // tile numbers are 32 bits
+    const int64_t group = p.group, own = cdiv(p.max_own, 32), sh = cdiv(p.max_shared, 32);
+    Q3_REQUIRE(r.plain || (own * cdiv((int64_t)b.max_rows * group, 16) * b.n + (shares ? sh * cdiv((int64_t)b.max_group_rows * group, 16) * b.n_groups : 0)) *
+                                  c.kv_heads < (1ll << 30),
+               "paged_attention: too much work for one call (smaller bounds in the batch make less)");
     ProfScope ps("paged_attn_kernel", 4.0 * b.rows * heads * (double)b.max_len * c.head_dim, s);
     if (c.head_dim == 64) launch_d<64>(p, r, s);
     else launch_d<128>(p, r, s);
