@@ -13,8 +13,8 @@
 //
 //   plain   few rows: a workgroup per sequence and KV head, its four waves taking tiles in turn; one launch, nothing shared
 //   stream  the tiles of all sequences and groups in one row, cut into equal parts, one per wave of a full device: no wave waits for
-//           another, and each has a tile in flight all the time.  Three launches: a plan (one workgroup: lengths -> where every
-//           sequence's tiles begin), the waves, and the join of what was cut.
+//           another, and each has a tile in flight all the time.  Where a wave goes over to other rows counts like a tile.  Two
+//           launches: the waves, which find out first where every sequence's tiles begin, and the join of what was cut.
 // Measured against 4-wave work items of up to 1024 keys, sorted by size: rounding to four tiles and joining cost 1.2 to 1.4 times
 // the mean load there.
 #include "paged.h"
@@ -62,17 +62,18 @@ __device__ __forceinline__ void wave_lds_fence() {
 // [k0, k1) of the pages of sequence seq, row r those below limit + r / group (SHARED: all of them).
 struct __attribute__((aligned(16))) Segment {
     int r0, M, seq, k0, k1, limit;
-    int start;    // first tile in the row of all tiles; tile t of query tile q and KV head h is start + (q * kv_heads + h) * ntiles + t
+    int start;    // place in the row of all tiles: stream h * query tiles + q (KV head h, query tile q) takes ntiles + 1 places from
+                  // start + stream * (ntiles + 1) on, one for its beginning and one per tile
     int whole;    // 1: its rows read nothing else
 };
 constexpr int SHARED = 0x7fffffff;
-// Where a row's parts are: tiles of its group's and of its own segment (0: none), their starts and first rows.
+// Where a row's parts are: tiles of its group's and of its own segment (0: none), their starts, first rows and query tiles.
 struct __attribute__((aligned(16))) RowParts {
-    int start[2], tiles[2], r0[2];
-    int known, pad;
+    int start[2], tiles[2], r0[2], streams[2];
+    int known, pad[3];
 };
 struct __attribute__((aligned(16))) Total {
-    int tiles, per, segments, pad;   // per: tiles of a wave
+    int places, per, segments, pad;   // per: places of a wave
 };
 
 struct AttnParams {
@@ -91,7 +92,7 @@ struct AttnParams {
     int tiles_q;                               // plain: query tiles of a sequence
     int per_min, slots_p, slots;               // parts of a row at most: of its group's segment first
     Total* total;
-    void* plan_ws;                             // what of a plan does not fit LDS
+    void* plan_ws;                             // of a plan that does not fit LDS, and its segments
     Segment* segments;
     RowParts* parts;                           // [rows]
     float2* part_ml;                           // [rows][heads][slots]: maximum (base 2), sum
@@ -120,34 +121,40 @@ __device__ __forceinline__ Entry entry_of(const AttnParams& p, int i, bool repor
 }
 
 // ---- plan ----
-// Two dependent loads per sequence (its number, its length), everything else from LDS: with one workgroup nothing covers latency.
-// Lists beyond HELD entries or groups stay in the workspace.
+// Where every segment's tiles begin, from the lengths.  Up to HELD groups and sequences every workgroup finds out for itself, in LDS
+// (two dependent loads per sequence, its number and its length, and no launch of its own); beyond that one workgroup does it
+// for all, in the workspace.  tell: errors are reported and the rows' parts written down, by one workgroup of all.
 constexpr int HELD = 1024;
-__global__ __launch_bounds__(PLAN) void paged_attn_plan_kernel(AttnParams p) {
-    __shared__ Entry held[HELD];
-    __shared__ int held_cu[HELD + 1], held_from[HELD], held_rows[HELD + 1], scan[PLAN / 64];
+struct PlanMemory {
+    Entry* entry;            // [n]
+    int *from, *cu, *rows;   // [n_groups] tokens that a group shares, [n_groups + 1], [n + 1]: of the batch
+    int* scan;               // a word per wave
+    Segment* segments;       // [n_groups + n]
+};
+template <int THREADS>
+__device__ __forceinline__ Total plan_segments(const AttnParams& p, const PlanMemory& mem, bool tell) {
     const int tid = threadIdx.x;
-    Entry* const entry = p.n <= HELD ? held : (Entry*)p.plan_ws;
-    int* const from = p.n_groups <= HELD ? held_from : (int*)((Entry*)p.plan_ws + p.n);   // tokens that a group shares
-    const int* const cu = p.n_groups <= HELD ? held_cu : p.cu_groups;
-    const int* const cu_rows = p.n <= HELD ? held_rows : p.cu_rows;
-    for (int r = tid; r < p.rows; r += PLAN) p.parts[r].known = 0;
-    if (p.n_groups > 0 && p.n_groups <= HELD)
-        for (int g = tid; g <= p.n_groups; g += PLAN) held_cu[g] = p.cu_groups[g];
-    for (int g = tid; g < p.n_groups; g += PLAN) from[g] = p.shared[g];
-    if (p.n <= HELD)
-        for (int i = tid; i <= p.n; i += PLAN) held_rows[i] = p.cu_rows[i];
-    for (int i = tid; i < p.n; i += PLAN) entry[i] = entry_of(p, i, true);
+    Entry* const entry = mem.entry;
+    int* const from = mem.from;
+    int *const cu = mem.cu, *const cu_rows = mem.rows, *const scan = mem.scan;
+    if (tell)
+        for (int r = tid; r < p.rows; r += THREADS) p.parts[r].known = 0;
+    if (p.n_groups > 0)
+        for (int g = tid; g <= p.n_groups; g += THREADS) cu[g] = p.cu_groups[g];
+    for (int g = tid; g < p.n_groups; g += THREADS) from[g] = p.shared[g];
+    for (int i = tid; i <= p.n; i += THREADS) cu_rows[i] = p.cu_rows[i];
+    for (int i = tid; i < p.n; i += THREADS) entry[i] = entry_of(p, i, tell);
     __syncthreads();
-    for (int g = tid; g < p.n_groups; g += PLAN) {
+    for (int g = tid; g < p.n_groups; g += THREADS) {
         const int i0 = cu[g], i1 = cu[g + 1], shared = from[g];
         from[g] = 0;
-        if (i0 < 0 || i1 < i0 || i1 > p.n) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, g);
-        else if (i1 > i0) {
+        if (i0 < 0 || i1 < i0 || i1 > p.n) {
+            if (tell) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, g);
+        } else if (i1 > i0) {
             const Entry first = entry[i0];
             const int end = cu_rows[i1];
             const bool fits = end >= first.r0 && end <= p.rows && end - first.r0 <= p.max_group_rows;
-            if (shared > p.max_shared || (first.ok && !fits)) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, i0);
+            if (shared > p.max_shared || (first.ok && !fits)) if (tell) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, i0);
             if (first.ok && fits) from[g] = max(0, min(min(shared, p.max_shared), first.len - first.T)) >> p.pt_shift << p.pt_shift;
         }
     }
@@ -155,7 +162,7 @@ __global__ __launch_bounds__(PLAN) void paged_attn_plan_kernel(AttnParams p) {
     // segments: the groups', then the sequences'
     const int all = p.n_groups + p.n;
     int carry = 0;
-    for (int w0 = 0; w0 < all; w0 += PLAN) {
+    for (int w0 = 0; w0 < all; w0 += THREADS) {
         const int w = w0 + tid;
         Segment sg{};
         int g = -1, count = 0;
@@ -183,14 +190,15 @@ __global__ __launch_bounds__(PLAN) void paged_attn_plan_kernel(AttnParams p) {
                     behind = from[lo];
                     ok = ok && entry[i0].ok;
                 } else {
-                    pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, i);
+                    if (tell) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, i);
                 }
             }
-            if (ok && (behind > max(0, e.len - e.T) || e.len - behind > p.max_own)) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, i);
+            if (ok && (behind > max(0, e.len - e.T) || e.len - behind > p.max_own)) if (tell) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, i);
             sg = Segment{e.r0, e.T * p.group, e.seq, behind, behind + min(max(0, e.len - behind), p.max_own), e.len - e.T + 1, 0, behind == 0};
         }
         const int tiles = (sg.k1 - sg.k0 + 31) >> 5;
-        count = tiles * ((sg.M + p.rows_q - 1) / p.rows_q) * p.kv_heads;
+        const int streams = (sg.M + p.rows_q - 1) / p.rows_q;
+        count = tiles > 0 ? (tiles + 1) * streams * p.kv_heads : 0;
         // exclusive prefix sum
         const int lane = tid & 63, wave = tid >> 6;
         int x = count;
@@ -202,29 +210,38 @@ __global__ __launch_bounds__(PLAN) void paged_attn_plan_kernel(AttnParams p) {
         if (lane == 63) scan[wave] = x;
         __syncthreads();
         int before = carry;
-        for (int v = 0; v < PLAN / 64; ++v) {
+        for (int v = 0; v < THREADS / 64; ++v) {
             before += v < wave ? scan[v] : 0;
             carry += scan[v];
         }
         sg.start = before + x - count;
-        if (w < all) p.segments[w] = sg;
+        if (w < all) mem.segments[w] = sg;
         __syncthreads();   // scan is written again; the groups' segments are read below
-        if (w >= p.n_groups && w < all) {
+        if (tell && w >= p.n_groups && w < all) {
             RowParts rp{};
             if (g >= 0 && from[g] > 0) {
-                const Segment& sh = p.segments[g];
+                const Segment& sh = mem.segments[g];
                 rp.start[0] = sh.start;
                 rp.tiles[0] = (sh.k1 - sh.k0 + 31) >> 5;
                 rp.r0[0] = sh.r0;
+                rp.streams[0] = (sh.M + p.rows_q - 1) / p.rows_q;
             }
             rp.start[1] = sg.start;
             rp.tiles[1] = tiles;
             rp.r0[1] = sg.r0;
+            rp.streams[1] = streams;
             rp.known = 1;
             for (int t = 0; t < e.T; ++t) p.parts[e.r0 + t] = rp;
         }
     }
-    if (tid == 0) *p.total = Total{carry, max(p.per_min, (carry + STREAM_WAVES - 1) / STREAM_WAVES), all, 0};
+    const Total total{carry, max(p.per_min, (carry + STREAM_WAVES - 1) / STREAM_WAVES), all, 0};
+    if (tell && tid == 0) *p.total = total;
+    return total;
+}
+__global__ __launch_bounds__(PLAN) void paged_attn_plan_kernel(AttnParams p) {
+    __shared__ int scan[PLAN / 64];
+    int* ints = (int*)((Entry*)p.plan_ws + p.n);
+    plan_segments<PLAN>(p, PlanMemory{(Entry*)p.plan_ws, ints, ints + p.n_groups, ints + 2 * p.n_groups + 1, scan, p.segments}, true);
 }
 
 // Without a plan the groups are not used; a workgroup of its own checks them all the same.
@@ -265,6 +282,7 @@ struct Wave {
     Frag qf[QT][NKS];             // queries as B fragments: lane (li, lg) holds values 32 ks + 8 lg .. of query 16 qt + li
     int limit[QT];                // the lane's queries see keys below
     int lowest;                   // keys below it are seen by all of them
+    int active;                   // groups of 16 queries that there are
     float m[QT], l[QT];           // l: of this lane's keys only, until the end
     f32x4 o[QT][NDT];             // lane (li, lg) holds values 16 dt + 4 lg .. of query 16 qt + li
     int ids, id_base;             // page numbers of 64 times 16 keys from key id_base on, one per lane
@@ -279,17 +297,28 @@ struct Wave {
             ids = 0;
         }
     }
-    __device__ int64_t base_of(int64_t head, int key, int k1) const {   // 16 keys; those behind the last 16 are read from these
-        const int at = min(key, (k1 - 1) & ~15);
-        const int64_t page = __builtin_amdgcn_readlane(ids, (at - id_base) >> 4);
-        return page * p.page_stride + head + (int64_t)(at & ((1 << p.pt_shift) - 1)) * D;
+    __device__ int64_t base_of(int64_t head, int key) const {   // 16 keys of a page
+        const int64_t page = __builtin_amdgcn_readlane(ids, (key - id_base) >> 4);
+        return page * p.page_stride + head + (int64_t)(key & ((1 << p.pt_shift) - 1)) * D;
     }
+    // Keys behind the last one are read from its row, so that they cost no memory traffic.
     __device__ void load(const bf16_t* pool, Frag (&x)[2][IV], int64_t head, int kv0, int k1) const {
+        if (kv0 + 32 <= k1) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const bf16_t* src = pool + base_of(head, kv0 + 16 * h, k1) + (lane / LPR) * D + 8 * (lane % LPR);
+            for (int h = 0; h < 2; ++h) {
+                const bf16_t* src = pool + base_of(head, kv0 + 16 * h) + (lane / LPR) * D + 8 * (lane % LPR);
 #pragma unroll
-            for (int i = 0; i < IV; ++i) x[h][i].v = __builtin_nontemporal_load((const bf16x8*)(src + i * RPI * D));
+                for (int i = 0; i < IV; ++i) x[h][i].v = __builtin_nontemporal_load((const bf16x8*)(src + i * RPI * D));
+            }
+        } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int key = min(kv0 + 16 * h, (k1 - 1) & ~15);
+                const bf16_t* src = pool + base_of(head, key) + 8 * (lane % LPR);
+#pragma unroll
+                for (int i = 0; i < IV; ++i)
+                    x[h][i].v = __builtin_nontemporal_load((const bf16x8*)(src + min(lane / LPR + i * RPI, k1 - 1 - key) * D));
+            }
         }
     }
     __device__ void queries(const Segment& sg, int first, int kvh) {
@@ -308,6 +337,7 @@ struct Wave {
             for (int dt = 0; dt < NDT; ++dt) o[qt][dt] = (f32x4){0.f, 0.f, 0.f, 0.f};
         }
         lowest = min(sg.k1, sg.limit);
+        active = (sg.M - first + 15) >> 4;
     }
     // The tile of keys kv0 .. whose rows are in kf and vf; next_k and next_v request the next tile's once these are free.
     template <class NK, class NV>
@@ -333,6 +363,7 @@ struct Wave {
         bool moved = false;
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) {
+            if (qt > 0 && qt >= active) break;   // wave-uniform
             f32x4 s[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -381,9 +412,11 @@ struct Wave {
         wave_lds_fence();
         if (__builtin_amdgcn_ballot_w64(moved) != 0) {
 #pragma unroll
-            for (int qt = 0; qt < QT; ++qt)
+            for (int qt = 0; qt < QT; ++qt) {
+                if (qt > 0 && qt >= active) break;
 #pragma unroll
                 for (int dt = 0; dt < NDT; ++dt) o[qt][dt] *= alpha[qt];
+            }
         }
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) {
@@ -394,7 +427,10 @@ struct Wave {
             va.h[0] = lo.u;
             va.h[1] = hi.u;
 #pragma unroll
-            for (int qt = 0; qt < QT; ++qt) o[qt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va.v, pf[qt].v, o[qt][dt], 0, 0, 0);
+            for (int qt = 0; qt < QT; ++qt) {
+                if (qt > 0 && qt >= active) break;
+                o[qt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va.v, pf[qt].v, o[qt][dt], 0, 0, 0);
+            }
         }
         __builtin_amdgcn_wave_barrier();   // the next tile's rows are written after these reads
     }
@@ -404,13 +440,22 @@ __device__ __forceinline__ float lse_of(float m, float l) { return (m + __builti
 __device__ __forceinline__ float inverse_of(float l) { return l > 0.f || l != l ? 1.0f / l : 0.f; }   // no keys: zeros
 
 // ---- stream ----
-template <int D, int QT>
+template <int D, int QT, bool PLANNED>
 __global__ __launch_bounds__(256, 2) void paged_attn_stream_kernel(AttnParams p) {
-    __shared__ __attribute__((aligned(16))) char lds[WAVES * Rows<D>::TILE];
+    constexpr int PLAN_BYTES = PLANNED ? 0 : HELD * (int)sizeof(Entry) + (3 * HELD + 2 + WAVES) * 4, TILES = WAVES * Rows<D>::TILE;
+    __shared__ __attribute__((aligned(16))) char lds[PLAN_BYTES > TILES ? PLAN_BYTES : TILES];
+    __shared__ Segment held[PLANNED ? 1 : HELD];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const Total total = *p.total;
+    const Segment* const segments = PLANNED ? p.segments : held;
+    Total total;
+    if constexpr (PLANNED) total = *p.total;
+    else {
+        int* ints = (int*)((Entry*)lds + HELD);
+        total = plan_segments<256>(p, PlanMemory{(Entry*)lds, ints, ints + HELD, ints + 2 * HELD + 1, ints + 3 * HELD + 2, held}, blockIdx.x == 0);
+        __syncthreads();   // the tiles go where the plan was made
+    }
     int pos = (blockIdx.x * WAVES + wave) * total.per;
-    const int end = min(total.tiles, pos + total.per);
+    const int end = min(total.places, pos + total.per);
     if (pos >= end) return;
     Wave<D, QT> w(p, lds + wave * Rows<D>::TILE);
 
@@ -418,15 +463,15 @@ __global__ __launch_bounds__(256, 2) void paged_attn_stream_kernel(AttnParams p)
     int lo = 0, hi = total.segments;
     while (hi - lo > 1) {
         const int step = (hi - lo + 63) >> 6, at = lo + lane * step;
-        const unsigned long long before = __ballot(at < hi && p.segments[at].start <= pos);
+        const unsigned long long before = __ballot(at < hi && segments[at].start <= pos);
         lo += (__popcll(before) - 1) * step;
         hi = min(hi, lo + step);
     }
     int which = lo;
     Segment sg;
-    int ntiles, rel, kvh, first;   // rel: tile within the segment's query tile and KV head
+    int ntiles, rel, kvh, first;   // rel: tile within the stream
     auto fetch = [&] {             // wave-uniform
-        const int* src = (const int*)&p.segments[which];
+        const int* src = (const int*)&segments[which];
         int* dst = (int*)&sg;
 #pragma unroll
         for (int e = 0; e < 8; ++e) dst[e] = __builtin_amdgcn_readfirstlane(src[e]);
@@ -434,10 +479,15 @@ __global__ __launch_bounds__(256, 2) void paged_attn_stream_kernel(AttnParams p)
     };
     fetch();
     {
-        const int at = pos - sg.start, stream = at / ntiles;   // segments without tiles are never the last one before a tile
-        rel = at - stream * ntiles;
-        kvh = stream % p.kv_heads;
-        first = stream / p.kv_heads * (16 * QT);
+        // segments without tiles are never the last one before a place
+        const int at = pos - sg.start, stream = at / (ntiles + 1), streams = (sg.M + 16 * QT - 1) / (16 * QT);
+        rel = at - stream * (ntiles + 1) - 1;
+        kvh = stream / streams;
+        first = (stream - kvh * streams) * (16 * QT);
+        if (rel < 0) {   // the place of a beginning; a wave has two places at least, so the tile behind it is its own
+            rel = 0;
+            ++pos;
+        }
     }
     int64_t head = (int64_t)kvh * p.head_stride;
     auto window = [&] { w.page_numbers(sg.seq, sg.k0 + 32 * rel, sg.k1); };
@@ -460,20 +510,20 @@ __global__ __launch_bounds__(256, 2) void paged_attn_stream_kernel(AttnParams p)
                 if (sg.k0 + 32 * rel - w.id_base >= 1024) window();
             } else {
                 rel = 0;
-                if (++kvh == p.kv_heads) {
-                    kvh = 0;
-                    first += 16 * QT;
-                    if (first >= sg.M) {
-                        first = 0;
+                first += 16 * QT;
+                bool other = false;
+                if (first >= sg.M) {
+                    first = 0;
+                    if (++kvh == p.kv_heads) {
+                        kvh = 0;
+                        other = true;
                         do {
                             ++which;
                             fetch();
                         } while (ntiles == 0 || sg.M == 0);   // there is a tile left, so there is such a segment
                     }
-                    window();
-                } else if (w.id_base != sg.k0) {
-                    window();
                 }
+                if (other || w.id_base != sg.k0) window();
                 head = (int64_t)kvh * p.head_stride;
             }
             w.load(p.K, w.kf, head, sg.k0 + 32 * rel, sg.k1);
@@ -484,7 +534,8 @@ __global__ __launch_bounds__(256, 2) void paged_attn_stream_kernel(AttnParams p)
         w.step(kv0, now.k1, next_k, next_v);
         if (over || LAST) {
             // a part, or all there is for these rows
-            const int begin = now.start + (now_first / (16 * QT) * p.kv_heads + now_kvh) * now_tiles;   // first tile of these rows
+            const int streams = (now.M + 16 * QT - 1) / (16 * QT);
+            const int begin = now.start + (now_kvh * streams + now_first / (16 * QT)) * (now_tiles + 1) + 1;   // the first tile's place
             const int before = begin / total.per, piece = pos / total.per - before;
             const bool direct = now.whole && (begin + now_tiles - 1) / total.per == before;
             const int slot = (now.limit == SHARED ? 0 : p.slots_p) + piece;
@@ -513,45 +564,47 @@ __global__ __launch_bounds__(256, 2) void paged_attn_stream_kernel(AttnParams p)
             if constexpr (!LAST) w.queries(sg, first, kvh);
         }
     };
-    for (; pos + 1 < end; ++pos) tile(std::false_type{});
+    for (;;) {
+        const int next = pos + (rel + 1 == ntiles ? 2 : 1);
+        if (next >= end) break;
+        tile(std::false_type{});
+        pos = next;
+    }
     tile(std::true_type{});
 }
 
-// Joins the parts of a row that has several, and writes rows without keys: one wave per (row, head).
+// Joins the parts of a row that has several, and writes rows without keys: D / 2 lanes per (row, head).
 template <int D>
 __global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnParams p) {
-    constexpr int PER = D / 64;
-    const int lane = threadIdx.x & 63;
-    const int64_t item = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (item >= (int64_t)p.rows * p.heads) return;
-    const int row = (int)(item / p.heads), hq = (int)(item - (int64_t)row * p.heads), kvh = hq / p.group;
+    constexpr int LANES = D / 2;
+    const int lane = threadIdx.x % LANES;
+    const int number = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;   // rows * heads is below 2^31
+    if (number >= p.rows * p.heads) return;
+    const int row = number / p.heads, hq = number - row * p.heads, kvh = hq / p.group;
+    const int64_t item = number;
     const RowParts rp = p.parts[row];
-    if (!rp.known) return;
     const int per = p.total->per;
+    if (!rp.known) return;
     int count[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
         const int r = (row - rp.r0[k]) * p.group + hq - kvh * p.group;
-        const int begin = rp.start[k] + (r / p.rows_q * p.kv_heads + kvh) * rp.tiles[k];
+        const int begin = rp.start[k] + (kvh * rp.streams[k] + r / p.rows_q) * (rp.tiles[k] + 1) + 1;
         count[k] = rp.tiles[k] > 0 ? (begin + rp.tiles[k] - 1) / per - begin / per + 1 : 0;
     }
     const int np = min(count[0], p.slots_p), n = np + min(count[1], p.slots - p.slots_p);
     if (np == 0 && n == 1) return;   // written already
     auto slot_of = [&](int i) { return item * p.slots + (i < np ? i : p.slots_p + i - np); };
-    float M = -INFINITY, L = 0.f, acc[PER];
-#pragma unroll
-    for (int e = 0; e < PER; ++e) acc[e] = 0.f;
+    float M = -INFINITY, L = 0.f, a0 = 0.f, a1 = 0.f;
     // parts are requested several at a time, behind the last one the last again
     auto turn = [&](int i0, auto ahead, bool maximum_known) {
         constexpr int A = decltype(ahead)::value;
-        float2 ml[A];
-        float v[A][PER];
+        float2 ml[A], v[A];
 #pragma unroll
         for (int a = 0; a < A; ++a) {
             const int64_t at = slot_of(min(i0 + a, n - 1));
             ml[a] = p.part_ml[at];
-#pragma unroll
-            for (int e = 0; e < PER; ++e) v[a][e] = p.part_o[at * D + lane * PER + e];
+            v[a] = *(const float2*)(p.part_o + at * D + lane * 2);
         }
         if (!maximum_known) {
 #pragma unroll
@@ -562,21 +615,22 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnParams p) {
         for (int a = 0; a < A; ++a) {
             const float f = i0 + a < n ? __builtin_amdgcn_exp2f(ml[a].x - use) : 0.f;
             L += ml[a].y * f;
-#pragma unroll
-            for (int e = 0; e < PER; ++e) acc[e] += v[a][e] * f;
+            a0 += v[a].x * f;
+            a1 += v[a].y * f;
         }
     };
-    if (n > 0 && n <= 2) turn(0, std::integral_constant<int, 2>{}, false);
-    else if (n <= 4 && n > 0) turn(0, std::integral_constant<int, 4>{}, false);
-    else if (n > 0) {
-        for (int i = lane; i < n; i += 64) M = fmaxf(M, p.part_ml[slot_of(i)].x);
-        M = wave_max(M);
+    if (n > 4) {
+        for (int i = lane; i < n; i += LANES) M = fmaxf(M, p.part_ml[slot_of(i)].x);
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, LANES));
         for (int i0 = 0; i0 < n; i0 += 8) turn(i0, std::integral_constant<int, 8>{}, true);
+    } else if (n > 2) {
+        turn(0, std::integral_constant<int, 4>{}, false);
+    } else if (n > 0) {
+        turn(0, std::integral_constant<int, 2>{}, false);
     }
     const float inv = inverse_of(L);
-    bf16_t* dst = p.out + (int64_t)row * p.o_ld + hq * D + lane * PER;
-    if constexpr (PER == 2) *(uint32_t*)dst = pack_bf16x2(acc[0] * inv, acc[1] * inv);
-    else *dst = f32_to_bf16(acc[0] * inv);
+    *(uint32_t*)(p.out + (int64_t)row * p.o_ld + hq * D + lane * 2) = pack_bf16x2(a0 * inv, a1 * inv);
     if (p.lse && lane == 0) p.lse[item] = lse_of(M == -INFINITY ? 0.f : M, L);
 }
 
@@ -668,7 +722,8 @@ Plan plan_for(const q3asr_kv_pages& c, const q3asr_attn_batch& b, int heads) {
     r.plain = b.max_len <= PLAIN_KEYS && (int64_t)b.n * r.tiles_q * c.kv_heads <= PLAIN_ITEMS;
     if (r.plain) return r;
     const bool shares = groups_count(c, b);
-    if (shares && (int64_t)b.max_group_rows * group > 16) r.qt = 2;
+    const int64_t rows = (int64_t)(shares ? b.max_group_rows : b.max_rows) * group;
+    r.qt = rows <= 16 ? 1 : rows <= 32 || c.head_dim == 128 ? 2 : 4;   // four times 16 x 128 sums would not fit the registers of two waves
     // Parts of a row: tiles of its longest segment by the least tiles of a wave, and one for where it begins.  More parts spread a few
     // long sequences over the device; their memory is kept to 64 MB (but 16 parts).
     const int64_t part = (int64_t)b.rows * heads * (c.head_dim * 4 + 8);
@@ -680,8 +735,8 @@ Plan plan_for(const q3asr_kv_pages& c, const q3asr_attn_batch& b, int heads) {
     auto round = [](int64_t x) { return (x + 255) & ~255ll; };
     const int64_t groups = shares ? b.n_groups : 0;
     r.at_plan = 256;
-    r.at_segments = r.at_plan + (b.n > HELD || groups > HELD ? round((int64_t)b.n * (int64_t)sizeof(Entry) + groups * 4) : 0);
-    r.at_parts = r.at_segments + round((b.n + groups) * (int64_t)sizeof(Segment));
+    r.at_segments = r.at_plan + (b.n + groups > HELD ? round((int64_t)b.n * (int64_t)sizeof(Entry) + (2 * groups + b.n + 2) * 4) : 0);
+    r.at_parts = r.at_segments + (b.n + groups > HELD ? round((b.n + groups) * (int64_t)sizeof(Segment)) : 0);
     r.at_ml = r.at_parts + round((int64_t)b.rows * (int64_t)sizeof(RowParts));
     r.at_o = r.at_ml + round((int64_t)b.rows * heads * r.slots * 8);
     r.bytes = r.at_o + round((int64_t)b.rows * heads * r.slots * c.head_dim * 4);
@@ -698,13 +753,22 @@ void launch_d(const AttnParams& p, const Plan& r, hipStream_t s) {
         HIP_CHECK(hipGetLastError());
         return;
     }
-    hipLaunchKernelGGL(paged_attn_plan_kernel, dim3(1), dim3(PLAN), 0, s, p);
-    HIP_CHECK(hipGetLastError());
     const dim3 grid(STREAM_WAVES / WAVES);
-    if (r.qt == 1) hipLaunchKernelGGL((paged_attn_stream_kernel<D, 1>), grid, block, 0, s, p);
-    else hipLaunchKernelGGL((paged_attn_stream_kernel<D, 2>), grid, block, 0, s, p);
+    const bool planned = p.n + p.n_groups > HELD;
+    if (planned) {
+        hipLaunchKernelGGL(paged_attn_plan_kernel, dim3(1), dim3(PLAN), 0, s, p);
+        HIP_CHECK(hipGetLastError());
+    }
+    constexpr int MOST = D == 128 ? 2 : 4;
+#define STREAM(QT)                                                                                                  \
+    if (planned) hipLaunchKernelGGL((paged_attn_stream_kernel<D, QT, true>), grid, block, 0, s, p);                 \
+    else hipLaunchKernelGGL((paged_attn_stream_kernel<D, QT, false>), grid, block, 0, s, p)
+    if (r.qt == 1) { STREAM(1); }
+    else if (r.qt == 2) { STREAM(2); }
+    else { STREAM(MOST); }
+#undef STREAM
     HIP_CHECK(hipGetLastError());
-    hipLaunchKernelGGL((paged_attn_join_kernel<D>), dim3(cdiv((int64_t)p.rows * p.heads, 4)), block, 0, s, p);
+    hipLaunchKernelGGL((paged_attn_join_kernel<D>), dim3(cdiv((int64_t)p.rows * p.heads, 256 / (D / 2))), block, 0, s, p);
     HIP_CHECK(hipGetLastError());
 }
 
@@ -740,8 +804,8 @@ void launch_paged_attention(const q3asr_kv_pages& c, int layer, const bf16_t* q,
     p.parts = (RowParts*)(ws + r.at_parts);
     p.part_ml = (float2*)(ws + r.at_ml);
     p.part_o = (float*)(ws + r.at_o);
-    // tile numbers are 32 bits
-    const int64_t group = p.group, own = cdiv(p.max_own, 32), sh = cdiv(p.max_shared, 32);
+    // places are 32-bit numbers
+    const int64_t group = p.group, own = cdiv(p.max_own, 32) + 1, sh = cdiv(p.max_shared, 32) + 1;
     Q3_REQUIRE(r.plain || (own * cdiv((int64_t)b.max_rows * group, 16) * b.n + (shares ? sh * cdiv((int64_t)b.max_group_rows * group, 16) * b.n_groups : 0)) *
                                   c.kv_heads < (1ll << 30),
                "paged_attention: too much work for one call (smaller bounds in the batch make less)");

@@ -353,11 +353,20 @@ __global__ __launch_bounds__(256) void pages_copy_kernel(Pages p) {
 }
 
 // ---- write: one workgroup per row of the step ----
+// All latency: four dependent loads (entry, length, page, its count) lead to the place; the row itself and the search for an earlier
+// entry of the same sequence travel beside them.
 __global__ __launch_bounds__(256) void pages_write_kernel(Pages p, int layer, const bf16_t* k, int64_t k_ld, const bf16_t* v, int64_t v_ld,
                                                           const int* seqs, const int* cu_rows, int n, int rows) {
     const int row = blockIdx.x, tid = threadIdx.x;
+    const int per_head = p.head_dim / 8, chunks = p.kv_heads * per_head;
+    auto source = [&](int c) {
+        const int which = c >= chunks;
+        return (const uint4*)((which ? v + (int64_t)row * v_ld : k + (int64_t)row * k_ld) + (c - which * chunks) * 8);
+    };
+    uint4 first = make_uint4(0, 0, 0, 0);
+    if (tid < 2 * chunks) first = *source(tid);
     // the entry of the list that the row belongs to: the row's own number where every sequence has one row, else by halving
-    int lo = min(row, n - 1), r0 = cu_rows[lo], r1 = cu_rows[lo + 1];
+    int lo = min(row, n - 1), r0 = cu_rows[lo], r1 = cu_rows[lo + 1], seq = seqs[lo];
     if (row < r0 || row >= r1) {
         lo = 0;
         int hi = n;
@@ -368,40 +377,35 @@ __global__ __launch_bounds__(256) void pages_write_kernel(Pages p, int layer, co
         }
         r0 = cu_rows[lo];
         r1 = cu_rows[lo + 1];
+        seq = seqs[lo];
     }
-    if (row < r0 || row >= r1 || r1 > rows) {
-        if (tid == 0) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, lo);
+    bool twice = false;
+    for (int i = tid; i < lo; i += 256) twice |= seqs[i] == seq;
+    twice = __syncthreads_or(twice);
+    int code = Q3ASR_PAGES_OK, page = 0, pos = 0;
+    if (row < r0 || row >= r1 || r1 > rows) code = Q3ASR_PAGES_BAD_BATCH;
+    else if ((unsigned)seq >= (unsigned)p.max_seqs) code = Q3ASR_PAGES_BAD_INDEX;
+    else if (twice) code = Q3ASR_PAGES_DUPLICATE;
+    else {
+        pos = p.lens[seq] - (r1 - row);
+        const int64_t slot = (int64_t)pos / p.page_tokens;
+        if (pos < 0 || slot >= p.max_seq_pages) code = Q3ASR_PAGES_BAD_BATCH;
+        else {
+            page = p.table[(int64_t)seq * p.max_seq_pages + slot];
+            if ((unsigned)page >= (unsigned)p.pages) code = Q3ASR_PAGES_BAD_INDEX;
+            else if (p.refs[page] != 1) code = Q3ASR_PAGES_BAD_BATCH;
+        }
+    }
+    if (code != Q3ASR_PAGES_OK) {   // the same for the whole workgroup
+        if (tid == 0) pages_error(p.status, code, lo);
         return;
     }
-    const int seq = seqs[lo];
-    if ((unsigned)seq >= (unsigned)p.max_seqs) {
-        if (tid == 0) pages_error(p.status, Q3ASR_PAGES_BAD_INDEX, lo);
-        return;
-    }
-    __shared__ int twice;
-    if (tid == 0) twice = 0;
-    __syncthreads();
-    for (int i = tid; i < lo; i += 256)
-        if (seqs[i] == seq) twice = 1;
-    __syncthreads();
-    const int pos = p.lens[seq] - (r1 - row);
-    const int64_t slot = (int64_t)pos / p.page_tokens;
-    if (twice || pos < 0 || slot >= p.max_seq_pages) {
-        if (tid == 0) pages_error(p.status, twice ? Q3ASR_PAGES_DUPLICATE : Q3ASR_PAGES_BAD_BATCH, lo);
-        return;
-    }
-    const int page = p.table[(int64_t)seq * p.max_seq_pages + slot];
-    if ((unsigned)page >= (unsigned)p.pages || p.refs[page] != 1) {
-        if (tid == 0) pages_error(p.status, (unsigned)page >= (unsigned)p.pages ? Q3ASR_PAGES_BAD_INDEX : Q3ASR_PAGES_BAD_BATCH, lo);
-        return;
-    }
-    const int per_head = p.head_dim / 8, chunks = p.kv_heads * per_head, token = pos & (p.page_tokens - 1);
+    const int token = pos & (p.page_tokens - 1);
     const int64_t base = ((int64_t)layer * p.pages + page) * p.kv_heads;
     for (int c = tid; c < 2 * chunks; c += 256) {
         const int which = c >= chunks, cc = c - which * chunks, h = cc / per_head, d = (cc - h * per_head) * 8;
-        const bf16_t* src = (which ? v + (int64_t)row * v_ld : k + (int64_t)row * k_ld) + h * p.head_dim + d;
         bf16_t* pool = which ? p.kv[1] : p.kv[0];
-        *(uint4*)(pool + ((base + h) * p.page_tokens + token) * p.head_dim + d) = *(const uint4*)src;
+        *(uint4*)(pool + ((base + h) * p.page_tokens + token) * p.head_dim + d) = c == tid ? first : *source(c);
     }
 }
 
