@@ -124,7 +124,7 @@ __device__ __forceinline__ Entry entry_of(const AttnParams& p, int i, bool repor
 // Where every segment's tiles begin, from the lengths.  Up to HELD groups and sequences every workgroup finds out for itself, in LDS
 // (two dependent loads per sequence, its number and its length, and no launch of its own); beyond that one workgroup does it
 // for all, in the workspace.  tell: errors are reported and the rows' parts written down, by one workgroup of all.
-constexpr int HELD = 1024;
+constexpr int HELD = 1024;   // as a launch of its own the plan costs 6 us, in front of every wave 4
 struct PlanMemory {
     Entry* entry;            // [n]
     int *from, *cu, *rows;   // [n_groups] tokens that a group shares, [n_groups + 1], [n + 1]: of the batch
@@ -723,7 +723,9 @@ Plan plan_for(const q3asr_kv_pages& c, const q3asr_attn_batch& b, int heads) {
     if (r.plain) return r;
     const bool shares = groups_count(c, b);
     const int64_t rows = (int64_t)(shares ? b.max_group_rows : b.max_rows) * group;
-    r.qt = rows <= 16 ? 1 : rows <= 32 || c.head_dim == 128 ? 2 : 4;   // four times 16 x 128 sums would not fit the registers of two waves
+    // as many rows at once as the registers of two waves per SIMD hold (64 x 128 sums do not fit; 64 x 64 against 32 x 64 at three
+    // waves: 34 against 39 us for 7 x 24 rows after 1111 tokens, 12 groups, 14 heads)
+    r.qt = rows <= 16 ? 1 : rows <= 32 || c.head_dim == 128 ? 2 : 4;
     // Parts of a row: tiles of its longest segment by the least tiles of a wave, and one for where it begins.  More parts spread a few
     // long sequences over the device; their memory is kept to 64 MB (but 16 parts).
     const int64_t part = (int64_t)b.rows * heads * (c.head_dim * 4 + 8);

@@ -9,6 +9,8 @@
 #include <algorithm>
 #include <climits>
 
+typedef __attribute__((ext_vector_type(4))) int i32x4;
+
 namespace {
 
 constexpr int PLAN = 1024;   // threads of a planning workgroup
@@ -24,7 +26,13 @@ Pages device_pages(const q3asr_kv_pages& c) {
                  c.max_seqs, c.max_seq_pages};
 }
 
-// Workspace, in 4-byte words: [0] entries of the copy list, [1] 1 where a call goes on to its second kernel, [16...) the parts below.
+// What an entry of reserve's list needs.
+struct __attribute__((aligned(16))) Need {
+    int seq, tokens, fill, page;        // fill, page: of the last page if tokens are added to a partly filled one, else fill 0
+    int old_pages, new_pages, start, copy;   // start: rank of its first new page; copy: 0, or 1 + rank among the copies
+};
+
+// Workspace, in 4-byte words: [0] entries of the copy list, [1] 1 where a call goes on in its next kernel, [16...) the parts below.
 struct Layout {
     int64_t rows, row_lens, need, copies, free, per_page, total;
 };
@@ -32,35 +40,47 @@ __host__ __device__ inline Layout layout(int pages, int max_seqs, int max_seq_pa
     Layout l;
     l.rows = 16;                                              // fork: the new table rows; reserve: marks of the named sequences
     l.row_lens = l.rows + (int64_t)max_seqs * max_seq_pages;  // fork: their lengths and marks
-    l.need = l.row_lens + 2 * (int64_t)max_seqs;              // reserve: first free page of an entry, and whether it copies
-    l.copies = l.need + max_seqs;                             // (from, to, tokens) of every copy
+    l.need = (l.row_lens + 2 * (int64_t)max_seqs + 3) & ~3ll;
+    l.copies = l.need + 8 * (int64_t)max_seqs;                // (from, to, tokens) of every copy
     l.free = l.copies + 3 * (int64_t)(max_seqs > pages ? max_seqs : pages);
     l.per_page = l.free + pages;                              // reserve: holders in the list and the first; compact: new number
     l.total = l.per_page + 2 * (int64_t)pages;
     return l;
 }
 
-// Exclusive prefix sum over the workgroup's threads, and the total.
-__device__ __forceinline__ int block_scan(int v, int* total, int* lds) {
+// Exclusive prefix sums over the workgroup's threads, and the totals.  Wanted pages need 64 bits: 1024 entries of 2^27.
+struct Sums {
+    long long wanted;
+    int copies;
+};
+__device__ __forceinline__ Sums block_scan(Sums v, Sums* total, Sums* lds) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int x = v;
+    Sums x = v;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-        const int t = __shfl_up(x, o, 64);
-        if (lane >= o) x += t;
+        const long long a = __shfl_up(x.wanted, o, 64);
+        const int b = __shfl_up(x.copies, o, 64);
+        if (lane >= o) {
+            x.wanted += a;
+            x.copies += b;
+        }
     }
     __syncthreads();
     if (lane == 63) lds[wave] = x;
     __syncthreads();
-    int before = 0, all = 0;
+    Sums before{0, 0}, all{0, 0};
 #pragma unroll
     for (int w = 0; w < PLAN / 64; ++w) {
-        const int t = lds[w];
-        before += w < wave ? t : 0;
-        all += t;
+        const Sums t = lds[w];
+        if (w < wave) {
+            before.wanted += t.wanted;
+            before.copies += t.copies;
+        }
+        all.wanted += t.wanted;
+        all.copies += t.copies;
     }
     *total = all;
-    return before + x - v;
+    return Sums{before.wanted + x.wanted - v.wanted, before.copies + x.copies - v.copies};
 }
 
 // A word that atomics of this kernel have changed: read where they are performed, past the compute unit's own cache.
@@ -80,11 +100,15 @@ __global__ __launch_bounds__(256) void pages_reset_kernel(Pages p) {
 __global__ void pages_clear_status_kernel(int* status) { if (threadIdx.x < 4) status[threadIdx.x] = 0; }
 
 // ---- fork ----
-__global__ __launch_bounds__(PLAN) void pages_fork_kernel(Pages p, const int* dst, const int* src, int n) {
+// One workgroup checks the list; short ones (up to FORK_HELD table entries) it carries out as well, with the rows to come in
+// registers between reading all old rows and writing the new ones.  Longer ones go on in two kernels over the whole device, with the
+// rows in the workspace.
+constexpr int FORK_ROUNDS = 2, FORK_HELD = FORK_ROUNDS * PLAN;
+
+__global__ __launch_bounds__(PLAN) void pages_fork_kernel(Pages p, const int* dst, const int* src, int n, int held) {
     __shared__ int worst;
     const int tid = threadIdx.x, width = p.max_seq_pages;
-    const Layout l = layout(p.pages, p.max_seqs, width);
-    int *rows = p.ws + l.rows, *row_lens = p.ws + l.row_lens, *mark = row_lens + p.max_seqs;
+    int* const mark = p.ws + layout(p.pages, p.max_seqs, width).row_lens + p.max_seqs;
     if (tid == 0) worst = INT_MAX;
     __syncthreads();
     for (int i = tid; i < n; i += PLAN) {
@@ -99,166 +123,220 @@ __global__ __launch_bounds__(PLAN) void pages_fork_kernel(Pages p, const int* ds
     }
     __syncthreads();
     if (worst != INT_MAX) {   // the same for the whole workgroup
-        if (tid == 0) pages_error(p.status, worst & 7, worst >> 3);
+        if (tid == 0) {
+            pages_error(p.status, worst & 7, worst >> 3);
+            p.ws[1] = 0;
+        }
         return;
     }
-    // the rows to come, from the table as it was; counts of the pages that come and go
-    const int64_t total = (int64_t)n * width;
-    for (int64_t e = tid; e < total; e += PLAN) {
-        const int i = (int)(e / width), j = (int)(e - (int64_t)i * width);
+    if (!held) {
+        if (tid == 0) p.ws[1] = 1;
+        return;
+    }
+    const int total = n * width;
+    const unsigned magic = 0xffffffffu / (unsigned)width + 1;   // e / width = e * magic >> 32 for these few e
+    int now[FORK_ROUNDS], old[FORK_ROUNDS], at[FORK_ROUNDS];
+#pragma unroll
+    for (int k = 0; k < FORK_ROUNDS; ++k) {
+        const int e = tid + k * PLAN;
+        now[k] = old[k] = at[k] = -1;
+        if (e < total) {
+            const int i = width > 1 ? (int)__umulhi((unsigned)e, magic) : e, j = e - i * width, s = src ? src[i] : -1;
+            at[k] = dst[i] * width + j;   // below 2^31: the table has fewer entries
+            if (s >= 0) now[k] = p.table[s * width + j];
+            old[k] = p.table[at[k]];
+        }
+    }
+    int lens = 0;
+    if (tid < n && src && src[tid] >= 0) lens = p.lens[src[tid]];
+    __syncthreads();          // every old row and length has been read
+#pragma unroll
+    for (int k = 0; k < FORK_ROUNDS; ++k)
+        if (at[k] >= 0) {
+            p.table[at[k]] = now[k];
+            if ((unsigned)now[k] < (unsigned)p.pages) atomicAdd(&p.refs[now[k]], 1);
+            if ((unsigned)old[k] < (unsigned)p.pages) atomicSub(&p.refs[old[k]], 1);
+        }
+    if (tid < n) p.lens[dst[tid]] = lens;
+}
+
+__global__ __launch_bounds__(256) void pages_fork_read_kernel(Pages p, const int* dst, const int* src, int n) {
+    if (p.ws[1] == 0) return;
+    const int width = p.max_seq_pages;
+    const Layout l = layout(p.pages, p.max_seqs, width);
+    int *rows = p.ws + l.rows, *row_lens = p.ws + l.row_lens;
+    const int lane = threadIdx.x & 63;
+    for (int i = blockIdx.x * 4 + (threadIdx.x >> 6); i < n; i += gridDim.x * 4) {
         const int s = src ? src[i] : -1;
-        const int now = s < 0 ? -1 : p.table[(int64_t)s * width + j], old = p.table[(int64_t)dst[i] * width + j];
-        rows[e] = now;
-        if ((unsigned)now < (unsigned)p.pages) atomicAdd(&p.refs[now], 1);
-        if ((unsigned)old < (unsigned)p.pages) atomicSub(&p.refs[old], 1);
+        const int64_t to = (int64_t)dst[i] * width, from = (int64_t)s * width;
+        for (int j = lane; j < width; j += 64) {
+            const int now = s < 0 ? -1 : p.table[from + j], old = p.table[to + j];
+            rows[(int64_t)i * width + j] = now;
+            if ((unsigned)now < (unsigned)p.pages) atomicAdd(&p.refs[now], 1);
+            if ((unsigned)old < (unsigned)p.pages) atomicSub(&p.refs[old], 1);
+        }
+        if (lane == 0) row_lens[i] = s < 0 ? 0 : p.lens[s];
     }
-    for (int i = tid; i < n; i += PLAN) {
-        const int s = src ? src[i] : -1;
-        row_lens[i] = s < 0 ? 0 : p.lens[s];
+}
+__global__ __launch_bounds__(256) void pages_fork_write_kernel(Pages p, const int* dst, int n) {
+    if (p.ws[1] == 0) return;
+    const int width = p.max_seq_pages;
+    const Layout l = layout(p.pages, p.max_seqs, width);
+    const int *rows = p.ws + l.rows, *row_lens = p.ws + l.row_lens;
+    const int lane = threadIdx.x & 63;
+    for (int i = blockIdx.x * 4 + (threadIdx.x >> 6); i < n; i += gridDim.x * 4) {
+        const int64_t to = (int64_t)dst[i] * width;
+        for (int j = lane; j < width; j += 64) p.table[to + j] = rows[(int64_t)i * width + j];
+        if (lane == 0) p.lens[dst[i]] = row_lens[i];
     }
-    __syncthreads();
-    for (int64_t e = tid; e < total; e += PLAN) {
-        const int i = (int)(e / width), j = (int)(e - (int64_t)i * width);
-        p.table[(int64_t)dst[i] * width + j] = rows[e];
-    }
-    for (int i = tid; i < n; i += PLAN) p.lens[dst[i]] = row_lens[i];
 }
 
 // ---- reserve ----
-// What an entry of the list needs.
-struct Need {
-    int seq, fill, last, page, old_pages, new_pages;
-    bool partly;   // adds to a page that is partly filled
-};
-__device__ __forceinline__ Need need_of(const Pages& p, int seq, int add) {
-    Need r;
-    r.seq = seq;
-    const int len = p.lens[seq], pt = p.page_tokens;
-    r.fill = len & (pt - 1);
-    r.partly = r.fill > 0 && add > 0;
-    r.old_pages = (len + pt - 1) / pt;
-    r.new_pages = (int)(((int64_t)len + add + pt - 1) / pt);
-    r.last = r.old_pages - 1;
-    r.page = r.partly ? p.table[(int64_t)seq * p.max_seq_pages + r.last] : 0;
-    return r;
-}
+constexpr int HELD_STARTS = 2048, HELD_FREE = 4096;
 
 __global__ __launch_bounds__(PLAN) void pages_reserve_kernel(Pages p, const int* seqs, const int* tokens, int n) {
-    __shared__ int worst, scan[PLAN / 64], wave_free[PLAN / 64];
+    __shared__ int worst, wave_free[PLAN / 64];
+    __shared__ Sums scan[PLAN / 64];
+    __shared__ int held_start[HELD_STARTS], held_free[HELD_FREE];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, width = p.max_seq_pages, pt = p.page_tokens;
     const Layout l = layout(p.pages, p.max_seqs, width);
-    int *mark = p.ws + l.rows, *need = p.ws + l.need, *copies = p.ws + l.copies, *free = p.ws + l.free;
+    int *mark = p.ws + l.rows, *copies = p.ws + l.copies;
     int *here = p.ws + l.per_page, *first = here + p.pages;
+    Need* const need = (Need*)(p.ws + l.need);
+    // free pages, counted by every wave over a contiguous span of the pool
+    const int span = ((p.pages + PLAN / 64 - 1) / (PLAN / 64) + 63) & ~63;
+    const int s0 = wave * span, s1 = min(p.pages, s0 + span);
+    int mine = 0;
+    for (int q = s0 + lane; q < s1; q += 64) mine += p.refs[q] == 0;
     if (tid == 0) {
         worst = INT_MAX;
         p.ws[0] = 0;
     }
     __syncthreads();
+    // what every entry needs; a thread keeps its first one in registers
+    Need own{};
     for (int i = tid; i < n; i += PLAN) {
-        const int s = seqs[i], add = tokens[i];
-        if ((unsigned)s >= (unsigned)p.max_seqs || add < 0) {
-            note(&worst, i, Q3ASR_PAGES_BAD_INDEX);
-            continue;
+        Need r{};
+        r.seq = seqs[i];
+        r.tokens = tokens[i];
+        int code = Q3ASR_PAGES_OK;
+        if ((unsigned)r.seq >= (unsigned)p.max_seqs || r.tokens < 0) code = Q3ASR_PAGES_BAD_INDEX;
+        else {
+            mark[r.seq] = i;
+            const int len = p.lens[r.seq];
+            if (len < 0 || (int64_t)len + r.tokens > (int64_t)width * pt) code = Q3ASR_PAGES_TOO_LONG;
+            else {
+                r.old_pages = (len + pt - 1) / pt;
+                r.new_pages = (len + r.tokens + pt - 1) / pt;   // both below 2^31 - pt: a table's tokens are
+                r.fill = r.tokens > 0 ? len & (pt - 1) : 0;
+                if (r.fill) {
+                    r.page = p.table[(int64_t)r.seq * width + r.old_pages - 1];
+                    if ((unsigned)r.page >= (unsigned)p.pages) code = Q3ASR_PAGES_BAD_INDEX;
+                    else {
+                        here[r.page] = 0;
+                        first[r.page] = INT_MAX;
+                    }
+                }
+            }
         }
-        mark[s] = i;
-        const int len = p.lens[s];
-        if (len < 0 || (int64_t)len + add > (int64_t)width * pt) {
-            note(&worst, i, Q3ASR_PAGES_TOO_LONG);
-            continue;
-        }
-        const Need r = need_of(p, s, add);
-        if ((unsigned)r.page >= (unsigned)p.pages) note(&worst, i, Q3ASR_PAGES_BAD_INDEX);
-        else if (r.partly) {
-            here[r.page] = 0;
-            first[r.page] = INT_MAX;
-        }
+        if (code != Q3ASR_PAGES_OK) note(&worst, i, code);
+        if (i == tid) own = r;
+        else need[i] = r;
     }
     __syncthreads();
-    for (int i = tid; i < n; i += PLAN)
-        if ((unsigned)seqs[i] < (unsigned)p.max_seqs && mark[seqs[i]] != i) note(&worst, i, Q3ASR_PAGES_DUPLICATE);
+    auto entry = [&](int i) { return i == tid ? own : need[i]; };
+    for (int i = tid; i < n; i += PLAN) {
+        const int s = seqs[i];
+        if ((unsigned)s < (unsigned)p.max_seqs && mark[s] != i) note(&worst, i, Q3ASR_PAGES_DUPLICATE);
+    }
     __syncthreads();
     if (worst != INT_MAX) {
         if (tid == 0) pages_error(p.status, worst & 7, worst >> 3);
         return;
     }
     for (int i = tid; i < n; i += PLAN) {
-        const Need r = need_of(p, seqs[i], tokens[i]);
-        if (!r.partly) continue;
+        const Need r = entry(i);
+        if (!r.fill) continue;
         atomicAdd(&here[r.page], 1);
         atomicMin(&first[r.page], i);
     }
-    __syncthreads();
-    // pages wanted: one for a copy, one for every page begun; ranks in the order of the list
-    int64_t carry = 0;
-    int copied = 0;
-    for (int i0 = 0; i0 < n; i0 += PLAN) {
-        const int i = i0 + tid;
-        int want = 0, copy = 0;
-        if (i < n) {
-            const Need r = need_of(p, seqs[i], tokens[i]);
-            if (r.partly) {
-                const int refs = p.refs[r.page];
-                copy = refs > 1 && !(counted(&here[r.page]) == refs && counted(&first[r.page]) == i);
-            }
-            want = copy + r.new_pages - r.old_pages;
-        }
-        int total, copies_total;
-        const int before = block_scan(want, &total, scan);
-        const int rank = block_scan(copy, &copies_total, scan);
-        if (i < n) {
-            // fewer than 2^30 pages are wanted before this entry, or the call is refused below
-            need[i] = (int)(min(carry + before, (int64_t)0x3fffffff) << 1) | copy;
-            if (copy) copies[3 * (copied + rank)] = i;
-        }
-        carry += total;
-        copied += copies_total;
-    }
-    // the lowest `carry` free pages: every wave counts, then lists, a contiguous span of the pool
-    const int span = ((p.pages + PLAN / 64 - 1) / (PLAN / 64) + 63) & ~63;
-    const int s0 = wave * span, s1 = min(p.pages, s0 + span);
-    int mine = 0;
-    for (int q = s0 + lane; q < s1; q += 64) mine += p.refs[q] == 0;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) mine += __shfl_xor(mine, o, 64);
     if (lane == 0) wave_free[wave] = mine;
     __syncthreads();
+    // pages wanted: one for a copy, one for every page begun; ranks in the order of the list
+    long long carry = 0;
+    int copied = 0;
+    for (int i0 = 0; i0 < n; i0 += PLAN) {
+        const int i = i0 + tid;
+        int copy = 0;
+        Need r{};
+        if (i < n) {
+            r = entry(i);
+            if (r.fill) {
+                const int refs = p.refs[r.page];
+                copy = refs > 1 && !(counted(&here[r.page]) == refs && counted(&first[r.page]) == i);
+            }
+        }
+        Sums total;
+        const Sums before = block_scan(Sums{copy + r.new_pages - r.old_pages, copy}, &total, scan);
+        if (i < n) {
+            r.start = (int)min(carry + before.wanted, (long long)INT_MAX);   // a call that wants so many pages is refused below
+            r.copy = copy ? 1 + copied + before.copies : 0;
+            if (i == tid) own = r;
+            need[i] = r;
+            if (i < HELD_STARTS) held_start[i] = r.start;
+        }
+        carry += total.wanted;
+        copied += total.copies;
+    }
+    // the lowest `carry` free pages
     int at = 0, all = 0;
     for (int w = 0; w < PLAN / 64; ++w) {
         at += w < wave ? wave_free[w] : 0;
         all += wave_free[w];
     }
     if (carry > all) {
-        if (tid == 0) pages_error(p.status, Q3ASR_PAGES_NO_PAGES, n, (int)min(carry - all, (int64_t)INT_MAX));
+        if (tid == 0) pages_error(p.status, Q3ASR_PAGES_NO_PAGES, n, (int)min(carry - all, (long long)INT_MAX));
         return;
     }
-    for (int q0 = s0; q0 < s1 && at < carry; q0 += 64) {
+    const int pages = (int)carry;
+    int* const free = pages <= HELD_FREE ? held_free : p.ws + l.free;
+    for (int q0 = s0; q0 < s1 && at < pages; q0 += 64) {
         const bool is = q0 + lane < s1 && p.refs[q0 + lane] == 0;
         const unsigned long long m = __ballot(is);
         const int k = at + __popcll(m & ((1ull << lane) - 1));
-        if (is && k < carry) free[k] = q0 + lane;
+        if (is && k < pages) free[k] = q0 + lane;
         at += __popcll(m);
     }
     __syncthreads();
-    for (int64_t k = tid; k < carry; k += PLAN) p.refs[free[k]] = 1;
-    // table entries of the new pages, by waves: one entry of the list at a time
-    for (int i = wave; i < n; i += PLAN / 64) {
-        const Need r = need_of(p, seqs[i], tokens[i]);
-        const int start = (need[i] >> 1) + (need[i] & 1);
-        for (int j = r.old_pages + lane; j < r.new_pages; j += 64)
-            p.table[(int64_t)r.seq * width + j] = free[start + j - r.old_pages];
+    // every page goes to the last entry that starts at or before its rank (those that want none start where the next one does)
+    const bool in_lds = n <= HELD_STARTS;
+    for (int k = tid; k < pages; k += PLAN) {
+        int lo = 0, hi = n;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if ((in_lds ? held_start[mid] : need[mid].start) <= k) lo = mid;
+            else hi = mid;
+        }
+        const Need r = need[lo];
+        const int to = free[k], j = k - r.start;
+        p.refs[to] = 1;
+        if (r.copy && j == 0) {
+            int* c = copies + 3 * (r.copy - 1);
+            c[0] = r.page;
+            c[1] = to;
+            c[2] = r.fill;
+            atomicSub(&p.refs[r.page], 1);
+            p.table[(int64_t)r.seq * width + r.old_pages - 1] = to;
+        } else {
+            p.table[(int64_t)r.seq * width + r.old_pages + j - (r.copy ? 1 : 0)] = to;
+        }
     }
-    for (int k = tid; k < copied; k += PLAN) {
-        const int i = copies[3 * k];
-        const Need r = need_of(p, seqs[i], tokens[i]);
-        const int to = free[need[i] >> 1];
-        copies[3 * k] = r.page;
-        copies[3 * k + 1] = to;
-        copies[3 * k + 2] = r.fill;
-        atomicSub(&p.refs[r.page], 1);
-        p.table[(int64_t)r.seq * width + r.last] = to;
+    for (int i = tid; i < n; i += PLAN) {
+        const Need r = entry(i);
+        if (r.tokens) p.lens[r.seq] += r.tokens;
     }
-    __syncthreads();
-    for (int i = tid; i < n; i += PLAN) p.lens[seqs[i]] += tokens[i];
     if (tid == 0) p.ws[0] = copied;
 }
 
@@ -321,34 +399,44 @@ __global__ __launch_bounds__(PLAN) void pages_compact_kernel(Pages p) {
     }
 }
 
-__global__ __launch_bounds__(256) void pages_renumber_kernel(Pages p) {
-    if (p.ws[0] == 0) return;
-    const Layout l = layout(p.pages, p.max_seqs, p.max_seq_pages);
-    const int* to = p.ws + l.per_page;
-    const int64_t n = (int64_t)p.max_seqs * p.max_seq_pages;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const int q = p.table[i];
-        if ((unsigned)q < (unsigned)p.pages && to[q] != q) p.table[i] = to[q];
-    }
-}
-
 // ---- copies of page contents: one wave per (K or V, page, layer, head), a run of filled tokens that is contiguous on both sides ----
-__global__ __launch_bounds__(256) void pages_copy_kernel(Pages p) {
+// Bound by HBM, as a large copy is.  RENUMBER: page numbers of the table change on the way (compact).
+constexpr int COPY_THREADS = 512;
+template <bool RENUMBER>
+__global__ __launch_bounds__(COPY_THREADS) void pages_copy_kernel(Pages p) {
     const int copies = p.ws[0];
-    const int* list = p.ws + layout(p.pages, p.max_seqs, p.max_seq_pages).copies;
+    if (copies == 0) return;
+    const Layout l = layout(p.pages, p.max_seqs, p.max_seq_pages);
+    const int* list = p.ws + l.copies;
+    if constexpr (RENUMBER) {
+        const int* to = p.ws + l.per_page;
+        const int64_t n = (int64_t)p.max_seqs * p.max_seq_pages;
+        for (int64_t i = (int64_t)blockIdx.x * COPY_THREADS + threadIdx.x; i < n; i += (int64_t)gridDim.x * COPY_THREADS) {
+            const int q = p.table[i];
+            if ((unsigned)q < (unsigned)p.pages && to[q] != q) p.table[i] = to[q];
+        }
+    }
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int runs = p.layers * p.kv_heads;
     const int64_t items = (int64_t)copies * runs * 2, head = (int64_t)p.page_tokens * p.head_dim;
-    for (int64_t it = (int64_t)blockIdx.x * 4 + wave; it < items; it += (int64_t)gridDim.x * 4) {
+    constexpr int PER = COPY_THREADS / 64;
+    for (int64_t it = (int64_t)blockIdx.x * PER + wave; it < items; it += (int64_t)gridDim.x * PER) {
         const int which = (int)(it & 1);
         const int k = (int)((it >> 1) / runs), run = (int)((it >> 1) - (int64_t)k * runs);
         const int layer = run / p.kv_heads, h = run - layer * p.kv_heads;
         const int from = list[3 * k], to = list[3 * k + 1], chunks = list[3 * k + 2] * (p.head_dim / 8);
         const int64_t base = (int64_t)layer * p.pages;
         bf16_t* pool = which ? p.kv[1] : p.kv[0];
-        const uint4* a = (const uint4*)(pool + ((base + from) * p.kv_heads + h) * head);
-        uint4* b = (uint4*)(pool + ((base + to) * p.kv_heads + h) * head);
-        for (int c = lane; c < chunks; c += 64) b[c] = a[c];
+        const i32x4* a = (const i32x4*)(pool + ((base + from) * p.kv_heads + h) * head);
+        i32x4* b = (i32x4*)(pool + ((base + to) * p.kv_heads + h) * head);
+        for (int c = lane; c < chunks; c += 256) {   // 4 KB under way at a time
+            const int last = chunks - 1;
+            const i32x4 v0 = a[c], v1 = a[min(c + 64, last)], v2 = a[min(c + 128, last)], v3 = a[min(c + 192, last)];
+            b[c] = v0;
+            if (c + 64 < chunks) b[c + 64] = v1;
+            if (c + 128 < chunks) b[c + 128] = v2;
+            if (c + 192 < chunks) b[c + 192] = v3;
+        }
     }
 }
 
@@ -410,11 +498,13 @@ __global__ __launch_bounds__(256) void pages_write_kernel(Pages p, int layer, co
 }
 
 // Copies take what the list holds; a grid that fills the device when it is long and ends at once when it is empty.
+template <bool RENUMBER>
 void launch_copies(const Pages& p, int64_t most, hipStream_t s) {
-    const int64_t items = most * p.layers * p.kv_heads * 2;
+    const int64_t items = std::max<int64_t>(most * p.layers * p.kv_heads * 2, RENUMBER ? 1 : 0);
     if (items <= 0) return;
     ProfScope ps("pages_copy_kernel", 0, s);
-    hipLaunchKernelGGL(pages_copy_kernel, dim3((int)std::min<int64_t>(cdiv(items, 4), 8 * device_cus())), dim3(256), 0, s, p);
+    const int grid = (int)std::min<int64_t>(cdiv(items, COPY_THREADS / 64), 4 * device_cus());
+    hipLaunchKernelGGL((pages_copy_kernel<RENUMBER>), dim3(grid), dim3(COPY_THREADS), 0, s, p);
     HIP_CHECK(hipGetLastError());
 }
 
@@ -438,7 +528,15 @@ void launch_pages_clear_status(const q3asr_kv_pages& c, hipStream_t s) {
 void launch_pages_fork(const q3asr_kv_pages& c, const int* dst, const int* src, int n, hipStream_t s) {
     const Pages p = device_pages(c);
     ProfScope ps("pages_fork_kernel", 12.0 * n * c.max_seq_pages, s);
-    hipLaunchKernelGGL(pages_fork_kernel, dim3(1), dim3(PLAN), 0, s, p, dst, src, n);
+    // the register form also needs an entry per thread and table offsets of 31 bits
+    const bool held = (int64_t)n * c.max_seq_pages <= FORK_HELD && n <= PLAN && (int64_t)c.max_seqs * c.max_seq_pages < (1ll << 31);
+    hipLaunchKernelGGL(pages_fork_kernel, dim3(1), dim3(PLAN), 0, s, p, dst, src, n, (int)held);
+    HIP_CHECK(hipGetLastError());
+    if (held) return;
+    const dim3 grid(std::min(cdiv(n, 4), 4 * device_cus()));
+    hipLaunchKernelGGL(pages_fork_read_kernel, grid, dim3(256), 0, s, p, dst, src, n);
+    HIP_CHECK(hipGetLastError());
+    hipLaunchKernelGGL(pages_fork_write_kernel, grid, dim3(256), 0, s, p, dst, n);
     HIP_CHECK(hipGetLastError());
 }
 
@@ -449,7 +547,7 @@ void launch_pages_reserve(const q3asr_kv_pages& c, const int* seqs, const int* t
         hipLaunchKernelGGL(pages_reserve_kernel, dim3(1), dim3(PLAN), 0, s, p, seqs, tokens, n);
         HIP_CHECK(hipGetLastError());
     }
-    launch_copies(p, n, s);
+    launch_copies<false>(p, n, s);
 }
 
 void launch_pages_compact(const q3asr_kv_pages& c, hipStream_t s) {
@@ -459,10 +557,7 @@ void launch_pages_compact(const q3asr_kv_pages& c, hipStream_t s) {
         hipLaunchKernelGGL(pages_compact_kernel, dim3(1), dim3(PLAN), 0, s, p);
         HIP_CHECK(hipGetLastError());
     }
-    const int64_t n = (int64_t)c.max_seqs * c.max_seq_pages;
-    hipLaunchKernelGGL(pages_renumber_kernel, dim3((int)std::min<int64_t>((n + 255) / 256, 1024)), dim3(256), 0, s, p);
-    HIP_CHECK(hipGetLastError());
-    launch_copies(p, c.pages / 2, s);
+    launch_copies<true>(p, c.pages / 2, s);
 }
 
 void launch_pages_write(const q3asr_kv_pages& c, int layer, const bf16_t* k, int64_t k_ld, const bf16_t* v, int64_t v_ld,
