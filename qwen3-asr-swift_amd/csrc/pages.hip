@@ -431,11 +431,18 @@ __global__ __launch_bounds__(COPY_THREADS) void pages_copy_kernel(Pages p) {
         i32x4* b = (i32x4*)(pool + ((base + to) * p.kv_heads + h) * head);
         for (int c = lane; c < chunks; c += 256) {   // 4 KB under way at a time
             const int last = chunks - 1;
-            const i32x4 v0 = a[c], v1 = a[min(c + 64, last)], v2 = a[min(c + 128, last)], v3 = a[min(c + 192, last)];
-            b[c] = v0;
-            if (c + 64 < chunks) b[c + 64] = v1;
-            if (c + 128 < chunks) b[c + 128] = v2;
-            if (c + 192 < chunks) b[c + 192] = v3;
+            // compact reads and writes every page once (past the caches: 16 / 12 sequences' turnover 554 against 571 us); a
+            // prompt's last page is read for each of its heirs
+            auto get = [&](int at) { return RENUMBER ? __builtin_nontemporal_load(a + at) : a[at]; };
+            auto put = [&](int at, i32x4 v) {
+                if (RENUMBER) __builtin_nontemporal_store(v, b + at);
+                else b[at] = v;
+            };
+            const i32x4 v0 = get(c), v1 = get(min(c + 64, last)), v2 = get(min(c + 128, last)), v3 = get(min(c + 192, last));
+            put(c, v0);
+            if (c + 64 < chunks) put(c + 64, v1);
+            if (c + 128 < chunks) put(c + 128, v2);
+            if (c + 192 < chunks) put(c + 192, v3);
         }
     }
 }
