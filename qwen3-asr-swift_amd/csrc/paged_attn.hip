@@ -11,7 +11,7 @@
 // they stand the B fragment of O^T = V^T P^T, whose A fragments are transposing reads of the V rows in the same LDS tile.  The
 // next tile's rows are requested as soon as this one's have left their registers.
 //
-//   plain   few rows: a workgroup per sequence and KV head, its four waves taking tiles in turn; one launch, nothing shared
+//   plain   few rows: a workgroup per sequence and KV head, its eight waves taking tiles in turn; one launch, nothing shared
 //   stream  the tiles of all sequences and groups in one row, cut into equal parts, one per wave of a full device: no wave waits for
 //           another, and each has a tile in flight all the time.  Where a wave goes over to other rows counts like a tile.  Two
 //           launches: the waves, which find out first where every sequence's tiles begin, and the join of what was cut.
@@ -88,7 +88,7 @@ struct AttnParams {
     int n, rows, n_groups, heads, kv_heads, group;
     int max_rows, max_group_rows, max_len, max_own, max_shared;
     float scale_log2;
-    int rows_q;                                // query rows of a wave: 16 * QT
+    int shift_q;                               // query rows of a wave: 16 * QT = 1 << shift_q
     int tiles_q;                               // plain: query tiles of a sequence
     int per_min, slots_p, slots;               // parts of a row at most: of its group's segment first
     Total* total;
@@ -197,7 +197,7 @@ __device__ __forceinline__ Total plan_segments(const AttnParams& p, const PlanMe
             sg = Segment{e.r0, e.T * p.group, e.seq, behind, behind + min(max(0, e.len - behind), p.max_own), e.len - e.T + 1, 0, behind == 0};
         }
         const int tiles = (sg.k1 - sg.k0 + 31) >> 5;
-        const int streams = (sg.M + p.rows_q - 1) / p.rows_q;
+        const int streams = (sg.M + (1 << p.shift_q) - 1) >> p.shift_q;
         count = tiles > 0 ? (tiles + 1) * streams * p.kv_heads : 0;
         // exclusive prefix sum
         const int lane = tid & 63, wave = tid >> 6;
@@ -224,7 +224,7 @@ __device__ __forceinline__ Total plan_segments(const AttnParams& p, const PlanMe
                 rp.start[0] = sh.start;
                 rp.tiles[0] = (sh.k1 - sh.k0 + 31) >> 5;
                 rp.r0[0] = sh.r0;
-                rp.streams[0] = (sh.M + p.rows_q - 1) / p.rows_q;
+                rp.streams[0] = (sh.M + (1 << p.shift_q) - 1) >> p.shift_q;
             }
             rp.start[1] = sg.start;
             rp.tiles[1] = tiles;
@@ -247,7 +247,7 @@ __global__ __launch_bounds__(PLAN) void paged_attn_plan_kernel(AttnParams p) {
 // Without a plan the groups are not used; a workgroup of its own checks them all the same.
 __device__ void check_groups(const AttnParams& p) {
     if (threadIdx.x == 0 && (p.cu_groups[0] != 0 || p.cu_groups[p.n_groups] != p.n)) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, 0);
-    for (int g = threadIdx.x; g < p.n_groups; g += 256) {
+    for (int g = threadIdx.x; g < p.n_groups; g += blockDim.x) {
         const int i0 = p.cu_groups[g], i1 = p.cu_groups[g + 1], shared = p.shared[g];
         if (i0 < 0 || i1 < i0 || i1 > p.n) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, g);
         else if (i1 > i0) {
@@ -577,20 +577,25 @@ __global__ __launch_bounds__(256, 2) void paged_attn_stream_kernel(AttnParams p)
 template <int D>
 __global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnParams p) {
     constexpr int LANES = D / 2;
-    const int lane = threadIdx.x % LANES;
-    const int number = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;   // rows * heads is below 2^31
-    if (number >= p.rows * p.heads) return;
-    const int row = number / p.heads, hq = number - row * p.heads, kvh = hq / p.group;
-    const int64_t item = number;
+    const int lane = threadIdx.x % LANES, row = blockIdx.x, hq = blockIdx.y * (256 / LANES) + threadIdx.x / LANES;
     const RowParts rp = p.parts[row];
     const int per = p.total->per;
-    if (!rp.known) return;
+    if (hq >= p.heads || !rp.known) return;
+    const int64_t item = (int64_t)row * p.heads + hq;
+    const int kvh = hq / p.group;
+    // quotients of places by the places of a wave: a first guess in 64 bits is off by one at most
+    const double inverse = 1.0 / per;
+    auto wave_of = [&](int place) {
+        int q = (int)(place * inverse);
+        const int rest = place - q * per;
+        return rest < 0 ? q - 1 : rest >= per ? q + 1 : q;
+    };
     int count[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
         const int r = (row - rp.r0[k]) * p.group + hq - kvh * p.group;
-        const int begin = rp.start[k] + (kvh * rp.streams[k] + r / p.rows_q) * (rp.tiles[k] + 1) + 1;
-        count[k] = rp.tiles[k] > 0 ? (begin + rp.tiles[k] - 1) / per - begin / per + 1 : 0;
+        const int begin = rp.start[k] + (kvh * rp.streams[k] + (r >> p.shift_q)) * (rp.tiles[k] + 1) + 1;
+        count[k] = rp.tiles[k] > 0 ? wave_of(begin + rp.tiles[k] - 1) - wave_of(begin) + 1 : 0;
     }
     const int np = min(count[0], p.slots_p), n = np + min(count[1], p.slots - p.slots_p);
     if (np == 0 && n == 1) return;   // written already
@@ -619,11 +624,13 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnParams p) {
             a1 += v[a].y * f;
         }
     };
-    if (n > 4) {
+    if (n > 8) {
         for (int i = lane; i < n; i += LANES) M = fmaxf(M, p.part_ml[slot_of(i)].x);
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, LANES));
         for (int i0 = 0; i0 < n; i0 += 8) turn(i0, std::integral_constant<int, 8>{}, true);
+    } else if (n > 4) {
+        turn(0, std::integral_constant<int, 8>{}, false);
     } else if (n > 2) {
         turn(0, std::integral_constant<int, 4>{}, false);
     } else if (n > 0) {
@@ -635,9 +642,10 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnParams p) {
 }
 
 // ---- plain ----
+constexpr int PLAIN_WAVES = 8;
 template <int D, int QT>
-__global__ __launch_bounds__(256, 2) void paged_attn_plain_kernel(AttnParams p) {
-    constexpr int OROW = D + 4, PER = D / 16;
+__global__ __launch_bounds__(64 * PLAIN_WAVES) void paged_attn_plain_kernel(AttnParams p) {
+    constexpr int WAVES = PLAIN_WAVES, OROW = D + 4, PER = D / 32;
     __shared__ __attribute__((aligned(16))) char lds[WAVES * Rows<D>::TILE];
     __shared__ float sm_m[WAVES][16], sm_l[WAVES][16];
     static_assert(WAVES * Rows<D>::TILE >= WAVES * 16 * OROW * 4, "the waves' results fit where their tiles were");
@@ -666,7 +674,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_plain_kernel(AttnParams p) 
             w.step(32 * t, sg.k1, [&] { w.load(p.K, w.kf, head, 32 * (t + WAVES), sg.k1); }, [&] { w.load(p.V, w.vf, head, 32 * (t + WAVES), sg.k1); });
         w.step(32 * t, sg.k1, [] {}, [] {});
     }
-    // join the four waves, 16 queries at a time
+    // join the waves, 16 queries at a time
     float* const so = (float*)lds;
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
@@ -679,7 +687,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_plain_kernel(AttnParams p) 
 #pragma unroll
         for (int dt = 0; dt < D / 16; ++dt) *(f32x4*)(so + (wave * 16 + w.li) * OROW + 16 * dt + 4 * w.lg) = w.o[qt][dt];
         __syncthreads();
-        const int qi = tid >> 4, d0 = (tid & 15) * PER, r = first + 16 * qt + qi;
+        const int qi = tid >> 5, d0 = (tid & 31) * PER, r = first + 16 * qt + qi;
         if (r < sg.M) {
             float M = -INFINITY, L = 0.f, acc[PER];
 #pragma unroll
@@ -700,8 +708,8 @@ __global__ __launch_bounds__(256, 2) void paged_attn_plain_kernel(AttnParams p) 
 #pragma unroll
             for (int d = 0; d < PER; d += 2) b[d / 2] = pack_bf16x2(acc[d] * inv, acc[d + 1] * inv);
             bf16_t* dst = p.out + (int64_t)row * p.o_ld + hq * D + d0;
-            if constexpr (PER == 8) *(uint4*)dst = make_uint4(b[0], b[1], b[2], b[3]);
-            else *(uint2*)dst = make_uint2(b[0], b[1]);
+            if constexpr (PER == 4) *(uint2*)dst = make_uint2(b[0], b[1]);
+            else *(uint32_t*)dst = b[0];
             if (p.lse && d0 == 0) p.lse[(int64_t)row * p.heads + hq] = lse_of(use, L);
         }
     }
@@ -750,8 +758,9 @@ void launch_d(const AttnParams& p, const Plan& r, hipStream_t s) {
     const dim3 block(256);
     if (r.plain) {
         const dim3 grid(p.n * r.tiles_q * p.kv_heads + (p.n_groups > 0));
-        if (r.qt == 1) hipLaunchKernelGGL((paged_attn_plain_kernel<D, 1>), grid, block, 0, s, p);
-        else hipLaunchKernelGGL((paged_attn_plain_kernel<D, 2>), grid, block, 0, s, p);
+        const dim3 plain_block(64 * PLAIN_WAVES);
+        if (r.qt == 1) hipLaunchKernelGGL((paged_attn_plain_kernel<D, 1>), grid, plain_block, 0, s, p);
+        else hipLaunchKernelGGL((paged_attn_plain_kernel<D, 2>), grid, plain_block, 0, s, p);
         HIP_CHECK(hipGetLastError());
         return;
     }
@@ -770,7 +779,7 @@ void launch_d(const AttnParams& p, const Plan& r, hipStream_t s) {
     else { STREAM(MOST); }
 #undef STREAM
     HIP_CHECK(hipGetLastError());
-    hipLaunchKernelGGL((paged_attn_join_kernel<D>), dim3(cdiv((int64_t)p.rows * p.heads, 256 / (D / 2))), block, 0, s, p);
+    hipLaunchKernelGGL((paged_attn_join_kernel<D>), dim3(p.rows, cdiv(p.heads, 256 / (D / 2))), block, 0, s, p);
     HIP_CHECK(hipGetLastError());
 }
 
@@ -798,7 +807,7 @@ void launch_paged_attention(const q3asr_kv_pages& c, int layer, const bf16_t* q,
     p.max_own = shares ? b.max_own : b.max_len;
     p.max_shared = b.max_shared;
     p.scale_log2 = scale * 1.44269504088896340736f;
-    p.rows_q = 16 * r.qt; p.tiles_q = r.tiles_q; p.per_min = r.per_min; p.slots_p = r.slots_p; p.slots = r.slots;
+    p.shift_q = r.qt == 1 ? 4 : r.qt == 2 ? 5 : 6; p.tiles_q = r.tiles_q; p.per_min = r.per_min; p.slots_p = r.slots_p; p.slots = r.slots;
     char* ws = (char*)workspace;
     p.total = (Total*)ws;
     p.plan_ws = ws + r.at_plan;

@@ -460,16 +460,13 @@ __global__ __launch_bounds__(256) void pages_write_kernel(Pages p, int layer, co
     };
     uint4 first = make_uint4(0, 0, 0, 0);
     if (tid < 2 * chunks) first = *source(tid);
-    // the entry of the list that the row belongs to: the row's own number where every sequence has one row, else by halving
+    // the entry of the list that the row belongs to: the row's own number where every sequence has one row, else the last that begins
+    // at or before it
     int lo = min(row, n - 1), r0 = cu_rows[lo], r1 = cu_rows[lo + 1], seq = seqs[lo];
-    if (row < r0 || row >= r1) {
-        lo = 0;
-        int hi = n;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (cu_rows[mid] <= row) lo = mid;
-            else hi = mid;
-        }
+    if (row < r0 || row >= r1) {   // the same for the whole workgroup
+        int before = 0;
+        for (int i0 = 0; i0 < n; i0 += 256) before += __syncthreads_count(i0 + tid < n && cu_rows[i0 + tid] <= row);
+        lo = max(before - 1, 0);
         r0 = cu_rows[lo];
         r1 = cu_rows[lo + 1];
         seq = seqs[lo];
