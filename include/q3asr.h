@@ -198,21 +198,22 @@ int q3asr_i8_quantize(q3asr_model* m, const void* x, int dtype, int64_t ldx, int
  * or Q3ASR_BF16 (rounded once) in rows ldo values apart.  a, w: rows lda / ldw bytes apart, both multiples of 16 and
  * aligned to 16; K a multiple of 16, at most 131056.  bias: [N] fp32 or NULL. */
 int q3asr_i8_matmul(q3asr_model* m, const int8_t* a, int64_t lda, const float* a_scales, const int8_t* w, int64_t ldw,
-                    const float* w_scales, const float* bias, int M, int N, int K, void* out, int out_dtype, int64_t ldo,
-                    void* workspace, int64_t workspace_bytes, void* stream);
+                    const float* w_scales, const float* bias, int M, int N, int K, void* out, int out_dtype, int64_t ldo, void* stream);
 /* The two together: activations x as in q3asr_i8_quantize, weights as in q3asr_i8_matmul but any K (at most 131056): a
  * weight row then has K rounded up to 16 readable bytes, of which those from K on may hold anything. */
 int q3asr_i8_linear(q3asr_model* m, const void* x, int x_dtype, int64_t ldx, const int8_t* w, int64_t ldw, const float* w_scales,
                     const float* bias, int M, int N, int K, void* out, int out_dtype, int64_t ldo, void* workspace,
                     int64_t workspace_bytes, void* stream);
-/* Bytes of workspace that q3asr_i8_linear and q3asr_i8_matmul need for these sizes (-1: sizes out of range). */
+/* Bytes of workspace that q3asr_i8_linear needs for these sizes (-1: sizes out of range). */
 int64_t q3asr_i8_workspace(q3asr_model* m, int M, int N, int K);
 
 /* -- A KV cache in pages --
  * A page holds page_tokens tokens of every layer and KV head.  A sequence s of lens[s] tokens owns the pages
  * table[s][0 .. ceil(lens[s] / page_tokens)); its other table entries are -1.  refs[p] counts the table entries that name
  * page p; a page with refs 0 is free.  All of it lives on the device and is changed there, in stream order, by the calls
- * below; several sequences may share a page, and a shared page is never written except through q3asr_pages_reserve's copy. */
+ * below; several sequences may share a page, and a shared page is never written except through q3asr_pages_reserve's copy.  The
+ * caller orders the calls that change a cache and those that read it (one stream, or events between streams).  In all lists
+ * of sequences, which have at most max_seqs entries, -1 stands for none, for lists of fixed length in captured graphs. */
 typedef struct q3asr_kv_pages {
     uint16_t* k;               /* bf16 [layers][pages][kv_heads][page_tokens][head_dim], aligned to 16 bytes */
     uint16_t* v;
@@ -241,8 +242,8 @@ enum {
  * attention that reports an error are not to be used.  The first
  * such error since the last reset of the status is kept: status[0] = code, [1] = number of the (first) wrong entry in the list,
  * [2] = pages short of (NO_PAGES), and [3] = pages in use after the last compact.  Calls on the model's own stream (stream
- * NULL) return the error at once and reset the status; after calls on another stream the host asks here: waits for the stream, copies the status to out
- * (host, 4 numbers) and, where clear is non-zero, sets it to zeros.  Not under graph capture. */
+ * NULL) return the error that is kept, if any, and reset the status; after calls on another stream the host asks here: waits for the
+ * stream, copies the status to out (host, 4 numbers) and, where clear is non-zero, sets it to zeros.  Not under graph capture. */
 int q3asr_pages_status(q3asr_model* m, const q3asr_kv_pages* c, int32_t* out, int clear, void* stream);
 int64_t q3asr_pages_workspace(const q3asr_kv_pages* c);
 /* No sequences, all pages free, status zero.  The pages' contents stay as they are. */
@@ -262,13 +263,14 @@ int q3asr_pages_reserve(q3asr_model* m, const q3asr_kv_pages* c, const int32_t* 
 int q3asr_pages_compact(q3asr_model* m, const q3asr_kv_pages* c, void* stream);
 
 /* The rows of a step: sequence seqs[i] has rows cu_rows[i] .. cu_rows[i + 1) of it, which are its last tokens (lens counts them
- * already: q3asr_pages_reserve).  A sequence stands in the list once.  Optionally, consecutive sequences of the list form groups
+ * already: q3asr_pages_reserve).  A sequence stands in the list once; an entry of -1 has no rows.  Rows from cu_rows[n] on (a
+ * padded batch) are left alone.  Optionally, consecutive sequences of the list form groups
  * (group g: entries cu_groups[g] .. cu_groups[g + 1)) whose first shared[g] tokens lie in the same pages; those are then read
  * once for the group.  shared[g] counts at most the tokens before the step's rows and is rounded down to whole pages.  The host
  * numbers bound what the arrays hold; smaller bounds make smaller grids. */
 typedef struct q3asr_attn_batch {
     const int32_t* seqs;       /* [n] */
-    const int32_t* cu_rows;    /* [n + 1], from 0 to rows */
+    const int32_t* cu_rows;    /* [n + 1], from 0 to at most rows */
     const int32_t* cu_groups;  /* [n_groups + 1], from 0 to n, or NULL */
     const int32_t* shared;     /* [n_groups] or NULL */
     int n, rows, n_groups;

@@ -115,30 +115,26 @@ int q3asr_i8_quantize(q3asr_model* m, const void* x, int dtype, int64_t ldx, int
     Q3_API_END
 }
 
-static void check_product(const int8_t* w, int64_t ldw, const float* w_scales, int M, int N, int K, const void* out, int out_dtype, int64_t ldo,
-                          const void* workspace) {
+static void check_product(const int8_t* w, int64_t ldw, const float* w_scales, int M, int N, int K, const void* out, int out_dtype, int64_t ldo) {
     Q3_REQUIRE(w && w_scales && out, "i8: null argument");
     Q3_REQUIRE(M > 0 && N > 0 && K > 0, "i8: empty problem");
     Q3_REQUIRE(K <= I8_MAX_K, "i8: K above 131056 could overflow the 32-bit sums");
     Q3_REQUIRE((int64_t)cdiv(M, 64) * cdiv(N, 64) < (1ll << 31), "i8: too many output tiles");
     check_i8("i8: w", w, ldw, K);
     check_rows("i8: out", out, out_dtype, ldo, N);
-    Q3_REQUIRE(aligned(workspace, 16), "i8: misaligned workspace");
 }
 
 int q3asr_i8_matmul(q3asr_model* m, const int8_t* a, int64_t lda, const float* a_scales, const int8_t* w, int64_t ldw,
-                    const float* w_scales, const float* bias, int M, int N, int K, void* out, int out_dtype, int64_t ldo,
-                    void* workspace, int64_t workspace_bytes, void* stream) {
+                    const float* w_scales, const float* bias, int M, int N, int K, void* out, int out_dtype, int64_t ldo, void* stream) {
     Q3_API_BEGIN
     Q3_REQUIRE(m && a && a_scales, "i8_matmul: null argument");
-    check_product(w, ldw, w_scales, M, N, K, out, out_dtype, ldo, workspace);
+    check_product(w, ldw, w_scales, M, N, K, out, out_dtype, ldo);
     Q3_REQUIRE(K % 16 == 0, "i8_matmul: K must be a multiple of 16");
     check_i8("i8: a", a, lda, K);
     Call call(m, stream);
     I8Params p;
     p.A = a; p.lda = lda; p.sa = a_scales; p.W = w; p.ldw = ldw; p.sw = w_scales; p.bias = bias;
     p.M = M; p.N = N; p.K = K; p.out = out; p.ldo = ldo; p.out_f32 = out_dtype == Q3ASR_F32;
-    (void)workspace_bytes;   // the product alone keeps nothing
     launch_i8_matmul(p, call.s);
     call.done();
     Q3_API_END
@@ -149,8 +145,9 @@ int q3asr_i8_linear(q3asr_model* m, const void* x, int x_dtype, int64_t ldx, con
                     int64_t workspace_bytes, void* stream) {
     Q3_API_BEGIN
     Q3_REQUIRE(m && x && workspace, "i8_linear: null argument");
-    check_product(w, ldw, w_scales, M, N, K, out, out_dtype, ldo, workspace);
+    check_product(w, ldw, w_scales, M, N, K, out, out_dtype, ldo);
     check_rows("i8_linear: x", x, x_dtype, ldx, K);
+    Q3_REQUIRE(aligned(workspace, 16), "i8_linear: misaligned workspace");
     Q3_REQUIRE(workspace_bytes >= quantized_bytes(M, K), "i8_linear: workspace too small");
     Call call(m, stream);
     I8Params p;
@@ -295,8 +292,10 @@ int64_t q3asr_paged_attention_workspace(q3asr_model* m, const q3asr_kv_pages* c,
         return paged_attention_workspace(*c, *b, heads);
     } catch (const std::exception& e) {
         q3_set_error(e.what());
-        return -1;
+    } catch (...) {
+        q3_set_error("q3asr: unknown error");
     }
+    return -1;
 }
 
 int q3asr_paged_attention(q3asr_model* m, const q3asr_kv_pages* c, int layer, const uint16_t* q, int64_t q_ld, int heads,
@@ -314,7 +313,7 @@ int q3asr_paged_attention(q3asr_model* m, const q3asr_kv_pages* c, int layer, co
         Q3_REQUIRE(q_ld >= width && o_ld >= width && q_ld % 8 == 0 && o_ld % 8 == 0 && q_ld < MAX_LD && o_ld < MAX_LD && aligned(q, 16) &&
                        aligned(out, 16) && aligned(lse, 4),
                    "paged_attention: rows of q and out must hold all heads and be aligned to 16 bytes");
-        Q3_REQUIRE(scale == scale && scale - scale == 0.f, "paged_attention: scale must be finite");
+        Q3_REQUIRE(scale > -1e30f && scale < 1e30f, "paged_attention: scale must be finite and below 1e30");
         const int64_t need = paged_attention_workspace(*c, *b, heads);
         Q3_REQUIRE(need == 0 || (workspace && aligned(workspace, 16) && workspace_bytes >= need), "paged_attention: workspace missing, misaligned or too small");
     }

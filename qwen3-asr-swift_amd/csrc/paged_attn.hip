@@ -108,12 +108,13 @@ __device__ __forceinline__ Entry entry_of(const AttnParams& p, int i, bool repor
     e.seq = p.seqs[i];
     const int a = p.cu_rows[i], b = p.cu_rows[i + 1];
     const bool in = (unsigned)e.seq < (unsigned)p.max_seqs, ok = in && a >= 0 && b >= a && b <= p.rows && b - a <= p.max_rows;
+    const bool none = e.seq == -1 && a == b;   // stands for no sequence: shares nothing, has no rows
     e.r0 = ok ? a : 0;
     e.T = ok ? b - a : 0;
     e.len = ok ? p.lens[e.seq] : 0;
     e.ok = ok && e.len >= 0 && e.len <= p.max_len;
     if (!e.ok) {
-        if (report) pages_error(p.status, in ? Q3ASR_PAGES_BAD_BATCH : Q3ASR_PAGES_BAD_INDEX, i);
+        if (report && !none) pages_error(p.status, in ? Q3ASR_PAGES_BAD_BATCH : Q3ASR_PAGES_BAD_INDEX, i);
         e.seq = in ? e.seq : 0;
         e.len = min(max(e.len, 0), p.max_len);
     }
@@ -454,9 +455,10 @@ __global__ __launch_bounds__(256, 2) void paged_attn_stream_kernel(AttnParams p)
         total = plan_segments<256>(p, PlanMemory{(Entry*)lds, ints, ints + HELD, ints + 2 * HELD + 1, ints + 3 * HELD + 2, held}, blockIdx.x == 0);
         __syncthreads();   // the tiles go where the plan was made
     }
-    int pos = (blockIdx.x * WAVES + wave) * total.per;
-    const int end = min(total.places, pos + total.per);
-    if (pos >= end) return;
+    const int64_t begin = (int64_t)(blockIdx.x * WAVES + wave) * total.per;   // may lie behind what 32 bits hold, places do not
+    if (begin >= total.places) return;
+    int pos = (int)begin;
+    const int end = (int)min((int64_t)total.places, begin + total.per);
     Wave<D, QT> w(p, lds + wave * Rows<D>::TILE);
 
     // the last segment that begins at or before pos: 64 probes at a time
@@ -535,9 +537,9 @@ __global__ __launch_bounds__(256, 2) void paged_attn_stream_kernel(AttnParams p)
         if (over || LAST) {
             // a part, or all there is for these rows
             const int streams = (now.M + 16 * QT - 1) / (16 * QT);
-            const int begin = now.start + (now_kvh * streams + now_first / (16 * QT)) * (now_tiles + 1) + 1;   // the first tile's place
-            const int before = begin / total.per, piece = pos / total.per - before;
-            const bool direct = now.whole && (begin + now_tiles - 1) / total.per == before;
+            const int tile0 = now.start + (now_kvh * streams + now_first / (16 * QT)) * (now_tiles + 1) + 1;   // the first tile's place
+            const int before = tile0 / total.per, piece = pos / total.per - before;
+            const bool direct = now.whole && (tile0 + now_tiles - 1) / total.per == before;
             const int slot = (now.limit == SHARED ? 0 : p.slots_p) + piece;
 #pragma unroll
             for (int qt = 0; qt < QT; ++qt) {

@@ -113,8 +113,8 @@ __global__ __launch_bounds__(PLAN) void pages_fork_kernel(Pages p, const int* ds
     __syncthreads();
     for (int i = tid; i < n; i += PLAN) {
         const int d = dst[i], s = src ? src[i] : -1;
-        if ((unsigned)d >= (unsigned)p.max_seqs || s < -1 || s >= p.max_seqs) note(&worst, i, Q3ASR_PAGES_BAD_INDEX);
-        else mark[d] = i;
+        if (d < -1 || d >= p.max_seqs || s < -1 || s >= p.max_seqs) note(&worst, i, Q3ASR_PAGES_BAD_INDEX);
+        else if (d >= 0) mark[d] = i;   // -1: no entry
     }
     __syncthreads();
     for (int i = tid; i < n; i += PLAN) {
@@ -141,10 +141,12 @@ __global__ __launch_bounds__(PLAN) void pages_fork_kernel(Pages p, const int* ds
         const int e = tid + k * PLAN;
         now[k] = old[k] = at[k] = -1;
         if (e < total) {
-            const int i = width > 1 ? (int)__umulhi((unsigned)e, magic) : e, j = e - i * width, s = src ? src[i] : -1;
-            at[k] = dst[i] * width + j;   // below 2^31: the table has fewer entries
-            if (s >= 0) now[k] = p.table[s * width + j];
-            old[k] = p.table[at[k]];
+            const int i = width > 1 ? (int)__umulhi((unsigned)e, magic) : e, j = e - i * width, d = dst[i], s = src ? src[i] : -1;
+            if (d >= 0) {
+                at[k] = d * width + j;   // below 2^31: the table has fewer entries
+                if (s >= 0) now[k] = p.table[s * width + j];
+                old[k] = p.table[at[k]];
+            }
         }
     }
     int lens = 0;
@@ -157,7 +159,7 @@ __global__ __launch_bounds__(PLAN) void pages_fork_kernel(Pages p, const int* ds
             if ((unsigned)now[k] < (unsigned)p.pages) atomicAdd(&p.refs[now[k]], 1);
             if ((unsigned)old[k] < (unsigned)p.pages) atomicSub(&p.refs[old[k]], 1);
         }
-    if (tid < n) p.lens[dst[tid]] = lens;
+    if (tid < n && dst[tid] >= 0) p.lens[dst[tid]] = lens;
 }
 
 __global__ __launch_bounds__(256) void pages_fork_read_kernel(Pages p, const int* dst, const int* src, int n) {
@@ -167,8 +169,9 @@ __global__ __launch_bounds__(256) void pages_fork_read_kernel(Pages p, const int
     int *rows = p.ws + l.rows, *row_lens = p.ws + l.row_lens;
     const int lane = threadIdx.x & 63;
     for (int i = blockIdx.x * 4 + (threadIdx.x >> 6); i < n; i += gridDim.x * 4) {
-        const int s = src ? src[i] : -1;
-        const int64_t to = (int64_t)dst[i] * width, from = (int64_t)s * width;
+        const int d = dst[i], s = src ? src[i] : -1;
+        if (d < 0) continue;
+        const int64_t to = (int64_t)d * width, from = (int64_t)s * width;
         for (int j = lane; j < width; j += 64) {
             const int now = s < 0 ? -1 : p.table[from + j], old = p.table[to + j];
             rows[(int64_t)i * width + j] = now;
@@ -185,9 +188,11 @@ __global__ __launch_bounds__(256) void pages_fork_write_kernel(Pages p, const in
     const int *rows = p.ws + l.rows, *row_lens = p.ws + l.row_lens;
     const int lane = threadIdx.x & 63;
     for (int i = blockIdx.x * 4 + (threadIdx.x >> 6); i < n; i += gridDim.x * 4) {
-        const int64_t to = (int64_t)dst[i] * width;
+        const int d = dst[i];
+        if (d < 0) continue;
+        const int64_t to = (int64_t)d * width;
         for (int j = lane; j < width; j += 64) p.table[to + j] = rows[(int64_t)i * width + j];
-        if (lane == 0) p.lens[dst[i]] = row_lens[i];
+        if (lane == 0) p.lens[d] = row_lens[i];
     }
 }
 
@@ -220,7 +225,8 @@ __global__ __launch_bounds__(PLAN) void pages_reserve_kernel(Pages p, const int*
         r.seq = seqs[i];
         r.tokens = tokens[i];
         int code = Q3ASR_PAGES_OK;
-        if ((unsigned)r.seq >= (unsigned)p.max_seqs || r.tokens < 0) code = Q3ASR_PAGES_BAD_INDEX;
+        if (r.seq < -1 || r.seq >= p.max_seqs || r.tokens < 0) code = Q3ASR_PAGES_BAD_INDEX;
+        else if (r.seq == -1) r.tokens = 0;   // no entry
         else {
             mark[r.seq] = i;
             const int len = p.lens[r.seq];
@@ -475,6 +481,7 @@ __global__ __launch_bounds__(256) void pages_write_kernel(Pages p, int layer, co
     for (int i = tid; i < lo; i += 256) twice |= seqs[i] == seq;
     twice = __syncthreads_or(twice);
     int code = Q3ASR_PAGES_OK, page = 0, pos = 0;
+    if (row >= cu_rows[n]) return;   // behind the last sequence; the same for the whole workgroup
     if (row < r0 || row >= r1 || r1 > rows) code = Q3ASR_PAGES_BAD_BATCH;
     else if ((unsigned)seq >= (unsigned)p.max_seqs) code = Q3ASR_PAGES_BAD_INDEX;
     else if (twice) code = Q3ASR_PAGES_DUPLICATE;

@@ -104,7 +104,7 @@ def load():
     c_i64 = ctypes.c_int64
     lib.q3asr_i8_quantize.argtypes = [c_void_p, c_void_p, c_int, c_i64, c_int, c_int, c_void_p, c_i64, c_void_p, c_void_p]
     lib.q3asr_i8_matmul.argtypes = [c_void_p, c_void_p, c_i64, c_void_p, c_void_p, c_i64, c_void_p, c_void_p, c_int, c_int, c_int,
-                                    c_void_p, c_int, c_i64, c_void_p, c_i64, c_void_p]
+                                    c_void_p, c_int, c_i64, c_void_p]
     lib.q3asr_i8_linear.argtypes = [c_void_p, c_void_p, c_int, c_i64, c_void_p, c_i64, c_void_p, c_void_p, c_int, c_int, c_int,
                                     c_void_p, c_int, c_i64, c_void_p, c_i64, c_void_p]
     lib.q3asr_i8_workspace.argtypes = [c_void_p, c_int, c_int, c_int]

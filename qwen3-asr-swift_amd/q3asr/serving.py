@@ -42,11 +42,11 @@ class Int8Linear:
             self._m._h, x, _dtype(x_dtype), self.K if ldx is None else ldx, self.w, self.ldw, self.w_scales, self.bias, rows, self.N, self.K,
             out, _dtype(out_dtype), self.N if ldo is None else ldo, workspace[0], workspace[1], stream))
 
-    def matmul(self, a, a_scales, rows, out, lda=None, out_dtype="bf16", ldo=None, workspace=(None, 0), stream=None):
+    def matmul(self, a, a_scales, rows, out, lda=None, out_dtype="bf16", ldo=None, stream=None):
         """The product alone, for activations that quantize_rows has rounded (K a multiple of 16)."""
         _lib.check(self._lib, self._lib.q3asr_i8_matmul(
             self._m._h, a, self.K if lda is None else lda, a_scales, self.w, self.ldw, self.w_scales, self.bias, rows, self.N, self.K, out,
-            _dtype(out_dtype), self.N if ldo is None else ldo, workspace[0], workspace[1], stream))
+            _dtype(out_dtype), self.N if ldo is None else ldo, stream))
 
 
 def quantize_rows(model, x, rows, cols, q, scales, x_dtype="bf16", ldx=None, ldq=None, stream=None):

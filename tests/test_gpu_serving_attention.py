@@ -12,7 +12,7 @@ pytestmark = pytest.mark.gpu
 class Step:
     """A cache with groups of sequences that share prefixes, and one step's rows."""
 
-    def __init__(self, dev, model, groups, heads, kv, dim, pg, seed, poison=True, layers=2, layer=1, spread=1.0):
+    def __init__(self, dev, model, groups, heads, kv, dim, pg, seed, poison=True, layers=2, layer=1, spread=1.0, spare=0):
         """groups: [(shared tokens, [(own tokens, rows), ...]), ...]; own tokens include the rows."""
         self.rng = rng = np.random.default_rng(seed)
         self.dev, self.heads, self.kv, self.dim, self.layer = dev, heads, kv, dim, layer
@@ -21,7 +21,7 @@ class Step:
         lens = [s + own for s, ms in groups for own, _ in ms]
         width = max(1, -(-max(max(lens), 1040) // pg)) + 1
         pages = sum(-(-x // pg) + 1 for x in lens) + sum(s // pg + 2 for s, _ in groups) + 3
-        self.c = c = Cache(dev, model, seqs=n + len(groups), width=width, pages=pages, layers=layers, heads=kv, dim=dim, pg=pg, seed=seed, poison=poison)
+        self.c = c = Cache(dev, model, seqs=n + len(groups) + spare, width=width, pages=pages, layers=layers, heads=kv, dim=dim, pg=pg, seed=seed, poison=poison)
         # every group grows from a base sequence, pages scattered over the pool by a few that come and go
         first = 0
         self.shared, self.seqs, self.cu_groups = [], [], [0]
@@ -129,6 +129,41 @@ def test_attention_matches_fp64(tiny_model, g, heads, kv, dim, pg):
         assert s.c.c.status()[:3] == (0, 0, 0)
 
 
+def test_more_sequences_than_a_workgroup_plans(tiny_model):
+    """Over 1024 groups and sequences: planned by a launch of its own."""
+    with Device() as dev:
+        s = Step(dev, tiny_model[0], [(20, [(3, 1), (5, 2)])] * 400, 4, 2, 64, 16, seed=6)
+        s.check(*s.run(s.batch()))
+        s.check(*s.run(s.batch(grouped=False, max_len=1040)))
+        assert s.c.c.status()[:3] == (0, 0, 0)
+
+
+def test_long_sequences(tiny_model):
+    """Tens of thousands of keys for one row and for a group: many parts, page windows that are renewed on the way."""
+    with Device() as dev:
+        s = Step(dev, tiny_model[0], [(0, [(21007, 1)]), (9000, [(40, 3), (1200, 1)])], 2, 1, 128, 32, seed=8)
+        s.check(*s.run(s.batch()))
+
+
+def test_padded_batches(tiny_model):
+    """Entries of -1, sequences without rows and rows behind the last sequence's: left alone, nothing is reported."""
+    with Device() as dev:
+        for over in ({}, dict(max_len=1040)):
+            s = Step(dev, tiny_model[0], [(40, [(3, 1), (9, 2)]), (64, [(30, 1)])], 4, 2, 128, 16, seed=12, spare=2)
+            n, rows = 7, s.cu[-1] + 3
+            real = s.cu[-1]
+            seqs, cu, groups, shared = s.seqs + [-1] * 4, s.cu + [real] * 4, s.cu_groups + [5, 7], s.shared + [48, 0]
+            s.q = np.concatenate([s.q, s.q[:3]])
+            s.cu[-1] = rows                       # buffers of the padded size
+            b = s.batch(seqs=s.c.ints(seqs), cu_rows=s.c.ints(cu), cu_groups=s.c.ints(groups), shared=s.c.ints(shared), n=n, rows=rows, n_groups=4,
+                        max_rows=2, max_group_rows=4, max_own=max(s.lens), **over)
+            out, lse = s.run(b)
+            assert s.c.c.status()[:3] == (0, 0, 0)
+            assert (out[real:] == 7).all() and (lse[real:] == 7).all()
+            s.cu[-1] = real
+            s.check(out[:real], lse[:real])
+
+
 def test_rows_without_keys_are_zero(tiny_model):
     """Empty sequences and rows before a sequence's first token: zeros and -inf, with and without groups."""
     with Device() as dev:
@@ -140,6 +175,14 @@ def test_rows_without_keys_are_zero(tiny_model):
             out, lse = s.run(b)
             s.check(out, lse)
             assert (out[:3] == 0).all() and (lse[:3] == -np.inf).all()
+    with Device() as dev:      # more rows than tokens: the first ones lie before the sequence
+        s = Step(dev, tiny_model[0], [(0, [(1, 1), (3, 3)])], 4, 2, 128, 16, seed=3)
+        s.rows, s.cu = [3, 5], [0, 3, 8]
+        s.q = bf16_bits(s.rng.standard_normal((8, 512)))
+        for b in (s.batch(), s.batch(grouped=False, max_len=1040)):
+            out, lse = s.run(b)
+            s.check(out, lse)
+            assert (out[[0, 1, 3, 4]] == 0).all() and np.isfinite(lse[[2, 5, 6, 7]]).all()
 
 
 def test_extreme_scores(tiny_model):

@@ -44,7 +44,8 @@ def _weights(rng, n, k):
 
 
 @pytest.mark.parametrize("kind", ["bf16", "f32"])
-@pytest.mark.parametrize("m,k,pad", [(1, 1, 0), (3, 15, 1), (5, 16, 0), (4, 17, 8), (70, 1003, 5), (33, 2048, 0), (2, 6144, 24), (9, 4100, 4)])
+@pytest.mark.parametrize("m,k,pad", [(1, 1, 0), (3, 15, 1), (5, 16, 0), (4, 17, 8), (70, 1003, 5), (33, 2048, 0), (2, 6144, 24), (9, 4100, 4),
+                                     (3, 9003, 0), (1100, 300, 3), (1030, 5000, 0), (1030, 7001, 1)])
 def test_quantize_rows_is_exact(tiny_model, m, k, pad, kind):
     from q3asr import quantize_rows
     rng = np.random.default_rng(m * 31 + k)
@@ -95,7 +96,7 @@ def test_quantize_rows_at_the_borders(tiny_model):
 
 SHAPES = [(1, 1, 1), (1, 4096, 2048), (2, 33, 100), (3, 2048, 6144), (4, 64, 33), (5, 70, 1003), (8, 256, 512), (16, 1000, 784),
           (17, 31, 48), (31, 515, 2080), (64, 64, 128), (65, 127, 129), (130, 2048, 4096), (200, 320, 6000), (333, 1027, 1003), (700, 769, 300),
-          (2100, 2304, 256), (300, 12288, 96)]
+          (2100, 2304, 256), (300, 12288, 96), (1000, 1500, 200), (3100, 4001, 130), (3100, 4000, 640), (40, 40000, 64), (6, 96, 6200), (2, 50, 13000)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
@@ -127,7 +128,7 @@ def test_linear_matches_whole_numbers(tiny_model, m, n, k, x, out, bias):
     assert (np.abs(got - want) <= tol + 1e-37).all()
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 40, 64), (6, 300, 4096), (70, 130, 1024), (260, 300, 2048), (1000, 768, 131056 // 16)])
+@pytest.mark.parametrize("m,n,k", [(1, 40, 64), (6, 300, 4096), (70, 130, 1024), (260, 300, 2048), (1000, 768, 131056 // 16), (2, 3, 131056)])
 def test_matmul_equals_linear_and_extremes(tiny_model, m, n, k):
     """quantize + matmul gives linear's bits; -128 (which quantize never makes) and rows of +-127 sum without overflow."""
     from q3asr import Int8Linear, quantize_rows
@@ -148,8 +149,8 @@ def test_matmul_equals_linear_and_extremes(tiny_model, m, n, k):
         x = dev.put(bf16_bits(xs))
         lin(x, m, o1, out_dtype="f32", workspace=scratch)
         quantize_rows(model, x, m, k, q, s)
-        lin.matmul(q, s, m, o2, out_dtype="f32", workspace=scratch)
-        lin.matmul(dev.put(a), dev.put(sa), m, o3, out_dtype="f32", workspace=scratch)
+        lin.matmul(q, s, m, o2, out_dtype="f32")
+        lin.matmul(dev.put(a), dev.put(sa), m, o3, out_dtype="f32")
         one, two, three = (dev.get(o, (m, n), np.float32) for o in (o1, o2, o3))
     assert np.array_equal(one, two)
     want = (a.astype(np.float64) @ w[:, :k].astype(np.float64).T) * sa.astype(np.float64)[:, None] * sw.astype(np.float64)

@@ -107,13 +107,14 @@ def test_refused_calls_change_nothing(tiny_model):
     with Device() as dev:
         c = _filled(dev, tiny_model[0], [20, 40, 8], seqs=6, width=4, pages=12)
         cases = [(lambda s: c.c.fork(c.ints([3, 6]), c.ints([0, 0]), 2, s), "out of range.*entry 1", 1),
-                 (lambda s: c.c.fork(c.ints([3, -1]), c.ints([0, 0]), 2, s), "out of range.*entry 1", 1),
+                 (lambda s: c.c.fork(c.ints([3, -2]), c.ints([0, 0]), 2, s), "out of range.*entry 1", 1),
                  (lambda s: c.c.fork(c.ints([3, 4]), c.ints([0, 9]), 2, s), "out of range.*entry 1", 1),
                  (lambda s: c.c.fork(c.ints([3, 4]), c.ints([-2, 0]), 2, s), "out of range.*entry 0", 1),
                  (lambda s: c.c.fork(c.ints([3, 4, 3]), c.ints([0, 1, 2]), 3, s), "named twice", 2),
                  (lambda s: c.c.free(c.ints([1, 1]), 2, s), "named twice", 2),
                  (lambda s: c.c.reserve(c.ints([0, 1, 0]), c.ints([1, 1, 1]), 3, s), "named twice", 2),
                  (lambda s: c.c.reserve(c.ints([0, 7]), c.ints([1, 1]), 2, s), "out of range.*entry 1", 1),
+                 (lambda s: c.c.reserve(c.ints([0, -2]), c.ints([1, 1]), 2, s), "out of range.*entry 1", 1),
                  (lambda s: c.c.reserve(c.ints([0, 1]), c.ints([1, -1]), 2, s), "out of range.*entry 1", 1),
                  (lambda s: c.c.reserve(c.ints([0, 1]), c.ints([1, 25]), 2, s), "outgrow.*entry 1", 4),
                  (lambda s: c.c.reserve(c.ints([3, 4]), c.ints([64, 2 ** 31 - 1]), 2, s), "outgrow.*entry 1", 4),
@@ -142,6 +143,23 @@ def test_refused_calls_change_nothing(tiny_model):
         c.check()
 
 
+@pytest.mark.parametrize("n", [6, 700])
+def test_entries_of_minus_one_stand_for_none(tiny_model, n):
+    """Lists of fixed length: -1 is skipped in fork, free and reserve, however often it stands there."""
+    with Device() as dev:
+        c = _filled(dev, tiny_model[0], [20, 37, 5], seqs=max(n, 8), width=6, pages=60, layers=2)
+        pad = [-1] * (n - 4)
+        c.c.fork(c.ints([3, -1, 4, 5] + pad), c.ints([0, 2, 1, -1] + [1] * len(pad)), n)
+        c.book.fork([3, 4, 5], [0, 1, -1])
+        c.check()
+        c.c.reserve(c.ints([-1, 4, 3, -1] + pad), c.ints([9, 1, 20, 0] + [7] * len(pad)), n)
+        c.book.reserve([4, 3], [1, 20])
+        c.check()
+        c.c.free(c.ints([-1, -1, 1, 4] + pad), n)
+        c.book.fork([1, 4], [-1, -1])
+        c.check()
+
+
 def test_write_puts_rows_at_the_ends(tiny_model):
     from q3asr import AttentionBatch
     rng = np.random.default_rng(8)
@@ -153,6 +171,12 @@ def test_write_puts_rows_at_the_ends(tiny_model):
         b = AttentionBatch(seqs=c.ints(seqs), cu_rows=c.ints(cu), n=5, rows=27, max_rows=18, max_len=96)
         c.c.write(1, dev.put(k), dev.put(v), b, k_ld=ld, v_ld=ld)
         c.book.write(1, k[:, :192], v[:, :192], seqs, cu)
+        c.check()
+        # rows behind the last sequence's are left out
+        b = AttentionBatch(seqs=c.ints(seqs), cu_rows=c.ints(cu), n=5, rows=40, max_rows=18, max_len=96)
+        k2 = bf16_bits(rng.standard_normal((40, ld)))
+        c.c.write(0, dev.put(k2), dev.put(k2), b, k_ld=ld, v_ld=ld)
+        c.book.write(0, k2[:, :192], k2[:, :192], seqs, cu)
         c.check()
         # a shared page is not written, a sequence named twice keeps its first row, rows before a sequence's start are left out
         c.fork([6], [2])

@@ -18,7 +18,8 @@ def lib():
 @pytest.fixture()
 def handle():
     """Stands for a model: a call that is refused never looks into it."""
-    return ctypes.addressof(ctypes.create_string_buffer(1 << 14))
+    held = ctypes.create_string_buffer(1 << 14)
+    yield ctypes.addressof(held)
 
 
 def _text(lib):
@@ -52,7 +53,7 @@ def test_i8_refusals(lib, handle):
         assert text in _text(lib), (kw, _text(lib))
 
     def matmul(a=P, lda=64, sa=P, K=64):
-        return lib.q3asr_i8_matmul(handle, a, lda, sa, P, 64, P, None, 4, 8, K, P, 1, 8, None, 0, None)
+        return lib.q3asr_i8_matmul(handle, a, lda, sa, P, 64, P, None, 4, 8, K, P, 1, 8, None)
 
     for kw, text in ((dict(a=None), "null"), (dict(sa=None), "null"), (dict(K=60), "multiple of 16"), (dict(lda=48), "stride"), (dict(a=P + 1), "aligned")):
         assert matmul(**kw) != 0 and text in _text(lib), (kw, _text(lib))
@@ -108,20 +109,24 @@ def test_attention_and_write_refusals(lib, handle):
         c, b = _cache(**(cache or {})), q3lib.AttentionBatch(**{**base, **(batch or {})})
         return lib.q3asr_paged_attention(handle, ctypes.byref(c), layer, q, ld, heads, scale, ctypes.byref(b), out, old, lse, ws, nb, None)
 
+    long = dict(cache=dict(max_seq_pages=100), batch=dict(max_len=1500, max_own=1468))   # a small step needs no workspace
     for kw, text in ((dict(batch=dict(n=-1)), "bad batch"), (dict(batch=dict(seqs=None)), "null"), (dict(batch=dict(n=5)), "more entries"),
                      (dict(batch=dict(max_rows=0)), "max_rows"), (dict(batch=dict(max_rows=7)), "max_rows"), (dict(batch=dict(max_len=81)), "max_len"),
                      (dict(batch=dict(n_groups=5)), "groups"), (dict(batch=dict(cu_groups=None)), "groups"), (dict(batch=dict(max_group_rows=1)), "max_group_rows"),
                      (dict(batch=dict(max_shared=71)), "max_shared"), (dict(batch=dict(max_own=-1)), "max_own"), (dict(layer=2), "layer"), (dict(layer=-1), "layer"),
                      (dict(heads=3), "multiple"), (dict(q=None), "null"), (dict(out=None), "null"), (dict(ld=511), "aligned"), (dict(ld=504), "hold all heads"),
-                     (dict(old=516), "aligned"), (dict(q=P + 8), "aligned"), (dict(scale=float("nan")), "finite"), (dict(scale=float("inf")), "finite"),
-                     (dict(ws=None), "workspace"), (dict(nb=16), "workspace"), (dict(cache=dict(head_dim=32)), "head_dim")):
+                     (dict(old=516), "aligned"), (dict(q=P + 8), "aligned"), (dict(scale=float("nan")), "finite"), (dict(scale=float("inf")), "finite"), (dict(scale=-2e30), "finite"),
+                     (dict(cache=dict(head_dim=32)), "head_dim"),
+                     (dict(ws=None, **long), "workspace"), (dict(nb=16, **long), "workspace"), (dict(ws=P + 8, **long), "workspace")):
         assert attention(**kw) != 0, kw
         assert text in _text(lib), (kw, _text(lib))
     c, b = _cache(), q3lib.AttentionBatch(**base)
     for args in ((2, P, 256, P, 256), (0, None, 256, P, 256), (0, P, 255, P, 256), (0, P, 248, P, 256), (0, P + 2, 256, P, 256)):
         assert lib.q3asr_pages_write(handle, ctypes.byref(c), args[0], args[1], args[2], args[3], args[4], ctypes.byref(b), None) != 0, args
     assert lib.q3asr_paged_attention_workspace(handle, ctypes.byref(c), ctypes.byref(b), 3) == -1
-    assert lib.q3asr_paged_attention_workspace(handle, ctypes.byref(c), ctypes.byref(b), 4) > 0
+    assert lib.q3asr_paged_attention_workspace(handle, ctypes.byref(c), ctypes.byref(b), 4) == 0
+    c, b = _cache(max_seq_pages=100), q3lib.AttentionBatch(**{**base, **long["batch"]})
+    assert lib.q3asr_paged_attention_workspace(handle, ctypes.byref(c), ctypes.byref(b), 4) > 6 * 4 * 128 * 4
     empty = q3lib.AttentionBatch(n=0, rows=0)
     assert lib.q3asr_paged_attention_workspace(handle, ctypes.byref(c), ctypes.byref(empty), 4) == 0
 
