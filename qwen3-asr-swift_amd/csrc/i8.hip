@@ -198,26 +198,30 @@ __device__ __forceinline__ void i8_store(const I8Params& p, int m, int c, const 
         }
 }
 
-// The same for rows that cannot take 16-byte stores: a wave's 16 rows x 4 * NC columns go through its own piece of LDS (16 rows of
-// 4 * NC + 1 words) so that a store instruction writes along rows instead of touching 64 lines.  Column q of the block is
-// column c + (q / NC) * step + q % NC of the matrix.
-template <int NC>
-__device__ __forceinline__ void i8_store_rows(const I8Params& p, int m, int c, int step, const float* y, float* piece) {
+// The same for rows that cannot take 16-byte stores: a wave's block of 16 rows x 4 * NC columns goes through its own piece of LDS, ROWS
+// rows of 4 * NC + 1 words at a time, so that a store instruction writes along rows instead of touching 64 lines.
+template <int NC, int ROWS>
+__device__ __forceinline__ void i8_store_rows(const I8Params& p, int m, int c, const float* y, float* piece) {
     constexpr int W = 4 * NC;
     const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
-    __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int e = 0; e < NC; ++e) piece[li * (W + 1) + lg * NC + e] = y[e];
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    for (int h = 0; h < 16 / ROWS; ++h) {
+        __builtin_amdgcn_wave_barrier();
+        if (li / ROWS == h) {
 #pragma unroll
-    for (int i = 0; i < W / 4; ++i) {
-        const int r = (i * 64 + lane) / W, q = (i * 64 + lane) % W, row = m + r, col = c + q / NC * step + q % NC;
-        const float v = piece[r * (W + 1) + q];
-        if (row < p.M && col < p.N) {
-            if (p.out_f32) ((float*)p.out)[(int64_t)row * p.ldo + col] = v;
-            else ((bf16_t*)p.out)[(int64_t)row * p.ldo + col] = f32_to_bf16(v);
+            for (int e = 0; e < NC; ++e) piece[li % ROWS * (W + 1) + lg * NC + e] = y[e];
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+        for (int i = 0; i < ROWS * W / 64; ++i) {
+            const int r = (i * 64 + lane) / W, q = (i * 64 + lane) % W, row = m + h * ROWS + r, col = c + q;
+            const float v = piece[r * (W + 1) + q];
+            if (row < p.M && col < p.N) {
+                if (p.out_f32) ((float*)p.out)[(int64_t)row * p.ldo + col] = v;
+                else ((bf16_t*)p.out)[(int64_t)row * p.ldo + col] = f32_to_bf16(v);
+            }
         }
     }
 }
@@ -360,7 +364,7 @@ __global__ __launch_bounds__(256, 2) void i8_gemm_kernel(I8Params p) {
         for (int b = 0; b < NT; ++b)
 #pragma unroll
             for (int r = 0; r < 4; ++r) y[b * 4 + r] = i8_scaled(acc[a][b][r], scale_a[a], scale_w[b * 4 + r]) + bias[b * 4 + r];
-        if (!p.vec_out) i8_store_rows<4 * NT>(p, m, n0 + wc * 16 * NT, 4 * NT, y, piece);
+        if (!p.vec_out) i8_store_rows<4 * NT, 16>(p, m, n0 + wc * 16 * NT, y, piece);
         else if (m + li < p.M) i8_store<4 * NT>(p, m + li, c0, y);
     }
 }
@@ -373,7 +377,7 @@ __global__ __launch_bounds__(256, 2) void i8_gemm_kernel(I8Params p) {
 // 16x16x32 bf16 or one 16x16x64 int8 MFMA of the same length.  Twice the work per byte moved, so the phases are the same and
 // the rate doubles.
 constexpr int UNIT = 128 * 128, BUF = 4 * UNIT;   // A0 | A1 | W0 | W1, two K tiles
-constexpr int SCALES = 3 * 256 * 4, PIECE = 16 * 33 * 4;
+constexpr int SCALES = 3 * 256 * 4, PIECE = 8 * 65 * 4;
 constexpr int LDS256 = 2 * BUF + 2 * SCALES + 8 * PIECE;   // scales of the tile's rows, columns, and the bias, for two tiles; a piece per wave
 
 __global__ __launch_bounds__(512, 2) void i8_gemm256_kernel(I8Params p) {
@@ -562,8 +566,7 @@ __global__ __launch_bounds__(512, 2) void i8_gemm256_kernel(I8Params p) {
                 for (int e = 0; e < 16; ++e) y[e] = __int_as_float(acc[a][f][e >> 3][(e >> 2) & 1][e & 3]);
                 if (!p.vec_out) {
                     float* const piece = (float*)(smem + 2 * BUF + 2 * SCALES + uwave * PIECE);
-                    i8_store_rows<8>(p, m, e_n0 + wc * 64, 16, y, piece);
-                    i8_store_rows<8>(p, m, e_n0 + wc * 64 + 8, 16, y + 8, piece);
+                    i8_store_rows<16, 8>(p, m, e_n0 + wc * 64, y, piece);
                 } else if (m + li < p.M) {
                     i8_store<16>(p, m + li, e_n0 + c0, y);
                 }
