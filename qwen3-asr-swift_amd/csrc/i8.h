@@ -16,10 +16,9 @@ struct I8Params {
     const float* bias = nullptr;
     int M = 0, N = 0, K = 0;
     void* out = nullptr; int64_t ldo = 0; int out_f32 = 0;
-    int vec_out = 0;       // rows of out can take 16-byte stores
 };
 
 void launch_i8_quantize(const I8Source& src, int rows, int cols, int8_t* q, int64_t ldq, float* scales, hipStream_t s);
 // Both steps in one kernel where the rows are few; false: it does not apply.
 bool launch_i8_linear_few_rows(const I8Params& p, const I8Source& src, hipStream_t s);
-void launch_i8_matmul(I8Params p, hipStream_t s);
+void launch_i8_matmul(const I8Params& p, hipStream_t s);

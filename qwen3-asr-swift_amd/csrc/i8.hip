@@ -69,17 +69,27 @@ __device__ __forceinline__ float i8_load(const void* row, int k) {
     else return bf16_to_f32(((const bf16_t*)row)[k]);
 }
 
-// 8 consecutive values of a row.  `vec`: the row is aligned to 16 bytes; values from `cols` on read as zero.
+// 16 bytes from a place aligned to a value only: one load, which the memory unit splits where it crosses a line.
+__device__ __forceinline__ uint4 i8_load16(const void* at) {
+    struct __attribute__((packed, aligned(2))) Loose { uint32_t x, y, z, w; };
+    const Loose a = *(const Loose*)at;
+    return make_uint4(a.x, a.y, a.z, a.w);
+}
+// 8 consecutive values of a row; values from `cols` on read as zero.
 template <bool F32>
-__device__ __forceinline__ void i8_load8(const void* row, int k, int cols, bool vec, float* v) {
-    if (vec && k + 8 <= cols) {
+__device__ __forceinline__ void i8_load8(const void* row, int k, int cols, float* v) {
+    if (k + 8 <= cols) {
+        const uint4 a = i8_load16((const char*)row + (int64_t)k * (F32 ? 4 : 2));
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
         if constexpr (F32) {
-            const float4 a = *(const float4*)((const float*)row + k), b = *(const float4*)((const float*)row + k + 4);
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-            v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+            const uint4 b = i8_load16((const float*)row + k + 4);
+            const uint32_t u[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[e] = __uint_as_float(w[e]);
+                v[4 + e] = __uint_as_float(u[e]);
+            }
         } else {
-            const uint4 a = *(const uint4*)((const bf16_t*)row + k);
-            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 v[2 * e] = __uint_as_float(w[e] << 16);
@@ -137,14 +147,13 @@ __global__ __launch_bounds__(256) void i8_quantize_kernel(const void* x, int64_t
         return __uint_as_float(m);
     };
     const void* src = (const char*)x + (int64_t)row * ldx * (F32 ? 4 : 2);
-    const bool vec = (uintptr_t)src % 16 == 0;
     int8_t* dst = q + (int64_t)row * ldq;
     const int k16 = (cols + 15) & ~15;
     uint32_t m = 0;
     if constexpr (HELD > 0) {
         float v[HELD][8];
 #pragma unroll
-        for (int i = 0; i < HELD; ++i) i8_load8<F32>(src, (i * STEP + lane) * 8, cols, vec, v[i]);
+        for (int i = 0; i < HELD; ++i) i8_load8<F32>(src, (i * STEP + lane) * 8, cols, v[i]);
 #pragma unroll
         for (int i = 0; i < HELD; ++i) m = i8_max8(m, v[i]);
         const RowScale rs(row_max(m));
@@ -157,13 +166,13 @@ __global__ __launch_bounds__(256) void i8_quantize_kernel(const void* x, int64_t
     } else {
         float v[8];
         for (int k = lane * 8; k < cols; k += 8 * STEP) {
-            i8_load8<F32>(src, k, cols, vec, v);
+            i8_load8<F32>(src, k, cols, v);
             m = i8_max8(m, v);
         }
         const RowScale rs(row_max(m));
         if (lane == 0) scales[row] = rs.scale;
         for (int k = lane * 8; k < k16; k += 8 * STEP) {
-            i8_load8<F32>(src, k, cols, vec, v);
+            i8_load8<F32>(src, k, cols, v);
             *(uint2*)(dst + k) = rs.pack8(v);
         }
     }
@@ -173,20 +182,27 @@ __global__ __launch_bounds__(256) void i8_quantize_kernel(const void* x, int64_t
 
 __device__ __forceinline__ float i8_scaled(int acc, float sa, float sw) { return ((float)acc * sw) * sa; }
 
-// Stores NV consecutive values of one row, from column c on.
+// Stores NV consecutive values of one row, from column c on, 16 bytes at a time whatever the row's alignment: the memory unit splits
+// a store where it crosses a line.  Through LDS, so that stores run along rows 4 bytes per lane, the product of 2165 x 7870 x 4123 took
+// 123 us against 109, of 8100 x 12289 x 2048 263 against 271.
 template <int NV>
 __device__ __forceinline__ void i8_store(const I8Params& p, int m, int c, const float* y) {
-    if (p.vec_out && c + NV <= p.N) {
+    if (c + NV <= p.N) {
         if (p.out_f32) {
+            struct __attribute__((packed, aligned(4))) Loose { float x, y, z, w; };
             float* o = (float*)p.out + (int64_t)m * p.ldo + c;
 #pragma unroll
-            for (int e = 0; e < NV; e += 4) *(float4*)(o + e) = make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]);
+            for (int e = 0; e < NV; e += 4) *(Loose*)(o + e) = Loose{y[e], y[e + 1], y[e + 2], y[e + 3]};
         } else {
+            struct __attribute__((packed, aligned(2))) Loose { uint32_t x[NV < 8 ? 2 : 4]; };
             bf16_t* o = (bf16_t*)p.out + (int64_t)m * p.ldo + c;
 #pragma unroll
-            for (int e = 0; e < NV; e += 8)
-                *(uint4*)(o + e) = make_uint4(pack_bf16x2(y[e], y[e + 1]), pack_bf16x2(y[e + 2], y[e + 3]),
-                                              pack_bf16x2(y[e + 4], y[e + 5]), pack_bf16x2(y[e + 6], y[e + 7]));
+            for (int e = 0; e < NV; e += 8) {
+                Loose v;
+#pragma unroll
+                for (int j = 0; j < (NV < 8 ? 2 : 4); ++j) v.x[j] = pack_bf16x2(y[e + 2 * j], y[e + 2 * j + 1]);
+                *(Loose*)(o + e) = v;
+            }
         }
         return;
     }
@@ -196,34 +212,6 @@ __device__ __forceinline__ void i8_store(const I8Params& p, int m, int c, const 
             if (p.out_f32) ((float*)p.out)[(int64_t)m * p.ldo + c + e] = y[e];
             else ((bf16_t*)p.out)[(int64_t)m * p.ldo + c + e] = f32_to_bf16(y[e]);
         }
-}
-
-// The same for rows that cannot take 16-byte stores: a wave's block of 16 rows x 4 * NC columns goes through its own piece of LDS, ROWS
-// rows of 4 * NC + 1 words at a time, so that a store instruction writes along rows instead of touching 64 lines.
-template <int NC, int ROWS>
-__device__ __forceinline__ void i8_store_rows(const I8Params& p, int m, int c, const float* y, float* piece) {
-    constexpr int W = 4 * NC;
-    const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
-#pragma unroll
-    for (int h = 0; h < 16 / ROWS; ++h) {
-        __builtin_amdgcn_wave_barrier();
-        if (li / ROWS == h) {
-#pragma unroll
-            for (int e = 0; e < NC; ++e) piece[li % ROWS * (W + 1) + lg * NC + e] = y[e];
-        }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#pragma unroll
-        for (int i = 0; i < ROWS * W / 64; ++i) {
-            const int r = (i * 64 + lane) / W, q = (i * 64 + lane) % W, row = m + h * ROWS + r, col = c + q;
-            const float v = piece[r * (W + 1) + q];
-            if (row < p.M && col < p.N) {
-                if (p.out_f32) ((float*)p.out)[(int64_t)row * p.ldo + col] = v;
-                else ((bf16_t*)p.out)[(int64_t)row * p.ldo + col] = f32_to_bf16(v);
-            }
-        }
-    }
 }
 
 // Tile BM x BN x 128 per 256-thread workgroup (4 waves as 2 x 2).  Operands are staged global -> LDS by 16-byte loads into a
@@ -354,18 +342,15 @@ __global__ __launch_bounds__(256, 2) void i8_gemm_kernel(I8Params p) {
     }
 
     // epilogue: lane (li, lg) owns row m, columns c0 .. c0 + 4 * NT - 1
-    float* const piece = (float*)smem + uwave * 16 * (16 * NT + 1);
-    if (!p.vec_out) __syncthreads();   // the tiles in LDS have been read by all waves
 #pragma unroll
     for (int a = 0; a < MT; ++a) {
-        const int m = m0 + wr * 16 * MT + a * 16;
+        const int m = m0 + wr * 16 * MT + a * 16 + li;
         float y[4 * NT];
 #pragma unroll
         for (int b = 0; b < NT; ++b)
 #pragma unroll
             for (int r = 0; r < 4; ++r) y[b * 4 + r] = i8_scaled(acc[a][b][r], scale_a[a], scale_w[b * 4 + r]) + bias[b * 4 + r];
-        if (!p.vec_out) i8_store_rows<4 * NT, 16>(p, m, n0 + wc * 16 * NT, y, piece);
-        else if (m + li < p.M) i8_store<4 * NT>(p, m + li, c0, y);
+        if (m < p.M) i8_store<4 * NT>(p, m, c0, y);
     }
 }
 
@@ -377,8 +362,8 @@ __global__ __launch_bounds__(256, 2) void i8_gemm_kernel(I8Params p) {
 // 16x16x32 bf16 or one 16x16x64 int8 MFMA of the same length.  Twice the work per byte moved, so the phases are the same and
 // the rate doubles.
 constexpr int UNIT = 128 * 128, BUF = 4 * UNIT;   // A0 | A1 | W0 | W1, two K tiles
-constexpr int SCALES = 3 * 256 * 4, PIECE = 8 * 65 * 4;
-constexpr int LDS256 = 2 * BUF + 2 * SCALES + 8 * PIECE;   // scales of the tile's rows, columns, and the bias, for two tiles; a piece per wave
+constexpr int SCALES = 3 * 256 * 4;
+constexpr int LDS256 = 2 * BUF + 2 * SCALES;   // scales of the tile's rows, columns, and the bias, for two tiles
 
 __global__ __launch_bounds__(512, 2) void i8_gemm256_kernel(I8Params p) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -560,16 +545,11 @@ __global__ __launch_bounds__(512, 2) void i8_gemm256_kernel(I8Params p) {
         for (int a = 0; a < 2; ++a)
 #pragma unroll
             for (int f = 0; f < 4; ++f) {
-                const int m = e_m0 + wr * 128 + a * 64 + f * 16;
+                const int m = e_m0 + wr * 128 + a * 64 + f * 16 + li;
                 float y[16];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) y[e] = __int_as_float(acc[a][f][e >> 3][(e >> 2) & 1][e & 3]);
-                if (!p.vec_out) {
-                    float* const piece = (float*)(smem + 2 * BUF + 2 * SCALES + uwave * PIECE);
-                    i8_store_rows<16, 8>(p, m, e_n0 + wc * 64, y, piece);
-                } else if (m + li < p.M) {
-                    i8_store<16>(p, m + li, e_n0 + c0, y);
-                }
+                if (m < p.M) i8_store<16>(p, m, e_n0 + c0, y);
             }
     }
 }
@@ -590,9 +570,9 @@ void launch_gemm256(const I8Params& p, hipStream_t s) {
 // wave's share of up to NS steps is requested at once.  The activation rows are rounded to 8 bits by every workgroup for itself,
 // underneath those loads: they are a few KB from the L2, and a second kernel in front would cost more than the whole product.
 // Weight rows are the MFMA "A" operand (lane: row li, bytes 16 lg ..), the activation rows in LDS the "B".
-// FROM: 0 bf16 rows, 1 fp32 rows, 2 rows that are rounded already.  HELD > 0: the rows are aligned to 16 bytes, K is a multiple
-// of 8 and a thread's share of the rows, at most HELD pieces of 8 values, is requested before the weights and held in registers, so
-// that nothing waits behind the weights; 0: rows of any alignment and number, read twice.
+// FROM: 0 bf16 rows, 1 fp32 rows, 2 rows that are rounded already.  HELD > 0: K is at least 8 and a thread's share of the rows, at
+// most HELD pieces of 8 values, is requested before the weights and held in registers, so that nothing waits behind the weights; 0:
+// any K, read twice.
 constexpr int FEW_THREADS = 512, FEW_WAVES = 8, FEW_ROWS = 6, FEW_LDS = 100 * 1024;
 constexpr int FEW_RED = FEW_WAVES * 256 * 4;
 __host__ __device__ inline int few_stride(int K) { return ((K + 63) & ~63) + 16; }   // rows 16 bytes apart modulo the banks
@@ -634,12 +614,31 @@ __global__ __launch_bounds__(FEW_THREADS, 2) void i8_few_rows_kernel(I8Params p,
             k_of[i] = (c - row_of[i] * per_row) * 8;
             const char* at = (const char*)src.x + ((int64_t)row_of[i] * src.ldx + min(k_of[i], p.K - 8)) * (F32 ? 4 : 2);
 #pragma unroll
-            for (int j = 0; j < WORDS; ++j) held[i][j] = *(const uint4*)(at + 16 * j);
+            for (int j = 0; j < WORDS; ++j) held[i][j] = i8_load16(at + 16 * j);
         }
         __builtin_amdgcn_sched_barrier(0);
         request(n0, 0);
         __builtin_amdgcn_sched_barrier(0);
         __syncthreads();
+        if (p.K & 7) {   // a row's last piece was read from its last 8 values: what precedes it moves out
+#pragma unroll
+            for (int i = 0; i < HELD; ++i) {
+                const int by = k_of[i] < p.K ? max(k_of[i] + 8 - p.K, 0) : 0;
+                uint32_t word[9] = {held[i][0].x, held[i][0].y, held[i][0].z, held[i][0].w, 0, 0, 0, 0, 0};
+                if constexpr (F32) { word[4] = held[i][1].x; word[5] = held[i][1].y; word[6] = held[i][1].z; word[7] = held[i][1].w; }
+                const int words = F32 ? by : by >> 1;
+#pragma unroll
+                for (int step = 4; step; step >>= 1)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) word[e] = words & step ? (e + step < 8 ? word[e + step] : 0u) : word[e];
+                if (!F32 && (by & 1)) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) word[e] = __builtin_amdgcn_alignbit(word[e + 1], word[e], 16);
+                }
+                held[i][0] = make_uint4(word[0], word[1], word[2], word[3]);
+                if constexpr (F32) held[i][1] = make_uint4(word[4], word[5], word[6], word[7]);
+            }
+        }
         auto values = [&](int i, float* v) {
             const uint32_t word[8] = {held[i][0].x, held[i][0].y, held[i][0].z, held[i][0].w,
                                       held[i][WORDS - 1].x, held[i][WORDS - 1].y, held[i][WORDS - 1].z, held[i][WORDS - 1].w};
@@ -692,7 +691,7 @@ __global__ __launch_bounds__(FEW_THREADS, 2) void i8_few_rows_kernel(I8Params p,
             const int c = min(c0 + tid, pieces - 1), m = c / per_row, k = (c - m * per_row) * 8;
             const char* row = (const char*)src.x + (int64_t)m * src.ldx * (F32 ? 4 : 2);
             float v[8];
-            i8_load8<F32>(row, k, p.K, (uintptr_t)row % 16 == 0, v);
+            i8_load8<F32>(row, k, p.K, v);
             const uint32_t top = i8_max8(0, v);
             const int first = __builtin_amdgcn_readfirstlane(m);
             if (first == __builtin_amdgcn_readlane(m, 63)) {
@@ -710,7 +709,7 @@ __global__ __launch_bounds__(FEW_THREADS, 2) void i8_few_rows_kernel(I8Params p,
             const RowScale rs = scales[m];
             const char* row = (const char*)src.x + (int64_t)m * src.ldx * (F32 ? 4 : 2);
             float v[8];
-            i8_load8<F32>(row, k, p.K, (uintptr_t)row % 16 == 0, v);
+            i8_load8<F32>(row, k, p.K, v);
             *(uint2*)(xq + m * stride + k) = rs.pack8(v);
         }
         request(n0, 0);
@@ -773,11 +772,10 @@ void launch_few_steps(const I8Params& p, const I8Source& src, hipStream_t s) {
 template <int FROM>
 bool launch_few_rows(const I8Params& p, const I8Source& src, hipStream_t s) {
     const int64_t held = cdiv((int64_t)p.M * (few_stride(p.K) >> 3), FEW_THREADS);
-    const bool vec = p.K % 8 == 0 && (uintptr_t)src.x % 16 == 0 && src.ldx * (src.f32 ? 4 : 2) % 16 == 0;
-    if (p.M > FEW_ROWS || held > (vec ? 8 : 2)) return false;
-    if (vec && held <= 2) launch_few_steps<FROM, 2>(p, src, s);
-    else if (vec) launch_few_steps<FROM, 8>(p, src, s);
-    else launch_few_steps<FROM, 0>(p, src, s);
+    if (p.M > FEW_ROWS || held > 8) return false;
+    if (p.K < 8) launch_few_steps<FROM, 0>(p, src, s);
+    else if (held <= 2) launch_few_steps<FROM, 2>(p, src, s);
+    else launch_few_steps<FROM, 8>(p, src, s);
     return true;
 }
 
@@ -822,12 +820,11 @@ bool launch_i8_linear_few_rows(const I8Params& p, const I8Source& src, hipStream
     return src.f32 ? launch_few_rows<1>(p, src, s) : launch_few_rows<0>(p, src, s);
 }
 
-void launch_i8_matmul(I8Params p, hipStream_t s) {
+void launch_i8_matmul(const I8Params& p, hipStream_t s) {
     if (p.M <= FEW_ROWS && p.M * (int64_t)few_stride(p.K) <= FEW_LDS) {
         launch_few_steps<2, 0>(p, {}, s);
         return;
     }
-    p.vec_out = ((uintptr_t)p.out % 16 == 0) && p.ldo % (p.out_f32 ? 4 : 8) == 0;
     // The smallest tiles that still fit the device at once win while the sums are short of workgroups, because the walk along K
     // is then all latency (us at K = 2048, and 6144 with *; 32 x 32 by 512 bytes of K, 32 x 64 by 512, by 256, 64 x 64, 128 x 128,
     // 256 x 256):  64 x 4096: 5.0, 5.7, 5.9, 8.2, 13.8, 24;  128 x 2048*: 8.7, 11.1, 12.6, 18, 37, 58;  256 x 4096: 14, 9.8, 7.7, 8.3,

@@ -128,6 +128,32 @@ def test_linear_matches_whole_numbers(tiny_model, m, n, k, x, out, bias):
     assert (np.abs(got - want) <= tol + 1e-37).all()
 
 
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("m,ks", [(1, range(7, 26)), (3, range(513, 523)), (5, range(2094, 2103)), (6, (1363, 1364)), (40, range(130, 139))])
+def test_linear_of_any_length_and_alignment(tiny_model, m, ks, kind):
+    """Every length against whole pieces of 8 values; activations and outputs begin one value behind an aligned address."""
+    from q3asr import Int8Linear
+    rng = np.random.default_rng(m)
+    n, size, dt = 90, 4 if kind == "f32" else 2, np.float32 if kind == "f32" else np.uint16
+    for k in ks:
+        xs = _rows(rng, m, k, kind)
+        w, ldw, sw = _weights(rng, n, k)
+        with Device() as dev:
+            lin = Int8Linear(tiny_model[0], dev.put(w), dev.put(sw), n, k, ldw=ldw)
+            ws, o = lin.workspace_bytes(m), dev.put(np.full(m * n + 2, 7, dt))
+            flat = np.full(m * k + 2, np.nan, np.float32)
+            flat[1:-1] = xs.reshape(-1)
+            x = dev.put(flat if kind == "f32" else bf16_bits(flat))
+            lin(x + size, m, o + size, x_dtype=kind, out_dtype=kind, workspace=(dev.raw(ws), ws))
+            got = dev.get(o, m * n + 2, dt)
+        assert got[0] == 7 and got[-1] == 7
+        got = (got if kind == "f32" else bf16_vals(got))[1:-1].reshape(m, n).astype(np.float64)
+        s, q = _quantize64(xs)
+        want = (q.astype(np.float64) @ w[:, :k].astype(np.float64).T) * s.astype(np.float64)[:, None] * sw.astype(np.float64)
+        tol = 3.01 * F32_HALF_STEP * np.abs(want) + (1.01 * BF16_HALF_STEP * np.abs(want) if kind == "bf16" else 0)
+        assert (np.abs(got - want) <= tol + 1e-37).all(), k
+
+
 @pytest.mark.parametrize("m,n,k", [(1, 40, 64), (6, 300, 4096), (70, 130, 1024), (260, 300, 2048), (1000, 768, 131056 // 16), (2, 3, 131056)])
 def test_matmul_equals_linear_and_extremes(tiny_model, m, n, k):
     """quantize + matmul gives linear's bits; -128 (which quantize never makes) and rows of +-127 sum without overflow."""
