@@ -20,6 +20,8 @@
 #include "paged.h"
 #include "prof.h"
 #include <algorithm>
+#include <cmath>
+#include <limits>
 #include <type_traits>
 
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
@@ -87,7 +89,8 @@ struct AttnParams {
     int max_seqs, max_seq_pages, pages, pt_shift;
     int n, rows, n_groups, heads, kv_heads, group;
     int max_rows, max_group_rows, max_len, max_own, max_shared;
-    float scale_log2;
+    float scale_log2;                          // positive; a negative scale's sign is taken into the queries
+    uint32_t flip;
     int shift_q;                               // query rows of a wave: 16 * QT = 1 << shift_q
     int tiles_q;                               // plain: query tiles of a sequence
     int per_min, slots_p, slots;               // parts of a row at most: of its group's segment first
@@ -272,9 +275,12 @@ struct Rows {
     static constexpr int TILE = 32 * VROW;
 };
 
-template <int D, int QT>
+// ONCE: no key is read by several waves, so its rows need not stay in a cache.  Loads that say so take 144 us where others take 161
+// (256 sequences after 900 tokens, 8 KV heads of 128); where three query tiles read each key they take 34 against 27 (7 x 24 rows
+// after 1111 tokens, 12 groups, 14 heads of 64).
+template <int D, int QT, bool ONCE>
 struct Wave {
-    static constexpr int NKS = D / 32, NDT = D / 16, LPR = D / 8, RPI = 64 / LPR, IV = 16 / RPI;
+    static constexpr int NKS = D / 32, NDT = D / 16, LPR = D / 8, RPI = 64 / LPR, IV = 16 / RPI, PAIR = QT < 2 ? 1 : 2;
     static constexpr int KROW = Rows<D>::KROW, VROW = Rows<D>::VROW;
     const AttnParams& p;
     const int lane, li, lg;
@@ -284,7 +290,10 @@ struct Wave {
     int limit[QT];                // the lane's queries see keys below
     int lowest;                   // keys below it are seen by all of them
     int active;                   // groups of 16 queries that there are
-    float m[QT], l[QT];           // l: of this lane's keys only, until the end
+    // Weights are powers of two above m, a bound that no score so far exceeds by more than SLACK: it is only moved, and the sums
+    // with it, when one does.  So weights are below 2^SLACK; fp32 sums and the relative rounding to bf16 are as good there.
+    static constexpr float SLACK = 8.f;
+    float m[QT], less[QT], l[QT];   // less: -m, 0 while there is no m; l: of this lane's keys only, until the end
     f32x4 o[QT][NDT];             // lane (li, lg) holds values 16 dt + 4 lg .. of query 16 qt + li
     int ids, id_base;             // page numbers of 64 times 16 keys from key id_base on, one per lane
     __device__ Wave(const AttnParams& p_, char* tile_) : p(p_), lane(threadIdx.x & 63), li(threadIdx.x & 15), lg((threadIdx.x & 63) >> 4), tile(tile_) {}
@@ -302,6 +311,10 @@ struct Wave {
         const int64_t page = __builtin_amdgcn_readlane(ids, (key - id_base) >> 4);
         return page * p.page_stride + head + (int64_t)(key & ((1 << p.pt_shift) - 1)) * D;
     }
+    static __device__ __forceinline__ bf16x8 row(const bf16x8* at) {
+        if constexpr (ONCE) return __builtin_nontemporal_load(at);
+        else return *at;
+    }
     // Keys behind the last one are read from its row, so that they cost no memory traffic.
     __device__ void load(const bf16_t* pool, Frag (&x)[2][IV], int64_t head, int kv0, int k1) const {
         if (kv0 + 32 <= k1) {
@@ -309,7 +322,7 @@ struct Wave {
             for (int h = 0; h < 2; ++h) {
                 const bf16_t* src = pool + base_of(head, kv0 + 16 * h) + (lane / LPR) * D + 8 * (lane % LPR);
 #pragma unroll
-                for (int i = 0; i < IV; ++i) x[h][i].v = __builtin_nontemporal_load((const bf16x8*)(src + i * RPI * D));
+                for (int i = 0; i < IV; ++i) x[h][i].v = row((const bf16x8*)(src + i * RPI * D));
             }
         } else {
 #pragma unroll
@@ -318,7 +331,7 @@ struct Wave {
                 const bf16_t* src = pool + base_of(head, key) + 8 * (lane % LPR);
 #pragma unroll
                 for (int i = 0; i < IV; ++i)
-                    x[h][i].v = __builtin_nontemporal_load((const bf16x8*)(src + min(lane / LPR + i * RPI, k1 - 1 - key) * D));
+                    x[h][i].v = row((const bf16x8*)(src + min(lane / LPR + i * RPI, k1 - 1 - key) * D));
             }
         }
     }
@@ -331,9 +344,12 @@ struct Wave {
             limit[qt] = !ok ? 0 : sg.limit == SHARED ? sg.k1 : min(sg.k1, sg.limit + tok);
             const bf16_t* src = p.q + (int64_t)(sg.r0 + tok) * p.q_ld + (kvh * p.group + (ok ? r - tok * p.group : 0)) * D + 8 * lg;
 #pragma unroll
-            for (int ks = 0; ks < NKS; ++ks) qf[qt][ks].u = *(const uint4*)(src + 32 * ks);
+            for (int ks = 0; ks < NKS; ++ks) {
+                const uint4 u = *(const uint4*)(src + 32 * ks);
+                qf[qt][ks].u = make_uint4(u.x ^ p.flip, u.y ^ p.flip, u.z ^ p.flip, u.w ^ p.flip);
+            }
             m[qt] = -INFINITY;
-            l[qt] = 0.f;
+            less[qt] = l[qt] = 0.f;
 #pragma unroll
             for (int dt = 0; dt < NDT; ++dt) o[qt][dt] = (f32x4){0.f, 0.f, 0.f, 0.f};
         }
@@ -360,41 +376,59 @@ struct Wave {
 #pragma unroll
             for (int ks = 0; ks < NKS; ++ks) ka[h][ks].u = *(const uint4*)(kr + 16 * h * KROW + 64 * ks);
         Frag pf[QT];
-        float alpha[QT];
-        bool moved = false;
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt) {
-            if (qt > 0 && qt >= active) break;   // wave-uniform
-            f32x4 s[2];
+        for (int g = 0; g < QT; g += PAIR) {
+            if (g > 0 && g >= active) break;   // wave-uniform
+            f32x4 s[PAIR][2];
+            float top[PAIR];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                s[h] = (f32x4){0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < PAIR; ++i)
 #pragma unroll
-                for (int ks = 0; ks < NKS; ++ks) s[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka[h][ks].v, qf[qt][ks].v, s[h], 0, 0, 0);
-            }
-            float sv[8], top = -INFINITY;
+                for (int h = 0; h < 2; ++h) {
+                    s[i][h] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int j = 0; j < 8; ++j) sv[j] = s[j >> 2][j & 3] * p.scale_log2;
+                    for (int ks = 0; ks < NKS; ++ks) s[i][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka[h][ks].v, qf[g + i][ks].v, s[i][h], 0, 0, 0);
+                }
             if (kv0 + 32 > lowest) {   // wave-uniform
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (kv0 + 16 * (j >> 2) + 4 * lg + (j & 3) >= limit[qt]) sv[j] = -INFINITY;
+                for (int i = 0; i < PAIR; ++i)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (kv0 + 16 * (j >> 2) + 4 * lg + (j & 3) >= limit[g + i]) s[i][j >> 2][j & 3] = -INFINITY;
+            }
+            bool beyond = false;
+#pragma unroll
+            for (int i = 0; i < PAIR; ++i) {
+                top[i] = s[i][0][0];
+#pragma unroll
+                for (int j = 1; j < 8; ++j) top[i] = __builtin_elementwise_maximum(top[i], s[i][j >> 2][j & 3]);   // a NaN stays: the row is NaN
+                beyond |= top[i] * p.scale_log2 > m[g + i] + SLACK;
+            }
+            if (__builtin_amdgcn_ballot_w64(beyond) != 0) {
+#pragma unroll
+                for (int i = 0; i < PAIR; ++i) {
+                    const int qt = g + i;
+                    const float m_new = fmaxf(m[qt], rows_max(top[i]) * p.scale_log2);
+                    const float use = m_new == -INFINITY ? 0.f : m_new;   // no key seen yet
+                    const float alpha = __builtin_amdgcn_exp2f(m[qt] - use);
+                    m[qt] = m_new;
+                    less[qt] = -use;
+                    l[qt] *= alpha;
+#pragma unroll
+                    for (int dt = 0; dt < NDT; ++dt) o[qt][dt] *= alpha;
+                }
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) top = fmaxf(top, sv[j]);
-            const float m_new = fmaxf(m[qt], rows_max(top));
-            const float m_use = m_new == -INFINITY ? 0.f : m_new;   // no key seen yet
-            alpha[qt] = __builtin_amdgcn_exp2f(m[qt] - m_use);
-            float pe[8], ps = 0.f;
+            for (int i = 0; i < PAIR; ++i) {
+                const int qt = g + i;
+                float pe[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                pe[j] = __builtin_amdgcn_exp2f(sv[j] - m_use);
-                ps += pe[j];
+                for (int j = 0; j < 8; ++j) {
+                    pe[j] = __builtin_amdgcn_exp2f(fmaf(s[i][j >> 2][j & 3], p.scale_log2, less[qt]));
+                    l[qt] += pe[j];
+                }
+                pf[qt].u = make_uint4(pack_bf16x2(pe[0], pe[1]), pack_bf16x2(pe[2], pe[3]), pack_bf16x2(pe[4], pe[5]), pack_bf16x2(pe[6], pe[7]));
             }
-            l[qt] = l[qt] * alpha[qt] + ps;
-            moved |= m_new != m[qt];
-            m[qt] = m_new;
-            pf[qt].u = make_uint4(pack_bf16x2(pe[0], pe[1]), pack_bf16x2(pe[2], pe[3]), pack_bf16x2(pe[4], pe[5]), pack_bf16x2(pe[6], pe[7]));
         }
         __builtin_amdgcn_wave_barrier();   // the V rows go where the K rows were
         if (kv0 + 32 > k1) {
@@ -411,14 +445,6 @@ struct Wave {
             for (int i = 0; i < IV; ++i) *(uint4*)(vw + (16 * h + i * RPI) * VROW) = vf[h][i].u;
         next_v();
         wave_lds_fence();
-        if (__builtin_amdgcn_ballot_w64(moved) != 0) {
-#pragma unroll
-            for (int qt = 0; qt < QT; ++qt) {
-                if (qt > 0 && qt >= active) break;
-#pragma unroll
-                for (int dt = 0; dt < NDT; ++dt) o[qt][dt] *= alpha[qt];
-            }
-        }
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) {
             union { s16x4 v; uint2 u; } lo, hi;   // keys 4 lg .. 4 lg + 3 and 16 + 4 lg .. of dim 16 dt + li
@@ -429,7 +455,7 @@ struct Wave {
             va.h[1] = hi.u;
 #pragma unroll
             for (int qt = 0; qt < QT; ++qt) {
-                if (qt > 0 && qt >= active) break;
+                if (qt >= PAIR && qt / PAIR * PAIR >= active) break;
                 o[qt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va.v, pf[qt].v, o[qt][dt], 0, 0, 0);
             }
         }
@@ -441,7 +467,7 @@ __device__ __forceinline__ float lse_of(float m, float l) { return (m + __builti
 __device__ __forceinline__ float inverse_of(float l) { return l > 0.f || l != l ? 1.0f / l : 0.f; }   // no keys: zeros
 
 // ---- stream ----
-template <int D, int QT, bool PLANNED>
+template <int D, int QT, bool ONCE, bool PLANNED>
 __global__ __launch_bounds__(256, 2) void paged_attn_stream_kernel(AttnParams p) {
     constexpr int PLAN_BYTES = PLANNED ? 0 : HELD * (int)sizeof(Entry) + (3 * HELD + 2 + WAVES) * 4, TILES = WAVES * Rows<D>::TILE;
     __shared__ __attribute__((aligned(16))) char lds[PLAN_BYTES > TILES ? PLAN_BYTES : TILES];
@@ -455,11 +481,18 @@ __global__ __launch_bounds__(256, 2) void paged_attn_stream_kernel(AttnParams p)
         total = plan_segments<256>(p, PlanMemory{(Entry*)lds, ints, ints + HELD, ints + 2 * HELD + 1, ints + 3 * HELD + 2, held}, blockIdx.x == 0);
         __syncthreads();   // the tiles go where the plan was made
     }
-    const int64_t begin = (int64_t)(blockIdx.x * WAVES + wave) * total.per;   // may lie behind what 32 bits hold, places do not
+    int share = blockIdx.x;
+    if constexpr (!ONCE) {   // neighbouring shares go to one XCD, in whose L2 all query tiles but the first find their keys
+        const int64_t used = (((int64_t)total.places + total.per - 1) / total.per + WAVES - 1) / WAVES;
+        const int chunk = (int)((used + 7) >> 3);
+        if ((int)(blockIdx.x >> 3) >= chunk) return;
+        share = (blockIdx.x & 7) * chunk + (blockIdx.x >> 3);
+    }
+    const int64_t begin = (int64_t)(share * WAVES + wave) * total.per;   // may lie behind what 32 bits hold, places do not
     if (begin >= total.places) return;
     int pos = (int)begin;
     const int end = (int)min((int64_t)total.places, begin + total.per);
-    Wave<D, QT> w(p, lds + wave * Rows<D>::TILE);
+    Wave<D, QT, ONCE> w(p, lds + wave * Rows<D>::TILE);
 
     // the last segment that begins at or before pos: 64 probes at a time
     int lo = 0, hi = total.segments;
@@ -575,11 +608,12 @@ __global__ __launch_bounds__(256, 2) void paged_attn_stream_kernel(AttnParams p)
     tile(std::true_type{});
 }
 
-// Joins the parts of a row that has several, and writes rows without keys: D / 2 lanes per (row, head).
-template <int D>
+// Joins the parts of a row that has several, and writes rows without keys: D / 2 lanes per (row, head), or (SPREAD) a workgroup, whose
+// teams of D / 2 lanes take its parts in turn.
+template <int D, bool SPREAD>
 __global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnParams p) {
-    constexpr int LANES = D / 2;
-    const int lane = threadIdx.x % LANES, row = blockIdx.x, hq = blockIdx.y * (256 / LANES) + threadIdx.x / LANES;
+    constexpr int LANES = D / 2, TEAMS = 256 / LANES;
+    const int lane = threadIdx.x % LANES, team = threadIdx.x / LANES, row = blockIdx.x, hq = SPREAD ? blockIdx.y : blockIdx.y * TEAMS + team;
     const RowParts rp = p.parts[row];
     const int per = p.total->per;
     if (hq >= p.heads || !rp.known) return;
@@ -626,7 +660,48 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnParams p) {
             a1 += v[a].y * f;
         }
     };
-    if (n > 8) {
+    if constexpr (SPREAD) {
+        __shared__ float2 ml_of[TEAMS], sum_of[TEAMS][LANES];
+        for (int i0 = team; i0 < n; i0 += 8 * TEAMS) {   // eight parts requested at a time, behind the last one the last again
+            float2 ml[8], v[8];
+#pragma unroll
+            for (int a = 0; a < 8; ++a) {
+                const int64_t at = slot_of(min(i0 + a * TEAMS, n - 1));
+                ml[a] = p.part_ml[at];
+                v[a] = *(const float2*)(p.part_o + at * D + lane * 2);
+            }
+            float top = M;
+#pragma unroll
+            for (int a = 0; a < 8; ++a) top = fmaxf(top, ml[a].x);
+            const float use = top == -INFINITY ? 0.f : top, before = __builtin_amdgcn_exp2f(M - use);
+            M = top;
+            L *= before;
+            a0 *= before;
+            a1 *= before;
+#pragma unroll
+            for (int a = 0; a < 8; ++a) {
+                const float f = i0 + a * TEAMS < n ? __builtin_amdgcn_exp2f(ml[a].x - use) : 0.f;
+                L += ml[a].y * f;
+                a0 += v[a].x * f;
+                a1 += v[a].y * f;
+            }
+        }
+        if (lane == 0) ml_of[team] = make_float2(M, L);
+        sum_of[team][lane] = make_float2(a0, a1);
+        __syncthreads();
+        if (team > 0) return;
+#pragma unroll
+        for (int t = 0; t < TEAMS; ++t) M = fmaxf(M, ml_of[t].x);
+        const float use = M == -INFINITY ? 0.f : M;
+        L = a0 = a1 = 0.f;
+#pragma unroll
+        for (int t = 0; t < TEAMS; ++t) {
+            const float f = __builtin_amdgcn_exp2f(ml_of[t].x - use);
+            L += ml_of[t].y * f;
+            a0 += sum_of[t][lane].x * f;
+            a1 += sum_of[t][lane].y * f;
+        }
+    } else if (n > 8) {
         for (int i = lane; i < n; i += LANES) M = fmaxf(M, p.part_ml[slot_of(i)].x);
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, LANES));
@@ -661,7 +736,7 @@ __global__ __launch_bounds__(64 * PLAIN_WAVES) void paged_attn_plain_kernel(Attn
     const Segment sg{e.r0, e.T * p.group, e.seq, 0, min(e.len, PLAIN_KEYS), e.len - e.T + 1, 0, 1};
     const int first = (x - i * p.tiles_q) * 16 * QT, ntiles = (sg.k1 + 31) >> 5;
     if (first >= sg.M) return;
-    Wave<D, QT> w(p, lds + wave * Rows<D>::TILE);
+    Wave<D, QT, true> w(p, lds + wave * Rows<D>::TILE);
     const int64_t head = (int64_t)kvh * p.head_stride;
     int t = wave;
     if (t < ntiles) {
@@ -718,7 +793,7 @@ __global__ __launch_bounds__(64 * PLAIN_WAVES) void paged_attn_plain_kernel(Attn
 }
 
 struct Plan {
-    bool plain;
+    bool plain, once, spread;
     int qt, tiles_q, per_min, slots_p, slots;
     int64_t at_plan, at_segments, at_parts, at_ml, at_o, bytes;
 };
@@ -726,16 +801,20 @@ bool groups_count(const q3asr_kv_pages& c, const q3asr_attn_batch& b) { return b
 Plan plan_for(const q3asr_kv_pages& c, const q3asr_attn_batch& b, int heads) {
     Plan r{};
     const int group = heads / c.kv_heads;
-    // A small step is all latency: whole sequences that fit the device at once, shared or not, in one launch.
+    // A small step is all latency: whole sequences that fit the device at once, shared or not, in one launch (head_dim 128: two
+    // workgroups per CU, 64: three, or four that follow soon).  us against the stream, the write of the step included: 128 sequences
+    // of 20 and of 900 tokens, 4 KV heads of 128: 11, 26 (there PLAIN_ITEMS is reached); 8 KV heads: 17, 40 against 13, 29; 256 of 20,
+    // 210, 450 and 900 tokens, 4 KV heads of 64: 11, 15, 18, 25 against 12, 19, 22, 24.
     r.qt = (int64_t)b.max_rows * group <= 16 ? 1 : 2;
     r.tiles_q = cdiv((int64_t)b.max_rows * group, 16 * r.qt);
-    r.plain = b.max_len <= PLAIN_KEYS && (int64_t)b.n * r.tiles_q * c.kv_heads <= PLAIN_ITEMS;
+    r.plain = b.max_len <= PLAIN_KEYS && (int64_t)b.n * r.tiles_q * c.kv_heads <= (c.head_dim == 128 ? PLAIN_ITEMS : 2 * PLAIN_ITEMS);
     if (r.plain) return r;
     const bool shares = groups_count(c, b);
     const int64_t rows = (int64_t)(shares ? b.max_group_rows : b.max_rows) * group;
     // as many rows at once as the registers of two waves per SIMD hold (64 x 128 sums do not fit; 64 x 64 against 32 x 64 at three
     // waves: 34 against 39 us for 7 x 24 rows after 1111 tokens, 12 groups, 14 heads)
     r.qt = rows <= 16 ? 1 : rows <= 32 || c.head_dim == 128 ? 2 : 4;
+    r.once = rows <= 16 * r.qt;
     // Parts of a row: tiles of its longest segment by the least tiles of a wave, and one for where it begins.  More parts spread a few
     // long sequences over the device; their memory is kept to 64 MB (but 16 parts).
     const int64_t part = (int64_t)b.rows * heads * (c.head_dim * 4 + 8);
@@ -744,6 +823,7 @@ Plan plan_for(const q3asr_kv_pages& c, const q3asr_attn_batch& b, int heads) {
     r.per_min = std::max(2, cdiv(cdiv(longest, 32), most));
     r.slots_p = shares ? cdiv(cdiv(b.max_shared, 32), r.per_min) + 1 : 0;
     r.slots = r.slots_p + cdiv(cdiv(own, 32), r.per_min) + 1;
+    r.spread = r.slots > 32 && (int64_t)b.rows * heads <= 1024;
     auto round = [](int64_t x) { return (x + 255) & ~255ll; };
     const int64_t groups = shares ? b.n_groups : 0;
     r.at_plan = 256;
@@ -773,15 +853,18 @@ void launch_d(const AttnParams& p, const Plan& r, hipStream_t s) {
         HIP_CHECK(hipGetLastError());
     }
     constexpr int MOST = D == 128 ? 2 : 4;
-#define STREAM(QT)                                                                                                  \
-    if (planned) hipLaunchKernelGGL((paged_attn_stream_kernel<D, QT, true>), grid, block, 0, s, p);                 \
-    else hipLaunchKernelGGL((paged_attn_stream_kernel<D, QT, false>), grid, block, 0, s, p)
-    if (r.qt == 1) { STREAM(1); }
-    else if (r.qt == 2) { STREAM(2); }
-    else { STREAM(MOST); }
-#undef STREAM
+    auto stream = [&](auto qt, auto once) {
+        if (planned) hipLaunchKernelGGL((paged_attn_stream_kernel<D, decltype(qt)::value, decltype(once)::value, true>), grid, block, 0, s, p);
+        else hipLaunchKernelGGL((paged_attn_stream_kernel<D, decltype(qt)::value, decltype(once)::value, false>), grid, block, 0, s, p);
+    };
+    if (r.qt == 1) stream(std::integral_constant<int, 1>{}, std::true_type{});
+    else if (r.once && r.qt == 2) stream(std::integral_constant<int, 2>{}, std::true_type{});
+    else if (r.qt == 2) stream(std::integral_constant<int, 2>{}, std::false_type{});
+    else if (r.once) stream(std::integral_constant<int, MOST>{}, std::true_type{});
+    else stream(std::integral_constant<int, MOST>{}, std::false_type{});
     HIP_CHECK(hipGetLastError());
-    hipLaunchKernelGGL((paged_attn_join_kernel<D>), dim3(p.rows, cdiv(p.heads, 256 / (D / 2))), block, 0, s, p);
+    if (r.spread) hipLaunchKernelGGL((paged_attn_join_kernel<D, true>), dim3(p.rows, p.heads), block, 0, s, p);
+    else hipLaunchKernelGGL((paged_attn_join_kernel<D, false>), dim3(p.rows, cdiv(p.heads, 256 / (D / 2))), block, 0, s, p);
     HIP_CHECK(hipGetLastError());
 }
 
@@ -808,7 +891,9 @@ void launch_paged_attention(const q3asr_kv_pages& c, int layer, const bf16_t* q,
     p.max_rows = b.max_rows; p.max_group_rows = b.max_group_rows; p.max_len = b.max_len;
     p.max_own = shares ? b.max_own : b.max_len;
     p.max_shared = b.max_shared;
-    p.scale_log2 = scale * 1.44269504088896340736f;
+    // not 0, so that a masked score stays minus infinity
+    p.scale_log2 = std::max(std::fabs(scale) * 1.44269504088896340736f, std::numeric_limits<float>::min());
+    p.flip = scale < 0.f ? 0x80008000u : 0u;
     p.shift_q = r.qt == 1 ? 4 : r.qt == 2 ? 5 : 6; p.tiles_q = r.tiles_q; p.per_min = r.per_min; p.slots_p = r.slots_p; p.slots = r.slots;
     char* ws = (char*)workspace;
     p.total = (Total*)ws;
