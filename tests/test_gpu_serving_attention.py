@@ -196,6 +196,25 @@ def test_extreme_scores(tiny_model):
             s.check(*s.run(b))
 
 
+@pytest.mark.parametrize("dim,heads,kv", [(128, 4, 2), (64, 14, 2)])
+@pytest.mark.parametrize("scale", [0.125, -0.5, 0.0])
+def test_scores_that_rise_along_the_keys(tiny_model, dim, heads, kv, scale):
+    """Running maxima that move at every key, by little and by much, or never after the first key; scales of either sign and zero.
+    Few sequences that are long enough for more parts than lanes take at once, and several rows per sequence."""
+    for seed, step in enumerate((0.3, 9.0)):
+        with Device() as dev:
+            s = Step(dev, tiny_model[0], [(2600, [(70, 1), (300, 3), (5, 1)])], heads, kv, dim, 16, seed=seed)
+            book = s.c.book
+            for i, q in enumerate(s.seqs):   # values along one dimension grow with the position, in their own pages and in shared ones
+                for pos in range(s.lens[i]):
+                    book.k[:, book.tables[q][pos // book.pg], :, pos % book.pg, 3] = bf16_bits(np.array([step * pos / 8]))[0]
+            dev.put(book.k, s.c.at["k"])
+            for sign in (1, -1):
+                s.q.reshape(len(s.q), heads, dim)[:, :, 3] = bf16_bits(np.array([float(sign)]))[0]
+                for grouped in (True, False):
+                    s.check(*s.run(s.batch(grouped), scale=scale), scale=scale)
+
+
 @pytest.mark.parametrize("dim,kv", [(128, 8), (64, 2)])
 def test_long_cache_past_32_bit_offsets(tiny_model, dim, kv):
     """A pool whose last pages lie behind 2^31 values."""
