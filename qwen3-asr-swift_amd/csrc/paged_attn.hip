@@ -106,10 +106,9 @@ struct Entry {             // a sequence of the step
     int seq, r0, T, len;
     bool ok;
 };
-__device__ __forceinline__ Entry entry_of(const AttnParams& p, int i, bool report) {
+__device__ __forceinline__ Entry entry_of(const AttnParams& p, int i, int seq, int a, int b, bool report) {
     Entry e;
-    e.seq = p.seqs[i];
-    const int a = p.cu_rows[i], b = p.cu_rows[i + 1];
+    e.seq = seq;
     const bool in = (unsigned)e.seq < (unsigned)p.max_seqs, ok = in && a >= 0 && b >= a && b <= p.rows && b - a <= p.max_rows;
     const bool none = e.seq == -1 && a == b;   // stands for no sequence: shares nothing, has no rows
     e.r0 = ok ? a : 0;
@@ -122,6 +121,9 @@ __device__ __forceinline__ Entry entry_of(const AttnParams& p, int i, bool repor
         e.len = min(max(e.len, 0), p.max_len);
     }
     return e;
+}
+__device__ __forceinline__ Entry entry_of(const AttnParams& p, int i, bool report) {
+    return entry_of(p, i, p.seqs[i], p.cu_rows[i], p.cu_rows[i + 1], report);
 }
 
 // ---- plan ----
@@ -143,11 +145,20 @@ __device__ __forceinline__ Total plan_segments(const AttnParams& p, const PlanMe
     int *const cu = mem.cu, *const cu_rows = mem.rows, *const scan = mem.scan;
     if (tell)
         for (int r = tid; r < p.rows; r += THREADS) p.parts[r].known = 0;
-    if (p.n_groups > 0)
-        for (int g = tid; g <= p.n_groups; g += THREADS) cu[g] = p.cu_groups[g];
-    for (int g = tid; g < p.n_groups; g += THREADS) from[g] = p.shared[g];
-    for (int i = tid; i <= p.n; i += THREADS) cu_rows[i] = p.cu_rows[i];
-    for (int i = tid; i < p.n; i += THREADS) entry[i] = entry_of(p, i, tell);
+    const int last_g = p.n_groups - 1, last = p.n - 1;
+    for (int i = tid; i <= p.n || i <= p.n_groups; i += THREADS) {   // n_groups may exceed n: empty groups
+        // all that does not depend on another load at once
+        const int seq = p.seqs[min(i, last)], a = p.cu_rows[min(i, last)], b = p.cu_rows[min(i, last) + 1];
+        const int group = last_g < 0 ? 0 : p.cu_groups[min(i, last_g + 1)], shared = last_g < 0 ? 0 : p.shared[min(i, last_g)];
+        __builtin_amdgcn_sched_barrier(0);
+        if (i <= last) {
+            entry[i] = entry_of(p, i, seq, a, b, tell);
+            cu_rows[i] = a;
+            if (i == last) cu_rows[i + 1] = b;
+        }
+        if (i <= last_g) from[i] = shared;
+        if (last_g >= 0 && i <= last_g + 1) cu[i] = group;
+    }
     __syncthreads();
     for (int g = tid; g < p.n_groups; g += THREADS) {
         const int i0 = cu[g], i1 = cu[g + 1], shared = from[g];
