@@ -573,7 +573,7 @@ void launch_gemm256(const I8Params& p, hipStream_t s) {
 // FROM: 0 bf16 rows, 1 fp32 rows, 2 rows that are rounded already.  HELD > 0: K is at least 8 and a thread's share of the rows, at
 // most HELD pieces of 8 values, is requested before the weights and held in registers, so that nothing waits behind the weights; 0:
 // any K, read twice.
-constexpr int FEW_THREADS = 512, FEW_WAVES = 8, FEW_ROWS = 6, FEW_LDS = 100 * 1024;
+constexpr int FEW_THREADS = 512, FEW_WAVES = 8, FEW_ROWS = 16, FEW_PLAIN = 6, FEW_LDS = 100 * 1024;
 constexpr int FEW_RED = FEW_WAVES * 256 * 4;
 __host__ __device__ inline int few_stride(int K) { return ((K + 63) & ~63) + 16; }   // rows 16 bytes apart modulo the banks
 
@@ -586,7 +586,7 @@ __global__ __launch_bounds__(FEW_THREADS, 2) void i8_few_rows_kernel(I8Params p,
     const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int k16 = (p.K + 15) & ~15, steps = (p.K + 63) >> 6, stride = few_stride(p.K);
-    const int per_row = stride >> 3, pieces = p.M * per_row;   // pieces of 8 values, those behind K zero
+    const int per_row = steps * 8, pieces = p.M * per_row;   // pieces of 8 values, those behind K zero
     int* const red = (int*)smem;                 // [wave][row][column]
     char* const xq = smem + FEW_RED;             // [M][stride]
 
@@ -767,14 +767,15 @@ void launch_few_steps(const I8Params& p, const I8Source& src, hipStream_t s) {
     else launch_few<FROM, 12, HELD>(p, src, s);
 }
 // Whether rounding the rows in every workgroup is cheaper than a launch of its own (us, one kernel against two): 1 x 2048 -> 4096:
-// 4.9, 7.3; 5 x 2048 -> 4096: 7.1, 7.3; 8 x 2048 -> 4096: 7.6, 7.3; 5 x 6144 -> 2048: 11.7, 13.2; rows of any alignment, read
-// twice: 2 x 2048 -> 2048: 6.8, 7.4; 4: 9.3, 7.4.
+// 4.9, 7.4; 5 x 2048 -> 4096: 6.0, 7.8; 8: 6.4, 7.9; 10 (more than 4 pieces per thread): 8.1, 7.7; 16 x 1024 -> 4096: 6.4, 7.8;
+// 5 x 6144 -> 2048: 11.3, 13.2; 6: 13.4, 14.4; 5 x 2047 -> 2048: 6.4, 7.9; 8 x 1003 -> 12288: 7.6, 8.0; 10: 8.6, 7.8.
 template <int FROM>
 bool launch_few_rows(const I8Params& p, const I8Source& src, hipStream_t s) {
-    const int64_t held = cdiv((int64_t)p.M * (few_stride(p.K) >> 3), FEW_THREADS);
-    if (p.M > FEW_ROWS || held > 8) return false;
+    const int64_t held = cdiv((int64_t)p.M * cdiv(p.K, 64) * 8, FEW_THREADS);
+    if (p.M > FEW_ROWS || held > (p.M <= 6 ? 8 : 4) || (p.M > 8 && p.N > 8192)) return false;
     if (p.K < 8) launch_few_steps<FROM, 0>(p, src, s);
     else if (held <= 2) launch_few_steps<FROM, 2>(p, src, s);
+    else if (held <= 4) launch_few_steps<FROM, 4>(p, src, s);
     else launch_few_steps<FROM, 8>(p, src, s);
     return true;
 }
@@ -821,7 +822,7 @@ bool launch_i8_linear_few_rows(const I8Params& p, const I8Source& src, hipStream
 }
 
 void launch_i8_matmul(const I8Params& p, hipStream_t s) {
-    if (p.M <= FEW_ROWS && p.M * (int64_t)few_stride(p.K) <= FEW_LDS) {
+    if (p.M <= FEW_PLAIN && p.M * (int64_t)few_stride(p.K) <= FEW_LDS) {
         launch_few_steps<2, 0>(p, {}, s);
         return;
     }

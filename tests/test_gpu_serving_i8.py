@@ -129,7 +129,8 @@ def test_linear_matches_whole_numbers(tiny_model, m, n, k, x, out, bias):
 
 
 @pytest.mark.parametrize("kind", ["bf16", "f32"])
-@pytest.mark.parametrize("m,ks", [(1, range(7, 26)), (3, range(513, 523)), (5, range(2094, 2103)), (6, (1363, 1364)), (40, range(130, 139))])
+@pytest.mark.parametrize("m,ks", [(1, range(7, 26)), (3, range(513, 523)), (5, range(2094, 2103)), (6, (1363, 1364, 4001)),
+                                  (8, (2041, 2048)), (13, (3, 7, 8)), (16, range(1009, 1026)), (40, range(130, 139))])
 def test_linear_of_any_length_and_alignment(tiny_model, m, ks, kind):
     """Every length against whole pieces of 8 values; activations and outputs begin one value behind an aligned address."""
     from q3asr import Int8Linear
