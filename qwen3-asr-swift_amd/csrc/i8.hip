@@ -130,6 +130,7 @@ __device__ __forceinline__ uint32_t wave_max_bits(uint32_t v) {
 
 // One wave per row, or (WHOLE) a workgroup's four waves where the rows are few; 8 values per lane and step.  Rows of up to
 // 512 * HELD values (2048 * HELD) stay in registers between the maximum and the rounding, longer ones are read twice.
+// HBM-bound: 8100 x 2048 bf16 15-19 us (2.6-3.3 TB/s read and written), 387 x 1003 fp32 3.0 us.
 template <bool F32, int HELD, bool WHOLE>
 __global__ __launch_bounds__(256) void i8_quantize_kernel(const void* x, int64_t ldx, int rows, int cols, int8_t* q, int64_t ldq, float* scales) {
     constexpr int STEP = WHOLE ? 256 : 64;
@@ -360,7 +361,7 @@ __global__ __launch_bounds__(256, 2) void i8_gemm_kernel(I8Params p) {
 // each {LDS -> registers, one staging unit's loads, barrier, 16 MFMAs, barrier}, waves 4-7 one barrier behind waves 0-3) carries
 // over byte for byte: a K tile is 128 bytes of a row, which are 64 bf16 or 128 int8 values, and a 16-byte fragment feeds one
 // 16x16x32 bf16 or one 16x16x64 int8 MFMA of the same length.  Twice the work per byte moved, so the phases are the same and
-// the rate doubles.
+// the rate doubles: 8100 x 2048 -> 12288 takes 186-211 us (1.9-2.2 POP/s), the library's 8-bit product of that size 223.
 constexpr int UNIT = 128 * 128, BUF = 4 * UNIT;   // A0 | A1 | W0 | W1, two K tiles
 constexpr int SCALES = 3 * 256 * 4;
 constexpr int LDS256 = 2 * BUF + 2 * SCALES;   // scales of the tile's rows, columns, and the bias, for two tiles
@@ -570,6 +571,7 @@ void launch_gemm256(const I8Params& p, hipStream_t s) {
 // wave's share of up to NS steps is requested at once.  The activation rows are rounded to 8 bits by every workgroup for itself,
 // underneath those loads: they are a few KB from the L2, and a second kernel in front would cost more than the whole product.
 // Weight rows are the MFMA "A" operand (lane: row li, bytes 16 lg ..), the activation rows in LDS the "B".
+// 1 x 2048 -> 4096: 4.5 us, of which a launch alone takes 2; 5 x 6144 -> 2048: 10.5, of which 4 are the rounding of 5 rows.
 // FROM: 0 bf16 rows, 1 fp32 rows, 2 rows that are rounded already.  HELD > 0: K is at least 8 and a thread's share of the rows, at
 // most HELD pieces of 8 values, is requested before the weights and held in registers, so that nothing waits behind the weights; 0:
 // any K, read twice.

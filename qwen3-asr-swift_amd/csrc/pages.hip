@@ -3,7 +3,7 @@
 // The tables, lengths and reference counts live on the device and change in stream order, so a decode loop never waits for the
 // host.  fork, reserve and compact are a plan -- one workgroup checks every entry, ranks what it needs with prefix sums and
 // changes the tables, all or nothing -- followed, where page contents move, by a grid of copies that reads its list from the
-// workspace.  All results are fixed by the order of the list: atomics only add to whole numbers or take a minimum of them.
+// workspace.  A plan is latency, phases of one workgroup: 2.5 us (fork of 5) to 11 (reserve for 200 sequences).  All results are fixed by the order of the list: atomics only add to whole numbers or take a minimum of them.
 #include "paged.h"
 #include "prof.h"
 #include <algorithm>
@@ -406,7 +406,8 @@ __global__ __launch_bounds__(PLAN) void pages_compact_kernel(Pages p) {
 }
 
 // ---- copies of page contents: one wave per (K or V, page, layer, head), a run of filled tokens that is contiguous on both sides ----
-// Bound by HBM, as a large copy is.  RENUMBER: page numbers of the table change on the way (compact).
+// Bound by HBM, as a large copy is: 657 MB moved in 264 us (5.0 TB/s read and written), 40 prompts' last pages to 5 heirs each 54 us.
+// RENUMBER: page numbers of the table change on the way (compact).
 constexpr int COPY_THREADS = 512;
 template <bool RENUMBER>
 __global__ __launch_bounds__(COPY_THREADS) void pages_copy_kernel(Pages p) {
