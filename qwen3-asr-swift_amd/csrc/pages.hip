@@ -3,7 +3,8 @@
 // The tables, lengths and reference counts live on the device and change in stream order, so a decode loop never waits for the
 // host.  fork, reserve and compact are a plan -- one workgroup checks every entry, ranks what it needs with prefix sums and
 // changes the tables, all or nothing -- followed, where page contents move, by a grid of copies that reads its list from the
-// workspace.  A plan is latency, phases of one workgroup: 2.5 us (fork of 5) to 11 (reserve for 200 sequences).  All results are fixed by the order of the list: atomics only add to whole numbers or take a minimum of them.
+// workspace.  A plan is latency, phases of one workgroup: 2.5 us (fork of 5) to 11 (reserve for 200 sequences).  All results are
+// fixed by the order of the list: atomics only add to whole numbers or take a minimum of them.
 #include "paged.h"
 #include "prof.h"
 #include <algorithm>
