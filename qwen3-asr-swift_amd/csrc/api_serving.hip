@@ -40,6 +40,9 @@ bool aligned(const void* p, size_t a) { return (uintptr_t)p % a == 0; }
 
 // Strides are counted in values; a buffer has to be addressable with 64 bits and a row's end must not wrap.
 constexpr int64_t MAX_LD = (int64_t)1 << 40;
+// Rows (and output channels) of one call: a workgroup each stays within what a launch may hold, rounding up to tiles within 32 bits.
+constexpr int MAX_ROWS = 1 << 24;
+constexpr int MAX_LD_I8 = 1 << 22;
 
 void check_rows(const char* what, const void* p, int dtype, int64_t ld, int cols) {
     const std::string w(what);
@@ -51,7 +54,7 @@ void check_i8(const char* what, const int8_t* p, int64_t ld, int cols) {
     const std::string w(what);
     Q3_REQUIRE(aligned(p, 16) && ld % 16 == 0, w + ": 8-bit rows must be aligned to 16 bytes");
     // a tile's rows are addressed by 32-bit byte offsets from its first one
-    Q3_REQUIRE(ld >= ((cols + 15) & ~15) && ld <= (1 << 22), w + ": row stride must lie between a row rounded up to 16 and 4194304");
+    Q3_REQUIRE(ld >= ((cols + 15) & ~15) && ld <= MAX_LD_I8, w + ": row stride must lie between a row rounded up to 16 and 4194304");
 }
 int64_t round256(int64_t n) { return (n + 255) & ~255ll; }
 int64_t quantized_bytes(int M, int K) { return round256((int64_t)M * ((K + 15) & ~15)) + round256((int64_t)M * 4); }
@@ -76,6 +79,7 @@ void check_batch(const q3asr_kv_pages* c, const q3asr_attn_batch* b) {
     if (b->n == 0 || b->rows == 0) return;
     Q3_REQUIRE(b->seqs && b->cu_rows, "pages: null argument in the batch");
     Q3_REQUIRE(b->n <= c->max_seqs, "pages: more entries than sequences");
+    Q3_REQUIRE(b->rows <= MAX_ROWS, "pages: more than 2^24 rows");
 }
 
 // After a call on the model's own stream: errors that the device found become this call's.
@@ -106,6 +110,7 @@ int q3asr_i8_quantize(q3asr_model* m, const void* x, int dtype, int64_t ldx, int
     Q3_API_BEGIN
     Q3_REQUIRE(m && x && q && scales, "i8_quantize: null argument");
     Q3_REQUIRE(rows > 0 && cols > 0, "i8_quantize: empty problem");
+    Q3_REQUIRE(rows <= MAX_ROWS && cols <= MAX_LD_I8, "i8_quantize: more than 2^24 rows or 4194304 columns");
     check_rows("i8_quantize: x", x, dtype, ldx, cols);
     Q3_REQUIRE(aligned(q, 16) && ldq % 16 == 0 && ldq >= (((int64_t)cols + 15) & ~15ll) && ldq < MAX_LD,
                "i8_quantize: rows of q must be aligned to 16 bytes and hold cols rounded up to 16");
@@ -120,6 +125,7 @@ static void check_product(const int8_t* w, int64_t ldw, const float* w_scales, i
     Q3_REQUIRE(M > 0 && N > 0 && K > 0, "i8: empty problem");
     Q3_REQUIRE(K <= I8_MAX_K, "i8: K above 131056 could overflow the 32-bit sums");
     Q3_REQUIRE((int64_t)cdiv(M, 64) * cdiv(N, 64) < (1ll << 31), "i8: too many output tiles");
+    Q3_REQUIRE(M <= MAX_ROWS && N <= MAX_ROWS, "i8: more than 2^24 rows or output channels");
     check_i8("i8: w", w, ldw, K);
     check_rows("i8: out", out, out_dtype, ldo, N);
 }
@@ -281,6 +287,10 @@ static void check_attention(const q3asr_kv_pages* c, const q3asr_attn_batch* b, 
         Q3_REQUIRE(b->max_shared >= 0 && b->max_shared <= b->max_len && b->max_own >= 0 && b->max_own <= b->max_len,
                    "paged_attention: max_shared and max_own must lie between 0 and max_len");
     }
+    // tiles of 32 keys by 16 rows, and one for every beginning, are counted in 32 bits: at most one incomplete tile of rows per sequence
+    // and group and KV head, twice for shared and own keys
+    const int64_t tiles = ((int64_t)b->max_len + 63) / 32, streams = (int64_t)b->rows * heads / 16 + (int64_t)b->n * c->kv_heads;
+    Q3_REQUIRE(2 * streams < (1ll << 31) / tiles, "paged_attention: too many rows for so many tokens in one call");
 }
 
 int64_t q3asr_paged_attention_workspace(q3asr_model* m, const q3asr_kv_pages* c, const q3asr_attn_batch* b, int heads) {
