@@ -198,12 +198,13 @@ __global__ __launch_bounds__(256) void pages_fork_write_kernel(Pages p, const in
 }
 
 // ---- reserve ----
-constexpr int HELD_STARTS = 2048, HELD_FREE = 4096;
+constexpr int HELD_STARTS = 2048, HELD_FREE = 4096, HELD_NEED = 512;
 
 __global__ __launch_bounds__(PLAN) void pages_reserve_kernel(Pages p, const int* seqs, const int* tokens, int n) {
     __shared__ int worst, wave_free[PLAN / 64];
     __shared__ Sums scan[PLAN / 64];
     __shared__ int held_start[HELD_STARTS], held_free[HELD_FREE];
+    __shared__ Need held_need[HELD_NEED];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, width = p.max_seq_pages, pt = p.page_tokens;
     const Layout l = layout(p.pages, p.max_seqs, width);
     int *mark = p.ws + l.rows, *copies = p.ws + l.copies;
@@ -221,6 +222,7 @@ __global__ __launch_bounds__(PLAN) void pages_reserve_kernel(Pages p, const int*
     __syncthreads();
     // what every entry needs; a thread keeps its first one in registers
     Need own{};
+    int own_refs = 0;
     for (int i = tid; i < n; i += PLAN) {
         Need r{};
         r.seq = seqs[i];
@@ -240,6 +242,7 @@ __global__ __launch_bounds__(PLAN) void pages_reserve_kernel(Pages p, const int*
                     r.page = p.table[(int64_t)r.seq * width + r.old_pages - 1];
                     if ((unsigned)r.page >= (unsigned)p.pages) code = Q3ASR_PAGES_BAD_INDEX;
                     else {
+                        if (i == tid) own_refs = p.refs[r.page];
                         here[r.page] = 0;
                         first[r.page] = INT_MAX;
                     }
@@ -281,7 +284,7 @@ __global__ __launch_bounds__(PLAN) void pages_reserve_kernel(Pages p, const int*
         if (i < n) {
             r = entry(i);
             if (r.fill) {
-                const int refs = p.refs[r.page];
+                const int refs = i == tid ? own_refs : p.refs[r.page];
                 copy = refs > 1 && !(counted(&here[r.page]) == refs && counted(&first[r.page]) == i);
             }
         }
@@ -291,7 +294,8 @@ __global__ __launch_bounds__(PLAN) void pages_reserve_kernel(Pages p, const int*
             r.start = (int)min(carry + before.wanted, (long long)INT_MAX);   // a call that wants so many pages is refused below
             r.copy = copy ? 1 + copied + before.copies : 0;
             if (i == tid) own = r;
-            need[i] = r;
+            if (n <= HELD_NEED) held_need[i] = r;
+            else need[i] = r;
             if (i < HELD_STARTS) held_start[i] = r.start;
         }
         carry += total.wanted;
@@ -326,7 +330,7 @@ __global__ __launch_bounds__(PLAN) void pages_reserve_kernel(Pages p, const int*
             if ((in_lds ? held_start[mid] : need[mid].start) <= k) lo = mid;
             else hi = mid;
         }
-        const Need r = need[lo];
+        const Need r = n <= HELD_NEED ? held_need[lo] : need[lo];
         const int to = free[k], j = k - r.start;
         p.refs[to] = 1;
         if (r.copy && j == 0) {
