@@ -39,8 +39,8 @@ struct Layout {
 };
 __host__ __device__ inline Layout layout(int pages, int max_seqs, int max_seq_pages) {
     Layout l;
-    l.rows = 16;                                              // fork: the new table rows; reserve: marks of the named sequences
-    l.row_lens = l.rows + (int64_t)max_seqs * max_seq_pages;  // fork: their lengths and marks
+    l.rows = 16;                                              // fork: the new table rows
+    l.row_lens = l.rows + (int64_t)max_seqs * max_seq_pages;  // fork: their lengths; behind them fork's and reserve's claims
     l.need = (l.row_lens + 2 * (int64_t)max_seqs + 3) & ~3ll;
     l.copies = l.need + 8 * (int64_t)max_seqs;                // (from, to, tokens) of every copy
     l.free = l.copies + 3 * (int64_t)(max_seqs > pages ? max_seqs : pages);
@@ -100,38 +100,54 @@ __global__ __launch_bounds__(256) void pages_reset_kernel(Pages p) {
 
 __global__ void pages_clear_status_kernel(int* status) { if (threadIdx.x < 4) status[threadIdx.x] = 0; }
 
+// Which entry of a list names a sequence first: in LDS where the cache has few sequences, else in `far`, a word per sequence.
+constexpr int HELD_SEQS = 4096;
+struct Claims {
+    int* near;
+    int* far;     // NULL: near
+    __device__ void open(int seq) const { if (far) far[seq] = INT_MAX; else near[seq] = INT_MAX; }
+    __device__ void claim(int seq, int entry) const { if (far) atomicMin(&far[seq], entry); else atomicMin(&near[seq], entry); }
+    __device__ int first(int seq) const { return far ? counted(&far[seq]) : near[seq]; }
+};
+
 // ---- fork ----
-// One workgroup checks the list; short ones (up to FORK_HELD table entries) it carries out as well, with the rows to come in
-// registers between reading all old rows and writing the new ones.  Longer ones go on in two kernels over the whole device, with the
-// rows in the workspace.
+// Short lists (up to FORK_HELD table entries) are checked and carried out by one workgroup, with the rows to come in registers between
+// reading all old rows and writing the new ones.  Longer ones take two kernels over the whole device, with the rows in the
+// workspace: every workgroup of the first one checks the list for itself, the second one learns the outcome from the workspace.
 constexpr int FORK_ROUNDS = 2, FORK_HELD = FORK_ROUNDS * PLAN;
 
-__global__ __launch_bounds__(PLAN) void pages_fork_kernel(Pages p, const int* dst, const int* src, int n, int held) {
-    __shared__ int worst;
+// The lowest wrong entry as entry * 8 + code, INT_MAX if there is none.  All threads of the workgroup; ends behind a barrier.
+__device__ __forceinline__ int fork_check(const Pages& p, const int* dst, const int* src, int n, const Claims& claims, int* worst) {
+    const int tid = threadIdx.x, threads = blockDim.x;
+    if (tid == 0) *worst = INT_MAX;
+    const int own = tid < n ? dst[tid] : -1, own_src = tid < n && src ? src[tid] : -1;
+    auto named = [&](int i) { return i == tid ? own : dst[i]; };
+    for (int i = tid; i < n; i += threads) {
+        const int d = named(i);
+        if ((unsigned)d < (unsigned)p.max_seqs) claims.open(d);
+    }
+    __syncthreads();
+    for (int i = tid; i < n; i += threads) {
+        const int d = named(i), s = i == tid ? own_src : src ? src[i] : -1;
+        if (d < -1 || d >= p.max_seqs || s < -1 || s >= p.max_seqs) note(worst, i, Q3ASR_PAGES_BAD_INDEX);
+        else if (d >= 0) claims.claim(d, i);   // -1: no entry
+    }
+    __syncthreads();
+    for (int i = tid; i < n; i += threads) {
+        const int d = named(i);
+        if ((unsigned)d < (unsigned)p.max_seqs && claims.first(d) < i) note(worst, i, Q3ASR_PAGES_DUPLICATE);
+    }
+    __syncthreads();
+    return *worst;
+}
+
+__global__ __launch_bounds__(PLAN) void pages_fork_kernel(Pages p, const int* dst, const int* src, int n) {
+    __shared__ int worst, claimed[HELD_SEQS];
     const int tid = threadIdx.x, width = p.max_seq_pages;
-    int* const mark = p.ws + layout(p.pages, p.max_seqs, width).row_lens + p.max_seqs;
-    if (tid == 0) worst = INT_MAX;
-    __syncthreads();
-    for (int i = tid; i < n; i += PLAN) {
-        const int d = dst[i], s = src ? src[i] : -1;
-        if (d < -1 || d >= p.max_seqs || s < -1 || s >= p.max_seqs) note(&worst, i, Q3ASR_PAGES_BAD_INDEX);
-        else if (d >= 0) mark[d] = i;   // -1: no entry
-    }
-    __syncthreads();
-    for (int i = tid; i < n; i += PLAN) {
-        const int d = dst[i];
-        if ((unsigned)d < (unsigned)p.max_seqs && mark[d] != i) note(&worst, i, Q3ASR_PAGES_DUPLICATE);
-    }
-    __syncthreads();
-    if (worst != INT_MAX) {   // the same for the whole workgroup
-        if (tid == 0) {
-            pages_error(p.status, worst & 7, worst >> 3);
-            p.ws[1] = 0;
-        }
-        return;
-    }
-    if (!held) {
-        if (tid == 0) p.ws[1] = 1;
+    const Claims claims{claimed, p.max_seqs <= HELD_SEQS ? nullptr : p.ws + layout(p.pages, p.max_seqs, width).row_lens + p.max_seqs};
+    const int wrong = fork_check(p, dst, src, n, claims, &worst);
+    if (wrong != INT_MAX) {   // the same for the whole workgroup
+        if (tid == 0) pages_error(p.status, wrong & 7, wrong >> 3);
         return;
     }
     const int total = n * width;
@@ -163,8 +179,30 @@ __global__ __launch_bounds__(PLAN) void pages_fork_kernel(Pages p, const int* ds
     if (tid < n && dst[tid] >= 0) p.lens[dst[tid]] = lens;
 }
 
+// A cache of more than HELD_SEQS sequences has its claims in the workspace, where there is one word per sequence: one workgroup checks the
+// list in a launch of its own.
+__global__ __launch_bounds__(PLAN) void pages_fork_check_kernel(Pages p, const int* dst, const int* src, int n) {
+    __shared__ int worst;
+    const Claims claims{nullptr, p.ws + layout(p.pages, p.max_seqs, p.max_seq_pages).row_lens + p.max_seqs};
+    const int wrong = fork_check(p, dst, src, n, claims, &worst);
+    if (threadIdx.x == 0) {
+        if (wrong != INT_MAX) pages_error(p.status, wrong & 7, wrong >> 3);
+        p.ws[1] = wrong == INT_MAX;
+    }
+}
+template <bool CHECK>
 __global__ __launch_bounds__(256) void pages_fork_read_kernel(Pages p, const int* dst, const int* src, int n) {
-    if (p.ws[1] == 0) return;
+    if constexpr (CHECK) {
+        __shared__ int worst, claimed[HELD_SEQS];
+        const int wrong = fork_check(p, dst, src, n, Claims{claimed, nullptr}, &worst);
+        if (blockIdx.x == 0 && threadIdx.x == 0) {
+            if (wrong != INT_MAX) pages_error(p.status, wrong & 7, wrong >> 3);
+            p.ws[1] = wrong == INT_MAX;   // for the next kernel
+        }
+        if (wrong != INT_MAX) return;
+    } else {
+        if (p.ws[1] == 0) return;
+    }
     const int width = p.max_seq_pages;
     const Layout l = layout(p.pages, p.max_seqs, width);
     int *rows = p.ws + l.rows, *row_lens = p.ws + l.row_lens;
@@ -207,7 +245,9 @@ __global__ __launch_bounds__(PLAN) void pages_reserve_kernel(Pages p, const int*
     __shared__ Need held_need[HELD_NEED];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, width = p.max_seq_pages, pt = p.page_tokens;
     const Layout l = layout(p.pages, p.max_seqs, width);
-    int *mark = p.ws + l.rows, *copies = p.ws + l.copies;
+    int* copies = p.ws + l.copies;
+    __shared__ int claimed[HELD_SEQS];
+    const Claims claims{claimed, p.max_seqs <= HELD_SEQS ? nullptr : p.ws + l.row_lens + p.max_seqs};
     int *here = p.ws + l.per_page, *first = here + p.pages;
     Need* const need = (Need*)(p.ws + l.need);
     // free pages, counted by every wave over a contiguous span of the pool
@@ -231,7 +271,7 @@ __global__ __launch_bounds__(PLAN) void pages_reserve_kernel(Pages p, const int*
         if (r.seq < -1 || r.seq >= p.max_seqs || r.tokens < 0) code = Q3ASR_PAGES_BAD_INDEX;
         else if (r.seq == -1) r.tokens = 0;   // no entry
         else {
-            mark[r.seq] = i;
+            claims.open(r.seq);
             const int len = p.lens[r.seq];
             if (len < 0 || (int64_t)len + r.tokens > (int64_t)width * pt) code = Q3ASR_PAGES_TOO_LONG;
             else {
@@ -256,8 +296,13 @@ __global__ __launch_bounds__(PLAN) void pages_reserve_kernel(Pages p, const int*
     __syncthreads();
     auto entry = [&](int i) { return i == tid ? own : need[i]; };
     for (int i = tid; i < n; i += PLAN) {
-        const int s = seqs[i];
-        if ((unsigned)s < (unsigned)p.max_seqs && mark[s] != i) note(&worst, i, Q3ASR_PAGES_DUPLICATE);
+        const int s = entry(i).seq;
+        if ((unsigned)s < (unsigned)p.max_seqs) claims.claim(s, i);
+    }
+    __syncthreads();
+    for (int i = tid; i < n; i += PLAN) {
+        const int s = entry(i).seq;
+        if ((unsigned)s < (unsigned)p.max_seqs && claims.first(s) < i) note(&worst, i, Q3ASR_PAGES_DUPLICATE);
     }
     __syncthreads();
     if (worst != INT_MAX) {
@@ -547,12 +592,21 @@ void launch_pages_fork(const q3asr_kv_pages& c, const int* dst, const int* src, 
     ProfScope ps("pages_fork_kernel", 12.0 * n * c.max_seq_pages, s);
     // the register form also needs an entry per thread and table offsets of 31 bits
     const bool held = (int64_t)n * c.max_seq_pages <= FORK_HELD && n <= PLAN && (int64_t)c.max_seqs * c.max_seq_pages < (1ll << 31);
-    hipLaunchKernelGGL(pages_fork_kernel, dim3(1), dim3(PLAN), 0, s, p, dst, src, n, (int)held);
-    HIP_CHECK(hipGetLastError());
-    if (held) return;
+    if (held) {
+        hipLaunchKernelGGL(pages_fork_kernel, dim3(1), dim3(PLAN), 0, s, p, dst, src, n);
+        HIP_CHECK(hipGetLastError());
+        return;
+    }
     const dim3 grid(std::min(cdiv(n, 4), 4 * device_cus()));
-    hipLaunchKernelGGL(pages_fork_read_kernel, grid, dim3(256), 0, s, p, dst, src, n);
-    HIP_CHECK(hipGetLastError());
+    if (c.max_seqs <= HELD_SEQS) {
+        hipLaunchKernelGGL(pages_fork_read_kernel<true>, grid, dim3(256), 0, s, p, dst, src, n);
+        HIP_CHECK(hipGetLastError());
+    } else {
+        hipLaunchKernelGGL(pages_fork_check_kernel, dim3(1), dim3(PLAN), 0, s, p, dst, src, n);
+        HIP_CHECK(hipGetLastError());
+        hipLaunchKernelGGL(pages_fork_read_kernel<false>, grid, dim3(256), 0, s, p, dst, src, n);
+        HIP_CHECK(hipGetLastError());
+    }
     hipLaunchKernelGGL(pages_fork_write_kernel, grid, dim3(256), 0, s, p, dst, n);
     HIP_CHECK(hipGetLastError());
 }

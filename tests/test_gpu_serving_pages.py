@@ -63,7 +63,7 @@ def test_beam_reordering_reads_the_table_before_it_writes(tiny_model):
         c.check()
 
 
-@pytest.mark.parametrize("n,width", [(3, 2), (1500, 3), (40, 700)])
+@pytest.mark.parametrize("n,width", [(3, 2), (1500, 3), (40, 700), (2100, 2)])
 def test_lists_of_any_length(tiny_model, n, width):
     """More entries than threads; longer tables than threads; many pages."""
     rng = np.random.default_rng(n)
@@ -140,6 +140,27 @@ def test_refused_calls_change_nothing(tiny_model):
         with pytest.raises(Q3Error, match="more entries than sequences"):
             c.c.fork(c.ints(range(7)), c.ints(range(7)), 7)
         c.c.fork(0, 0, 0)                    # nothing to do
+        c.check()
+
+
+@pytest.mark.parametrize("seqs,width", [(600, 1), (600, 9), (4096, 2), (5000, 1), (5000, 3)])
+def test_the_first_repeated_entry_is_named(tiny_model, seqs, width):
+    """Few and many sequences, short and long tables: the entry that is reported is the first one that names a sequence again."""
+    rng = np.random.default_rng(seqs + width)
+    with Device() as dev:
+        c = _filled(dev, tiny_model[0], [3, 16, 9], seqs=seqs, width=width, pages=30)
+        for n, later in ((600, (599,)), (600, (3, 400)), (40, (17, 18, 39)), (seqs, (seqs - 1, seqs // 2))):
+            names = rng.permutation(seqs)[:n]
+            for at in later:
+                names[at] = names[rng.integers(0, min(later))]
+            first = min(later)
+            zeros = c.ints(np.zeros(n))
+            for call in (lambda: c.c.fork(c.ints(names), zeros, n), lambda: c.c.free(c.ints(names), n), lambda: c.c.reserve(c.ints(names), zeros, n)):
+                with pytest.raises(Q3Error, match=f"named twice .entry {first}."):
+                    call()
+        c.check()
+        order = rng.permutation(seqs).tolist()          # the whole cache in one call
+        c.fork(order, [2 if q == 2 else -1 if q % 2 else 0 for q in order])
         c.check()
 
 
