@@ -101,6 +101,44 @@ __device__ __forceinline__ void i8_load8(const void* row, int k, int cols, float
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = k + e < cols ? i8_load<F32>(row, k + e) : 0.f;
 }
+// 8 values of a row of at least 8, requested unconditionally: a load behind a branch is waited for at once.  What reaches behind the
+// row's end is read from its last 8 values; then those that precede it move out.
+template <bool F32>
+struct I8Piece {
+    static constexpr int WORDS = F32 ? 8 : 4;
+    uint32_t w[WORDS];
+    __device__ __forceinline__ void request(const void* row, int k, int cols) {
+        const char* at = (const char*)row + (int64_t)min(k, cols - 8) * (F32 ? 4 : 2);
+#pragma unroll
+        for (int j = 0; j < WORDS; j += 4) {
+            const uint4 u = i8_load16(at + 4 * j);
+            w[j] = u.x;
+            w[j + 1] = u.y;
+            w[j + 2] = u.z;
+            w[j + 3] = u.w;
+        }
+    }
+    // Behind the request: values from cols on become zero.
+    __device__ __forceinline__ void settle(int k, int cols) {
+        if (cols & 7) {   // wave-uniform
+            const int by = k < cols ? max(k + 8 - cols, 0) : 0, words = F32 ? by : by >> 1;
+#pragma unroll
+            for (int step = WORDS / 2; step; step >>= 1)
+#pragma unroll
+                for (int e = 0; e < WORDS; ++e) w[e] = words & step ? (e + step < WORDS ? w[e + step] : 0u) : w[e];
+            if (!F32 && (by & 1)) {
+#pragma unroll
+                for (int e = 0; e < WORDS; ++e) w[e] = __builtin_amdgcn_alignbit(e + 1 < WORDS ? w[e + 1] : 0u, w[e], 16);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < WORDS; ++e) w[e] = k < cols ? w[e] : 0u;
+    }
+    __device__ __forceinline__ void values(float* v) const {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(F32 ? w[e % WORDS] : (e & 1) ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+    }
+};
 // Magnitudes are compared as the bits of non-negative floats, an order in which a NaN lies above infinity.
 __device__ __forceinline__ uint32_t i8_max8(uint32_t m, const float* v) {
 #pragma unroll
@@ -112,6 +150,16 @@ __device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
     typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
     const u16x2 m = __builtin_elementwise_max(__builtin_bit_cast(u16x2, a & 0x7fff7fffu), __builtin_bit_cast(u16x2, b & 0x7fff7fffu));
     return (uint32_t)max(m.x, m.y) << 16;
+}
+template <bool F32>
+__device__ __forceinline__ uint32_t i8_top(const I8Piece<F32>& x) {
+    if constexpr (F32) {
+        float v[8];
+        x.values(v);
+        return i8_max8(0, v);
+    } else {
+        return max(max_bf16x2(x.w[0], x.w[1]), max_bf16x2(x.w[2], x.w[3]));
+    }
 }
 template <int CTRL>
 __device__ __forceinline__ uint32_t dpp_max_bits(uint32_t v) {
@@ -128,9 +176,10 @@ __device__ __forceinline__ uint32_t wave_max_bits(uint32_t v) {
     return max(max(a, b), max(c, d));
 }
 
-// One wave per row, or (WHOLE) a workgroup's four waves where the rows are few; 8 values per lane and step.  Rows of up to
-// 512 * HELD values (2048 * HELD) stay in registers between the maximum and the rounding, longer ones are read twice.
-// HBM-bound: 8100 x 2048 bf16 15-19 us (2.6-3.3 TB/s read and written), 387 x 1003 fp32 3.0 us.
+// A workgroup's four waves per row (WHOLE), or one wave where rows are many and short; 8 values per lane and step.  Rows of up to
+// 2048 * HELD values (512 * HELD) stay in registers between the maximum and the rounding, longer ones (HELD 0) are read twice.
+// HBM-bound: 8100 x 2048 bf16 13.5 us (3.7 TB/s read and written, a launch's 4 included), 8100 x 6144 29 (5.1), 387 x 1003 fp32 4.6.
+// A wave per row: 14.3, 36; 8100 x 1003: 9.4 against 10.7 for a workgroup.
 template <bool F32, int HELD, bool WHOLE>
 __global__ __launch_bounds__(256) void i8_quantize_kernel(const void* x, int64_t ldx, int rows, int cols, int8_t* q, int64_t ldq, float* scales) {
     constexpr int STEP = WHOLE ? 256 : 64;
@@ -151,30 +200,57 @@ __global__ __launch_bounds__(256) void i8_quantize_kernel(const void* x, int64_t
     int8_t* dst = q + (int64_t)row * ldq;
     const int k16 = (cols + 15) & ~15;
     uint32_t m = 0;
+    auto place = [&](int i) { return (i * STEP + lane) * 8; };
     if constexpr (HELD > 0) {
-        float v[HELD][8];
+        I8Piece<F32> x8[HELD];
 #pragma unroll
-        for (int i = 0; i < HELD; ++i) i8_load8<F32>(src, (i * STEP + lane) * 8, cols, v[i]);
+        for (int i = 0; i < HELD; ++i) x8[i].request(src, place(i), cols);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < HELD; ++i) m = i8_max8(m, v[i]);
+        for (int i = 0; i < HELD; ++i) {
+            x8[i].settle(place(i), cols);
+            m = max(m, i8_top(x8[i]));
+        }
         const RowScale rs(row_max(m));
         if (lane == 0) scales[row] = rs.scale;
 #pragma unroll
         for (int i = 0; i < HELD; ++i) {
-            const int k = (i * STEP + lane) * 8;
-            if (k < k16) *(uint2*)(dst + k) = rs.pack8(v[i]);
+            float v[8];
+            x8[i].values(v);
+            if (place(i) < k16) *(uint2*)(dst + place(i)) = rs.pack8(v);
         }
-    } else {
+    } else if (cols < 8) {
         float v[8];
-        for (int k = lane * 8; k < cols; k += 8 * STEP) {
-            i8_load8<F32>(src, k, cols, v);
-            m = i8_max8(m, v);
+        i8_load8<F32>(src, place(0), cols, v);
+        const RowScale rs(row_max(i8_max8(0, v)));
+        if (lane == 0) scales[row] = rs.scale;
+        if (place(0) < k16) *(uint2*)(dst + place(0)) = rs.pack8(v);
+    } else {
+        constexpr int AT_ONCE = 4;
+        I8Piece<F32> x8[AT_ONCE];
+        auto read = [&](int i0) {
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) x8[i].request(src, place(i0 + i), cols);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) x8[i].settle(place(i0 + i), cols);
+        };
+        const int pieces = (k16 + 8 * STEP - 1) / (8 * STEP);
+        for (int i0 = 0; i0 < pieces; i0 += AT_ONCE) {
+            read(i0);
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) m = max(m, i8_top(x8[i]));
         }
         const RowScale rs(row_max(m));
         if (lane == 0) scales[row] = rs.scale;
-        for (int k = lane * 8; k < k16; k += 8 * STEP) {
-            i8_load8<F32>(src, k, cols, v);
-            *(uint2*)(dst + k) = rs.pack8(v);
+        for (int i0 = 0; i0 < pieces; i0 += AT_ONCE) {
+            read(i0);
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) {
+                float v[8];
+                x8[i].values(v);
+                if (place(i0 + i) < k16) *(uint2*)(dst + place(i0 + i)) = rs.pack8(v);
+            }
         }
     }
 }
@@ -645,62 +721,23 @@ __global__ __launch_bounds__(FEW_THREADS, 2) void i8_few_rows_kernel(I8Params p,
     int n0 = blockIdx.x * 16;
     if (tid < FEW_ROWS) amax[tid] = 0;
     if constexpr (HELD > 0) {
-        constexpr int WORDS = F32 ? 2 : 1;
-        uint4 held[HELD][WORDS];
+        I8Piece<F32> held[HELD];
         int row_of[HELD], k_of[HELD];
 #pragma unroll
         for (int i = 0; i < HELD; ++i) {
             const int c = min(tid + FEW_THREADS * i, pieces - 1);
             row_of[i] = c / per_row;
             k_of[i] = (c - row_of[i] * per_row) * 8;
-            const char* at = (const char*)src.x + ((int64_t)row_of[i] * src.ldx + min(k_of[i], p.K - 8)) * (F32 ? 4 : 2);
-#pragma unroll
-            for (int j = 0; j < WORDS; ++j) held[i][j] = i8_load16(at + 16 * j);
+            held[i].request((const char*)src.x + (int64_t)row_of[i] * src.ldx * (F32 ? 4 : 2), k_of[i], p.K);
         }
         __builtin_amdgcn_sched_barrier(0);
         request(n0, 0);
         __builtin_amdgcn_sched_barrier(0);
         __syncthreads();
-        if (p.K & 7) {   // a row's last piece was read from its last 8 values: what precedes it moves out
-#pragma unroll
-            for (int i = 0; i < HELD; ++i) {
-                const int by = k_of[i] < p.K ? max(k_of[i] + 8 - p.K, 0) : 0;
-                uint32_t word[9] = {held[i][0].x, held[i][0].y, held[i][0].z, held[i][0].w, 0, 0, 0, 0, 0};
-                if constexpr (F32) { word[4] = held[i][1].x; word[5] = held[i][1].y; word[6] = held[i][1].z; word[7] = held[i][1].w; }
-                const int words = F32 ? by : by >> 1;
-#pragma unroll
-                for (int step = 4; step; step >>= 1)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) word[e] = words & step ? (e + step < 8 ? word[e + step] : 0u) : word[e];
-                if (!F32 && (by & 1)) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) word[e] = __builtin_amdgcn_alignbit(word[e + 1], word[e], 16);
-                }
-                held[i][0] = make_uint4(word[0], word[1], word[2], word[3]);
-                if constexpr (F32) held[i][1] = make_uint4(word[4], word[5], word[6], word[7]);
-            }
-        }
-        auto values = [&](int i, float* v) {
-            const uint32_t word[8] = {held[i][0].x, held[i][0].y, held[i][0].z, held[i][0].w,
-                                      held[i][WORDS - 1].x, held[i][WORDS - 1].y, held[i][WORDS - 1].z, held[i][WORDS - 1].w};
-            const bool in = k_of[i] < p.K;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const uint32_t bits = F32 ? word[e] : (e & 1) ? word[e >> 1] & 0xffff0000u : word[e >> 1] << 16;
-                v[e] = in ? __uint_as_float(bits) : 0.f;
-            }
-        };
 #pragma unroll
         for (int i = 0; i < HELD; ++i) {
-            uint32_t top = 0;
-            if constexpr (F32) {
-                float v[8];
-                values(i, v);
-                top = i8_max8(0, v);
-            } else {
-                top = max(max_bf16x2(held[i][0].x, held[i][0].y), max_bf16x2(held[i][0].z, held[i][0].w));
-                top = k_of[i] < p.K ? top : 0;
-            }
+            held[i].settle(k_of[i], p.K);
+            const uint32_t top = i8_top(held[i]);
             const int first = __builtin_amdgcn_readfirstlane(row_of[i]);
             if (first == __builtin_amdgcn_readlane(row_of[i], 63)) {   // the wave's pieces lie in one row
                 const uint32_t all = wave_max_bits(top);
@@ -716,7 +753,7 @@ __global__ __launch_bounds__(FEW_THREADS, 2) void i8_few_rows_kernel(I8Params p,
         for (int i = 0; i < HELD; ++i) {
             const RowScale rs = scales[row_of[i]];
             float v[8];
-            values(i, v);
+            held[i].values(v);
             if (tid + FEW_THREADS * i < pieces) *(uint2*)(xq + row_of[i] * stride + k_of[i]) = rs.pack8(v);
         }
     } else if constexpr (FROM == 2) {
@@ -837,21 +874,21 @@ void launch_tile(const I8Params& p, hipStream_t s) {
 
 void launch_i8_quantize(const I8Source& src, int rows, int cols, int8_t* q, int64_t ldq, float* scales, hipStream_t s) {
     ProfScope ps("i8_quantize_kernel", (double)rows * cols * (src.f32 ? 5 : 3), s);
-    const bool whole = rows <= 1024;
+    const bool whole = cols >= 8 && (rows <= 1024 || cols > 1024);
     const dim3 grid(whole ? rows : cdiv(rows, 4)), block(256);
 #define I8_QUANTIZE(F32, HELD, WHOLE) \
     hipLaunchKernelGGL((i8_quantize_kernel<F32, HELD, WHOLE>), grid, block, 0, s, src.x, src.ldx, rows, cols, q, ldq, scales)
 #define I8_QUANTIZE_TYPE(HELD, WHOLE) \
     if (src.f32) I8_QUANTIZE(true, HELD, WHOLE); \
     else I8_QUANTIZE(false, HELD, WHOLE)
-    if (whole) {
+    if (cols < 8) { I8_QUANTIZE_TYPE(0, false); }
+    else if (whole) {
         if (cols <= 2048) { I8_QUANTIZE_TYPE(1, true); }
         else if (cols <= 8192) { I8_QUANTIZE_TYPE(4, true); }
+        else if (cols <= 24576) { I8_QUANTIZE_TYPE(12, true); }
         else { I8_QUANTIZE_TYPE(0, true); }
     } else {
-        if (cols <= 2048) { I8_QUANTIZE_TYPE(4, false); }
-        else if (cols <= 6144) { I8_QUANTIZE_TYPE(12, false); }
-        else { I8_QUANTIZE_TYPE(0, false); }
+        I8_QUANTIZE_TYPE(2, false);
     }
 #undef I8_QUANTIZE_TYPE
 #undef I8_QUANTIZE
