@@ -187,7 +187,7 @@ int q3asr_op_attention(q3asr_model* m, const uint16_t* q, const uint16_t* k, con
  * Rows are rounded to whole numbers with one scale per row: scale = max |x| / 127 (fp32), q = x / scale rounded to the
  * nearest whole number, ties to even, decided without a rounding of the quotient.  A row of zeros has scale 0; a row that
  * holds an infinity or a NaN has scale NaN and q = 0, so whatever is computed from it is NaN.  Weights take one such scale
- * per output channel (quantise the [N][K] matrix by rows).  M, N and rows are at most 2^24. */
+ * per output channel (quantise the [N][K] matrix by rows).  M, N and rows are below 2^24. */
 
 /* x: [rows][cols] Q3ASR_F32 or Q3ASR_BF16, rows ldx values apart (any stride >= cols, any alignment of the type);
  * q: [rows][ldq] bytes, ldq a multiple of 16 and >= cols rounded up to 16, aligned to 16: columns from cols to the next
@@ -267,7 +267,7 @@ int q3asr_pages_compact(q3asr_model* m, const q3asr_kv_pages* c, void* stream);
  * padded batch) are left alone.  Optionally, consecutive sequences of the list form groups
  * (group g: entries cu_groups[g] .. cu_groups[g + 1)) whose first shared[g] tokens lie in the same pages; those are then read
  * once for the group.  shared[g] counts at most the tokens before the step's rows and is rounded down to whole pages.  The host
- * numbers bound what the arrays hold; smaller bounds make smaller grids.  rows is at most 2^24, and rows * heads / 16 times
+ * numbers bound what the arrays hold; smaller bounds make smaller grids.  rows is below 2^24, and rows * heads / 16 times
  * max_len / 32 stays below 2^30. */
 typedef struct q3asr_attn_batch {
     const int32_t* seqs;       /* [n] */

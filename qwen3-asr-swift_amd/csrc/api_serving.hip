@@ -41,7 +41,7 @@ bool aligned(const void* p, size_t a) { return (uintptr_t)p % a == 0; }
 // Strides are counted in values; a buffer has to be addressable with 64 bits and a row's end must not wrap.
 constexpr int64_t MAX_LD = (int64_t)1 << 40;
 // Rows (and output channels) of one call: a workgroup each stays within what a launch may hold, rounding up to tiles within 32 bits.
-constexpr int MAX_ROWS = 1 << 24;
+constexpr int MAX_ROWS = (1 << 24) - 1;
 constexpr int MAX_LD_I8 = 1 << 22;
 
 void check_rows(const char* what, const void* p, int dtype, int64_t ld, int cols) {
@@ -79,7 +79,7 @@ void check_batch(const q3asr_kv_pages* c, const q3asr_attn_batch* b) {
     if (b->n == 0 || b->rows == 0) return;
     Q3_REQUIRE(b->seqs && b->cu_rows, "pages: null argument in the batch");
     Q3_REQUIRE(b->n <= c->max_seqs, "pages: more entries than sequences");
-    Q3_REQUIRE(b->rows <= MAX_ROWS, "pages: more than 2^24 rows");
+    Q3_REQUIRE(b->rows <= MAX_ROWS, "pages: 2^24 rows or more");
 }
 
 // After a call on the model's own stream: errors that the device found become this call's.
@@ -110,7 +110,7 @@ int q3asr_i8_quantize(q3asr_model* m, const void* x, int dtype, int64_t ldx, int
     Q3_API_BEGIN
     Q3_REQUIRE(m && x && q && scales, "i8_quantize: null argument");
     Q3_REQUIRE(rows > 0 && cols > 0, "i8_quantize: empty problem");
-    Q3_REQUIRE(rows <= MAX_ROWS && cols <= MAX_LD_I8, "i8_quantize: more than 2^24 rows or 4194304 columns");
+    Q3_REQUIRE(rows <= MAX_ROWS && cols <= MAX_LD_I8, "i8_quantize: 2^24 rows or more, or more than 4194304 columns");
     check_rows("i8_quantize: x", x, dtype, ldx, cols);
     Q3_REQUIRE(aligned(q, 16) && ldq % 16 == 0 && ldq >= (((int64_t)cols + 15) & ~15ll) && ldq < MAX_LD,
                "i8_quantize: rows of q must be aligned to 16 bytes and hold cols rounded up to 16");
@@ -125,7 +125,7 @@ static void check_product(const int8_t* w, int64_t ldw, const float* w_scales, i
     Q3_REQUIRE(M > 0 && N > 0 && K > 0, "i8: empty problem");
     Q3_REQUIRE(K <= I8_MAX_K, "i8: K above 131056 could overflow the 32-bit sums");
     Q3_REQUIRE((int64_t)cdiv(M, 64) * cdiv(N, 64) < (1ll << 31), "i8: too many output tiles");
-    Q3_REQUIRE(M <= MAX_ROWS && N <= MAX_ROWS, "i8: more than 2^24 rows or output channels");
+    Q3_REQUIRE(M <= MAX_ROWS && N <= MAX_ROWS, "i8: 2^24 rows or output channels, or more");
     check_i8("i8: w", w, ldw, K);
     check_rows("i8: out", out, out_dtype, ldo, N);
 }

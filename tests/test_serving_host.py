@@ -48,8 +48,8 @@ def test_i8_refusals(lib, handle):
                      (dict(ws=None), "null"), (dict(M=0), "empty"), (dict(N=-1), "empty"), (dict(K=0), "empty"), (dict(K=131057, ldx=200000, ldw=131072), "131056"),
                      (dict(ldx=63), "stride"), (dict(ldw=48), "stride"), (dict(ldw=65), "aligned"), (dict(w=P + 8), "aligned"), (dict(ldo=7), "stride"),
                      (dict(dt=2), "type"), (dict(odt=7), "type"), (dict(x=P + 1), "aligned"), (dict(dt=0, x=P + 2), "aligned"), (dict(nb=100), "too small"),
-                     (dict(ws=P + 4), "workspace"), (dict(M=2 ** 31 - 1, N=2 ** 31 - 1, ldo=2 ** 31), "tiles"), (dict(M=2 ** 24 + 1), "2^24"),
-                     (dict(N=2 ** 24 + 1, ldo=2 ** 25), "2^24")):
+                     (dict(ws=P + 4), "workspace"), (dict(M=2 ** 31 - 1, N=2 ** 31 - 1, ldo=2 ** 31), "tiles"), (dict(M=2 ** 24), "2^24"),
+                     (dict(N=2 ** 24, ldo=2 ** 25), "2^24")):
         assert linear(**kw) != 0, kw
         assert text in _text(lib), (kw, _text(lib))
 
@@ -63,7 +63,7 @@ def test_i8_refusals(lib, handle):
         return lib.q3asr_i8_quantize(handle, x, dt, ldx, rows, cols, q, ldq, s, None)
 
     for kw, text in ((dict(x=None), "null"), (dict(q=None), "null"), (dict(s=None), "null"), (dict(rows=0), "empty"), (dict(ldx=19), "stride"),
-                     (dict(ldq=16), "aligned"), (dict(ldq=40), "aligned"), (dict(rows=2 ** 24 + 1), "2^24"), (dict(q=P + 4), "aligned"), (dict(dt=3), "type")):
+                     (dict(ldq=16), "aligned"), (dict(ldq=40), "aligned"), (dict(rows=2 ** 24), "2^24"), (dict(q=P + 4), "aligned"), (dict(dt=3), "type")):
         assert quantize(**kw) != 0 and text in _text(lib), (kw, _text(lib))
     assert lib.q3asr_i8_workspace(handle, 0, 8, 8) == -1 and lib.q3asr_i8_workspace(handle, 8, 8, 131057) == -1
     assert lib.q3asr_i8_workspace(handle, 5, 8, 33) >= 5 * 48 + 20
@@ -117,7 +117,7 @@ def test_attention_and_write_refusals(lib, handle):
                      (dict(batch=dict(max_shared=71)), "max_shared"), (dict(batch=dict(max_own=-1)), "max_own"), (dict(layer=2), "layer"), (dict(layer=-1), "layer"),
                      (dict(heads=3), "multiple"), (dict(q=None), "null"), (dict(out=None), "null"), (dict(ld=511), "aligned"), (dict(ld=504), "hold all heads"),
                      (dict(old=516), "aligned"), (dict(q=P + 8), "aligned"), (dict(scale=float("nan")), "finite"), (dict(scale=float("inf")), "finite"), (dict(scale=-2e30), "finite"),
-                     (dict(cache=dict(head_dim=32)), "head_dim"), (dict(batch=dict(rows=2 ** 24 + 1)), "2^24"),
+                     (dict(cache=dict(head_dim=32)), "head_dim"), (dict(batch=dict(rows=2 ** 24)), "2^24"),
                      (dict(cache=dict(max_seq_pages=(1 << 27) - 1), batch=dict(rows=100000, max_len=2 ** 31 - 16)), "too many rows"),
                      (dict(ws=None, **long), "workspace"), (dict(nb=16, **long), "workspace"), (dict(ws=P + 8, **long), "workspace")):
         assert attention(**kw) != 0, kw
