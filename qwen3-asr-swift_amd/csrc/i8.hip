@@ -476,7 +476,7 @@ __global__ __launch_bounds__(256, 2) void i8_gemm_kernel(I8Params p) {
 // each {LDS -> registers, one staging unit's loads, barrier, 16 MFMAs, barrier}, waves 4-7 one barrier behind waves 0-3) carries
 // over byte for byte: a K tile is 128 bytes of a row, which are 64 bf16 or 128 int8 values, and a 16-byte fragment feeds one
 // 16x16x32 bf16 or one 16x16x64 int8 MFMA of the same length.  Twice the work per byte moved, so the phases are the same and
-// the rate doubles: 8100 x 2048 -> 12288 takes 186-211 us (1.9-2.2 POP/s), the library's 8-bit product of that size 223.
+// the rate doubles: 8100 x 2048 -> 12288 takes 184-212 us (1.9-2.2 POP/s), the library's 8-bit product of that size 223.
 constexpr int UNIT = 128 * 128, BUF = 4 * UNIT;   // A0 | A1 | W0 | W1, two K tiles
 constexpr int SCALES = 3 * 256 * 4;
 constexpr int LDS256 = 2 * BUF + 2 * SCALES;   // scales of the tile's rows, columns, and the bias, for two tiles
