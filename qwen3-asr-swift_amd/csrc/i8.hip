@@ -23,8 +23,14 @@ namespace {
 // Rounding is bound by vector instructions, so eight values take a short way first: adding 1.5 * 2^23 in the multiply-add leaves
 // the rounded quotient in the low bits, from where bytes are picked.  It is right unless some remainder reaches half of scale
 // (about one value in 10^5 for arbitrary data), and then the long way is taken.
+// Rows of bf16 need no remainder.  With x = a 2^i and max |x| = b 2^j for whole a, b < 256, the ratio 127 x / max |x| is either half way
+// between two whole numbers or at least 1 / (254 * 255) > 2^-16 of itself away from there; the true quotient differs from it by 2^-24, the
+// computed one by 2^-22.  So only the ratios that are half way have to be decided, by the side that scale was rounded to: side is the
+// reciprocal, moved by one step where it lies on the other side of 127 / max |x| than 1 / scale does.  (Where 127 * scale is max |x|
+// itself, scale is a power of two and so is its reciprocal.)
 struct RowScale {
-    float scale, s, inv, lift;
+    float scale, s, inv, lift, side;
+    bool simple;
     __device__ RowScale() {}
     __device__ explicit RowScale(float amax) {
         scale = amax / 127.0f;
@@ -32,6 +38,10 @@ struct RowScale {
         lift = scale < 7.8886090522101181e-31f ? 18446744073709551616.0f : 1.0f;   // 2^-100, 2^64
         s = bad ? 0.f : scale * lift;
         inv = s > 0.f ? 1.0f / s : 0.f;
+        simple = !bad && (s == 0.f || lift == 1.0f);
+        const float up = fmaf(scale, 127.0f, -amax), over = fmaf(inv, amax, -127.0f);
+        side = up > 0.f && over >= 0.f ? __uint_as_float(__float_as_uint(inv) - 1) : up < 0.f && over <= 0.f ? __uint_as_float(__float_as_uint(inv) + 1) : inv;
+        if (s == 0.f) side = 0.f;
         if (bad) scale = __builtin_nanf("");
     }
     __device__ int whole(float x) const {
@@ -41,8 +51,22 @@ struct RowScale {
         if (e2 > s || (e2 == s && ((int)r & 1))) r += dir;
         return inv > 0.f ? (int)fminf(fmaxf(r, -127.0f), 127.0f) : 0;
     }
+    static __device__ uint2 low_bytes(const uint32_t* bits) {
+        uint2 b;
+        b.x = __builtin_amdgcn_perm(__builtin_amdgcn_perm(bits[3], bits[2], 0x0c0c0400), __builtin_amdgcn_perm(bits[1], bits[0], 0x0c0c0400), 0x05040100);
+        b.y = __builtin_amdgcn_perm(__builtin_amdgcn_perm(bits[7], bits[6], 0x0c0c0400), __builtin_amdgcn_perm(bits[5], bits[4], 0x0c0c0400), 0x05040100);
+        return b;
+    }
+    template <bool F32>
     __device__ uint2 pack8(const float* v) const {
         uint32_t bits[8];
+        if constexpr (!F32) {
+            if (simple) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) bits[e] = __float_as_uint(fmaf(v[e], side, 12582912.0f));
+                return low_bytes(bits);
+            }
+        }
         float far = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -51,10 +75,7 @@ struct RowScale {
             far = fmaxf(far, fabsf(fmaf(12582912.0f - t, s, v[e])));
         }
         if (2.0f * far < s && lift == 1.0f) {   // false for rows of zeros and rows that are not finite as well
-            uint2 b;
-            b.x = __builtin_amdgcn_perm(__builtin_amdgcn_perm(bits[3], bits[2], 0x0c0c0400), __builtin_amdgcn_perm(bits[1], bits[0], 0x0c0c0400), 0x05040100);
-            b.y = __builtin_amdgcn_perm(__builtin_amdgcn_perm(bits[7], bits[6], 0x0c0c0400), __builtin_amdgcn_perm(bits[5], bits[4], 0x0c0c0400), 0x05040100);
-            return b;
+            return low_bytes(bits);
         }
         uint32_t b[2] = {0, 0};
 #pragma unroll
@@ -178,8 +199,8 @@ __device__ __forceinline__ uint32_t wave_max_bits(uint32_t v) {
 
 // A workgroup's four waves per row (WHOLE), or one wave where rows are many and short; 8 values per lane and step.  Rows of up to
 // 2048 * HELD values (512 * HELD) stay in registers between the maximum and the rounding, longer ones (HELD 0) are read twice.
-// HBM-bound: 8100 x 2048 bf16 13.5 us (3.7 TB/s read and written, a launch's 4 included), 8100 x 6144 29 (5.1), 387 x 1003 fp32 4.6.
-// A wave per row: 14.3, 36; 8100 x 1003: 9.4 against 10.7 for a workgroup.
+// HBM-bound: 8100 x 2048 bf16 13.2 us (3.8 TB/s read and written, a launch's 4 included), 8100 x 6144 28 (5.3), 387 x 1003 fp32 4.6.
+// With a wave per row, before bf16 rows lost their remainders: 14.3 against 13.5, 36 against 29; 8100 x 1003: 9.4 against 10.7.
 template <bool F32, int HELD, bool WHOLE>
 __global__ __launch_bounds__(256) void i8_quantize_kernel(const void* x, int64_t ldx, int rows, int cols, int8_t* q, int64_t ldq, float* scales) {
     constexpr int STEP = WHOLE ? 256 : 64;
@@ -217,14 +238,14 @@ __global__ __launch_bounds__(256) void i8_quantize_kernel(const void* x, int64_t
         for (int i = 0; i < HELD; ++i) {
             float v[8];
             x8[i].values(v);
-            if (place(i) < k16) *(uint2*)(dst + place(i)) = rs.pack8(v);
+            if (place(i) < k16) *(uint2*)(dst + place(i)) = rs.template pack8<F32>(v);
         }
     } else if (cols < 8) {
         float v[8];
         i8_load8<F32>(src, place(0), cols, v);
         const RowScale rs(row_max(i8_max8(0, v)));
         if (lane == 0) scales[row] = rs.scale;
-        if (place(0) < k16) *(uint2*)(dst + place(0)) = rs.pack8(v);
+        if (place(0) < k16) *(uint2*)(dst + place(0)) = rs.template pack8<F32>(v);
     } else {
         constexpr int AT_ONCE = 4;
         I8Piece<F32> x8[AT_ONCE];
@@ -249,7 +270,7 @@ __global__ __launch_bounds__(256) void i8_quantize_kernel(const void* x, int64_t
             for (int i = 0; i < AT_ONCE; ++i) {
                 float v[8];
                 x8[i].values(v);
-                if (place(i0 + i) < k16) *(uint2*)(dst + place(i0 + i)) = rs.pack8(v);
+                if (place(i0 + i) < k16) *(uint2*)(dst + place(i0 + i)) = rs.template pack8<F32>(v);
             }
         }
     }
@@ -686,7 +707,7 @@ void launch_gemm256(const I8Params& p, hipStream_t s) {
 // wave's share of up to NS steps is requested at once.  The activation rows are rounded to 8 bits by every workgroup for itself,
 // underneath those loads: they are a few KB from the L2, and a second kernel in front would cost more than the whole product.
 // Weight rows are the MFMA "A" operand (lane: row li, bytes 16 lg ..), the activation rows in LDS the "B".
-// 1 x 2048 -> 4096: 4.5 us, of which a launch alone takes 2; 5 x 6144 -> 2048: 10.5, of which 4 are the rounding of 5 rows.
+// 1 x 2048 -> 4096: 4.5 us, of which a launch alone takes 2; 5 x 6144 -> 2048: 9.8, of which 2.6 are the rounding of 5 rows.
 // FROM: 0 bf16 rows, 1 fp32 rows, 2 rows that are rounded already.  HELD > 0: K is at least 8 and a thread's share of the rows, at
 // most HELD pieces of 8 values, is requested before the weights and held in registers, so that nothing waits behind the weights; 0:
 // any K, read twice.
@@ -754,7 +775,7 @@ __global__ __launch_bounds__(FEW_THREADS, 2) void i8_few_rows_kernel(I8Params p,
             const RowScale rs = scales[row_of[i]];
             float v[8];
             held[i].values(v);
-            if (tid + FEW_THREADS * i < pieces) *(uint2*)(xq + row_of[i] * stride + k_of[i]) = rs.pack8(v);
+            if (tid + FEW_THREADS * i < pieces) *(uint2*)(xq + row_of[i] * stride + k_of[i]) = rs.template pack8<F32>(v);
         }
     } else if constexpr (FROM == 2) {
         request(n0, 0);
@@ -788,7 +809,7 @@ __global__ __launch_bounds__(FEW_THREADS, 2) void i8_few_rows_kernel(I8Params p,
             const char* row = (const char*)src.x + (int64_t)m * src.ldx * (F32 ? 4 : 2);
             float v[8];
             i8_load8<F32>(row, k, p.K, v);
-            *(uint2*)(xq + m * stride + k) = rs.pack8(v);
+            *(uint2*)(xq + m * stride + k) = rs.template pack8<F32>(v);
         }
         request(n0, 0);
     }
@@ -845,8 +866,8 @@ void launch_few_steps(const I8Params& p, const I8Source& src, hipStream_t s) {
     else launch_few<FROM, 12, HELD>(p, src, s);
 }
 // Whether rounding the rows in every workgroup is cheaper than a launch of its own (us, one kernel against two): 1 x 2048 -> 4096:
-// 4.9, 7.4; 5 x 2048 -> 4096: 6.0, 7.8; 8: 6.4, 7.9; 10 (more than 4 pieces per thread): 8.1, 7.7; 16 x 1024 -> 4096: 6.4, 7.8;
-// 5 x 6144 -> 2048: 11.3, 13.2; 6: 13.4, 14.4; 5 x 2047 -> 2048: 6.4, 7.9; 8 x 1003 -> 12288: 7.6, 8.0; 10: 8.6, 7.8.
+// 4.9, 7.4; 5 x 2048 -> 4096: 5.4, 7.8; 8: 6.4, 7.9; 10 (more than 4 pieces per thread): 8.1, 7.7; 16 x 1024 -> 4096: 6.4, 7.8;
+// 5 x 6144 -> 2048: 9.9, 13.2; 6: 12.3, 14.4; 5 x 2047 -> 2048: 5.8, 7.9; 8 x 1003 -> 12288: 7.6, 8.0; 10: 8.6, 7.8.
 template <int FROM>
 bool launch_few_rows(const I8Params& p, const I8Source& src, hipStream_t s) {
     const int64_t held = cdiv((int64_t)p.M * cdiv(p.K, 64) * 8, FEW_THREADS);

@@ -94,6 +94,34 @@ def test_quantize_rows_at_the_borders(tiny_model):
     assert np.isnan(scale[1]) and np.isnan(scale[2]) and scale[0] == 0
 
 
+@pytest.mark.parametrize("rows", [128, 1152])
+def test_quantize_every_ratio_of_bf16_values(tiny_model, rows):
+    """Every pair of bf16 mantissas as value and maximum of a row, the value smaller by up to 2^9, either sign: all quotients that lie
+    half way between two whole numbers before the scale is rounded, and all next to them; with the product's own rounding as well."""
+    from q3asr import Int8Linear, quantize_rows
+    a = (np.arange(256)[None, :] / 2.0 ** np.arange(10)[:, None]).reshape(-1)
+    a = np.concatenate([a, -a])
+    tops = np.arange(128, 256, dtype=np.float64)
+    x = np.where(np.abs(a) <= tops[:, None], a, 0)
+    x[:, 0] = tops
+    x = np.concatenate([x * 2.0 ** e for e in range(-40, -40 + 10 * (rows // 128), 10)]).astype(np.float32)
+    assert np.array_equal(bf16_vals(bf16_bits(x)), x)
+    m, k = x.shape
+    with Device() as dev:
+        model = tiny_model[0]
+        q, s, at = dev.raw(m * k), dev.raw(4 * m), dev.put(bf16_bits(x))
+        quantize_rows(model, at, m, k, q, s)
+        got, scale = dev.get(q, (m, k), np.int8), dev.get(s, m, np.float32)
+        want_s, want_q = _quantize64(x)
+        assert np.array_equal(scale, want_s) and np.array_equal(got, want_q)
+        lin = Int8Linear(model, q, s, m, k)          # few rows are rounded inside the product
+        o, ref, ws = dev.raw(4 * m), dev.raw(4 * m), lin.workspace_bytes(1)
+        for row in range(0, m, 37):
+            lin(at + 2 * k * row, 1, o, out_dtype="f32", workspace=(dev.raw(ws), ws))
+            lin.matmul(q + k * row, s + 4 * row, 1, ref, out_dtype="f32")
+            assert np.array_equal(dev.get(o, m, np.float32), dev.get(ref, m, np.float32)), row
+
+
 SHAPES = [(1, 1, 1), (1, 4096, 2048), (2, 33, 100), (3, 2048, 6144), (4, 64, 33), (5, 70, 1003), (8, 256, 512), (16, 1000, 784),
           (17, 31, 48), (31, 515, 2080), (64, 64, 128), (65, 127, 129), (130, 2048, 4096), (200, 320, 6000), (333, 1027, 1003), (700, 769, 300),
           (2100, 2304, 256), (300, 12288, 96), (1000, 1500, 200), (3100, 4001, 130), (3100, 4000, 640), (40, 40000, 64), (6, 96, 6200), (2, 50, 13000)]
