@@ -263,8 +263,8 @@ int q3asr_pages_reserve(q3asr_model* m, const q3asr_kv_pages* c, const int32_t* 
 int q3asr_pages_compact(q3asr_model* m, const q3asr_kv_pages* c, void* stream);
 
 /* The rows of a step: sequence seqs[i] has rows cu_rows[i] .. cu_rows[i + 1) of it, which are its last tokens (lens counts them
- * already: q3asr_pages_reserve).  A sequence stands in the list once; an entry of -1 has no rows.  Rows from cu_rows[n] on (a
- * padded batch) are left alone.  Optionally, consecutive sequences of the list form groups
+ * already: q3asr_pages_reserve).  A sequence stands in the list once; an entry of -1 has no rows and changes nothing for the
+ * others, wherever in the list or a group it stands.  Rows from cu_rows[n] on (a padded batch) are left alone.  Optionally, consecutive sequences of the list form groups
  * (group g: entries cu_groups[g] .. cu_groups[g + 1)) whose first shared[g] tokens lie in the same pages; those are then read
  * once for the group.  shared[g] counts at most the tokens before the step's rows and is rounded down to whole pages.  The host
  * numbers bound what the arrays hold; smaller bounds make smaller grids.  rows is below 2^24, and rows * heads / 16 times

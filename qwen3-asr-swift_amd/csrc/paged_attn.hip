@@ -135,20 +135,25 @@ __device__ __forceinline__ Entry entry_of(const AttnParams& p, int i, bool repor
 constexpr int HELD = 1024;   // as a launch of its own the plan costs 6 us, in front of every wave 4
 struct PlanMemory {
     Entry* entry;            // [n]
-    int *from, *cu, *rows;   // [n_groups] tokens that a group shares, [n_groups + 1], [n + 1]: of the batch
-    int* scan;               // a word per wave
-    Segment* segments;       // [n_groups + n]
+    int *from, *lead;        // [n_groups] tokens that a group shares, and its first entry that stands for a sequence
+    int *cu, *rows;          // [n_groups + 1], [n + 1]: of the batch
+    static constexpr int64_t bytes(int64_t n, int64_t groups) { return n * (int64_t)sizeof(Entry) + (3 * groups + n + 2) * 4; }
+    __device__ PlanMemory(void* at, int n, int groups) {
+        entry = (Entry*)at;
+        from = (int*)(entry + n);
+        lead = from + groups;
+        cu = lead + groups;
+        rows = cu + groups + 1;
+    }
 };
+// The batch's entries, and what its groups share.  All threads of the workgroup; ends behind a barrier.
 template <int THREADS>
-__device__ __forceinline__ Total plan_segments(const AttnParams& p, const PlanMemory& mem, bool tell) {
-    const int tid = threadIdx.x;
+__device__ __forceinline__ void read_batch(const AttnParams& p, const PlanMemory& mem, bool tell) {
+    const int tid = threadIdx.x, lane = tid & 63;
     Entry* const entry = mem.entry;
-    int* const from = mem.from;
-    int *const cu = mem.cu, *const cu_rows = mem.rows, *const scan = mem.scan;
-    if (tell)
-        for (int r = tid; r < p.rows; r += THREADS) p.parts[r].known = 0;
+    int *const from = mem.from, *const cu = mem.cu, *const cu_rows = mem.rows;
     const int last_g = p.n_groups - 1, last = p.n - 1;
-    for (int i = tid; i <= p.n || i <= p.n_groups; i += THREADS) {   // n_groups may exceed n: empty groups
+    for (int i = tid; i <= p.n || i <= p.n_groups; i += THREADS) {
         // all that does not depend on another load at once
         const int seq = p.seqs[min(i, last)], a = p.cu_rows[min(i, last)], b = p.cu_rows[min(i, last) + 1];
         const int group = last_g < 0 ? 0 : p.cu_groups[min(i, last_g + 1)], shared = last_g < 0 ? 0 : p.shared[min(i, last_g)];
@@ -162,20 +167,75 @@ __device__ __forceinline__ Total plan_segments(const AttnParams& p, const PlanMe
         if (last_g >= 0 && i <= last_g + 1) cu[i] = group;
     }
     __syncthreads();
-    for (int g = tid; g < p.n_groups; g += THREADS) {
-        const int i0 = cu[g], i1 = cu[g + 1], shared = from[g];
+    for (int g0 = 0; g0 < p.n_groups; g0 += THREADS) {
+        const int g = g0 + tid;
+        int i0 = 0, i1 = 0;
+        if (g < p.n_groups) {
+            i0 = cu[g];
+            i1 = cu[g + 1];
+            if (i0 < 0 || i1 < i0 || i1 > p.n) {
+                if (tell) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, g);
+                i0 = i1 = 0;
+            }
+        }
+        // Entries that stand for no sequence (-1: hypotheses that have ended) may come first: a thread looks past a few, its wave past more.
+        int lead = i0;
+        const int near = min(i1, i0 + 8);
+        while (lead < near && !entry[lead].ok) ++lead;
+        for (unsigned long long open = __ballot(lead == near && near < i1); open; open &= open - 1) {
+            const int who = __ffsll(open) - 1, end = __shfl(i1, who, 64);
+            int at = __shfl(lead, who, 64);
+            unsigned long long found = 0;
+            while (at < end) {
+                found = __ballot(at + lane < end && entry[min(at + lane, last)].ok);
+                if (found) break;
+                at += 64;
+            }
+            if (lane == who) lead = found ? at + __ffsll(found) - 1 : end;
+        }
+        if (g >= p.n_groups) continue;
+        const int shared = from[g];
         from[g] = 0;
-        if (i0 < 0 || i1 < i0 || i1 > p.n) {
-            if (tell) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, g);
-        } else if (i1 > i0) {
-            const Entry first = entry[i0];
+        mem.lead[g] = lead;
+        if (lead < i1) {   // a group without sequences shares nothing
+            const Entry first = entry[lead];
             const int end = cu_rows[i1];
             const bool fits = end >= first.r0 && end <= p.rows && end - first.r0 <= p.max_group_rows;
-            if (shared > p.max_shared || (first.ok && !fits)) if (tell) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, i0);
-            if (first.ok && fits) from[g] = max(0, min(min(shared, p.max_shared), first.len - first.T)) >> p.pt_shift << p.pt_shift;
+            if (shared > p.max_shared || !fits) if (tell) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, lead);
+            if (fits) from[g] = max(0, min(min(shared, p.max_shared), first.len - first.T)) >> p.pt_shift << p.pt_shift;
         }
     }
     __syncthreads();
+}
+// Behind read_batch: the group of entry i (-1: none), and how many of the entry's first keys are read by the group.
+struct Member {
+    int group, behind;
+};
+__device__ __forceinline__ Member member_of(const AttnParams& p, const PlanMemory& mem, int i, bool tell) {
+    Member m{-1, 0};
+    const Entry e = mem.entry[i];
+    if (p.n_groups > 0) {
+        int lo = 0, hi = p.n_groups;   // the last group that begins at or before entry i
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (mem.cu[mid] <= i) lo = mid;
+            else hi = mid;
+        }
+        const int i0 = mem.cu[lo], i1 = mem.cu[lo + 1];
+        if (i0 >= 0 && i >= i0 && i < i1 && i1 <= p.n) m = Member{lo, mem.from[lo]};
+        else if (tell) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, i);
+    }
+    // keys behind max_own would be left out
+    if (tell && e.ok && (m.behind > max(0, e.len - e.T) || e.len - m.behind > p.max_own)) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, i);
+    return m;
+}
+// scan: a word per wave; segments: [n_groups + n].
+template <int THREADS>
+__device__ __forceinline__ Total plan_segments(const AttnParams& p, const PlanMemory& mem, int* scan, Segment* segments, bool tell) {
+    const int tid = threadIdx.x;
+    if (tell)
+        for (int r = tid; r < p.rows; r += THREADS) p.parts[r].known = 0;
+    read_batch<THREADS>(p, mem, tell);
     // segments: the groups', then the sequences'
     const int all = p.n_groups + p.n;
     int carry = 0;
@@ -185,33 +245,16 @@ __device__ __forceinline__ Total plan_segments(const AttnParams& p, const PlanMe
         int g = -1, count = 0;
         Entry e{};
         if (w < p.n_groups) {
-            if (from[w] > 0) {   // a group without sequences or with wrong ones shares nothing
-                const Entry first = entry[cu[w]];
-                sg = Segment{first.r0, (cu_rows[cu[w + 1]] - first.r0) * p.group, first.seq, 0, from[w], SHARED, 0, 0};
+            if (mem.from[w] > 0) {
+                const Entry first = mem.entry[mem.lead[w]];
+                sg = Segment{first.r0, (mem.rows[mem.cu[w + 1]] - first.r0) * p.group, first.seq, 0, mem.from[w], SHARED, 0, 0};
             }
         } else if (w < all) {
             const int i = w - p.n_groups;
-            e = entry[i];
-            int behind = 0;      // keys before it are read by the group
-            bool ok = e.ok;
-            if (p.n_groups > 0) {
-                int lo = 0, hi = p.n_groups;   // the last group that begins at or before entry i
-                while (hi - lo > 1) {
-                    const int mid = (lo + hi) >> 1;
-                    if (cu[mid] <= i) lo = mid;
-                    else hi = mid;
-                }
-                const int i0 = cu[lo], i1 = cu[lo + 1];
-                if (i0 >= 0 && i >= i0 && i < i1 && i1 <= p.n) {
-                    g = lo;
-                    behind = from[lo];
-                    ok = ok && entry[i0].ok;
-                } else {
-                    if (tell) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, i);
-                }
-            }
-            if (ok && (behind > max(0, e.len - e.T) || e.len - behind > p.max_own)) if (tell) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, i);
-            sg = Segment{e.r0, e.T * p.group, e.seq, behind, behind + min(max(0, e.len - behind), p.max_own), e.len - e.T + 1, 0, behind == 0};
+            e = mem.entry[i];
+            const Member m = member_of(p, mem, i, tell);
+            g = m.group;
+            sg = Segment{e.r0, e.T * p.group, e.seq, m.behind, m.behind + min(max(0, e.len - m.behind), p.max_own), e.len - e.T + 1, 0, m.behind == 0};
         }
         const int tiles = (sg.k1 - sg.k0 + 31) >> 5;
         const int streams = (sg.M + (1 << p.shift_q) - 1) >> p.shift_q;
@@ -232,12 +275,12 @@ __device__ __forceinline__ Total plan_segments(const AttnParams& p, const PlanMe
             carry += scan[v];
         }
         sg.start = before + x - count;
-        if (w < all) mem.segments[w] = sg;
+        if (w < all) segments[w] = sg;
         __syncthreads();   // scan is written again; the groups' segments are read below
         if (tell && w >= p.n_groups && w < all) {
             RowParts rp{};
-            if (g >= 0 && from[g] > 0) {
-                const Segment& sh = mem.segments[g];
+            if (g >= 0 && mem.from[g] > 0) {
+                const Segment& sh = segments[g];
                 rp.start[0] = sh.start;
                 rp.tiles[0] = (sh.k1 - sh.k0 + 31) >> 5;
                 rp.r0[0] = sh.r0;
@@ -257,28 +300,7 @@ __device__ __forceinline__ Total plan_segments(const AttnParams& p, const PlanMe
 }
 __global__ __launch_bounds__(PLAN) void paged_attn_plan_kernel(AttnParams p) {
     __shared__ int scan[PLAN / 64];
-    int* ints = (int*)((Entry*)p.plan_ws + p.n);
-    plan_segments<PLAN>(p, PlanMemory{(Entry*)p.plan_ws, ints, ints + p.n_groups, ints + 2 * p.n_groups + 1, scan, p.segments}, true);
-}
-
-// Without a plan the groups are not used; a workgroup of its own checks them all the same.
-__device__ void check_groups(const AttnParams& p) {
-    if (threadIdx.x == 0 && (p.cu_groups[0] != 0 || p.cu_groups[p.n_groups] != p.n)) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, 0);
-    for (int g = threadIdx.x; g < p.n_groups; g += blockDim.x) {
-        const int i0 = p.cu_groups[g], i1 = p.cu_groups[g + 1], shared = p.shared[g];
-        if (i0 < 0 || i1 < i0 || i1 > p.n) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, g);
-        else if (i1 > i0) {
-            const Entry first = entry_of(p, i0, false);
-            const int end = p.cu_rows[i1], behind = max(0, min(shared, first.len - first.T)) >> p.pt_shift << p.pt_shift;
-            if (!first.ok) continue;
-            if (shared > p.max_shared || end < first.r0 || end > p.rows || end - first.r0 > p.max_group_rows)
-                pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, i0);
-            for (int i = i0; i < i1; ++i) {
-                const Entry e = entry_of(p, i, false);
-                if (e.ok && (behind > max(0, e.len - e.T) || e.len - behind > p.max_own)) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, i);
-            }
-        }
-    }
+    plan_segments<PLAN>(p, PlanMemory(p.plan_ws, p.n, p.n_groups), scan, p.segments, true);
 }
 
 // ---- a wave's work ----
@@ -482,7 +504,7 @@ __device__ __forceinline__ float inverse_of(float l) { return l > 0.f || l != l 
 // ---- stream ----
 template <int D, int QT, bool ONCE, bool PLANNED>
 __global__ __launch_bounds__(256, 2) void paged_attn_stream_kernel(AttnParams p) {
-    constexpr int PLAN_BYTES = PLANNED ? 0 : HELD * (int)sizeof(Entry) + (3 * HELD + 2 + WAVES) * 4, TILES = WAVES * Rows<D>::TILE;
+    constexpr int PLAN_BYTES = PLANNED ? 0 : (int)PlanMemory::bytes(HELD, HELD) + WAVES * 4, TILES = WAVES * Rows<D>::TILE;
     __shared__ __attribute__((aligned(16))) char lds[PLAN_BYTES > TILES ? PLAN_BYTES : TILES];
     __shared__ Segment held[PLANNED ? 1 : HELD];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -490,8 +512,8 @@ __global__ __launch_bounds__(256, 2) void paged_attn_stream_kernel(AttnParams p)
     Total total;
     if constexpr (PLANNED) total = *p.total;
     else {
-        int* ints = (int*)((Entry*)lds + HELD);
-        total = plan_segments<256>(p, PlanMemory{(Entry*)lds, ints, ints + HELD, ints + 2 * HELD + 1, ints + 3 * HELD + 2, held}, blockIdx.x == 0);
+        const PlanMemory mem(lds, HELD, HELD);
+        total = plan_segments<256>(p, mem, mem.rows + HELD + 1, held, blockIdx.x == 0);
         __syncthreads();   // the tiles go where the plan was made
     }
     int share = blockIdx.x;
@@ -739,10 +761,13 @@ __global__ __launch_bounds__(64 * PLAIN_WAVES) void paged_attn_plain_kernel(Attn
     __shared__ __attribute__((aligned(16))) char lds[WAVES * Rows<D>::TILE];
     __shared__ float sm_m[WAVES][16], sm_l[WAVES][16];
     static_assert(WAVES * Rows<D>::TILE >= WAVES * 16 * OROW * 4, "the waves' results fit where their tiles were");
+    static_assert(WAVES * Rows<D>::TILE >= PlanMemory::bytes(HELD, HELD) && HELD >= 2 * PLAIN_ITEMS, "so does the batch");
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int kvh = blockIdx.x % p.kv_heads, x = blockIdx.x / p.kv_heads, i = x / p.tiles_q;
-    if (i == p.n) {
-        check_groups(p);
+    if (i == p.n) {   // the groups are not used here; a workgroup of its own checks them all the same
+        const PlanMemory mem(lds, HELD, HELD);
+        read_batch<64 * PLAIN_WAVES>(p, mem, true);
+        for (int k = tid; k < p.n; k += 64 * PLAIN_WAVES) member_of(p, mem, k, true);
         return;
     }
     const Entry e = entry_of(p, i, true);
@@ -840,7 +865,7 @@ Plan plan_for(const q3asr_kv_pages& c, const q3asr_attn_batch& b, int heads) {
     auto round = [](int64_t x) { return (x + 255) & ~255ll; };
     const int64_t groups = shares ? b.n_groups : 0;
     r.at_plan = 256;
-    r.at_segments = r.at_plan + (b.n + groups > HELD ? round((int64_t)b.n * (int64_t)sizeof(Entry) + (2 * groups + b.n + 2) * 4) : 0);
+    r.at_segments = r.at_plan + (b.n + groups > HELD ? round(PlanMemory::bytes(b.n, groups)) : 0);
     r.at_parts = r.at_segments + (b.n + groups > HELD ? round((b.n + groups) * (int64_t)sizeof(Segment)) : 0);
     r.at_ml = r.at_parts + round((int64_t)b.rows * (int64_t)sizeof(RowParts));
     r.at_o = r.at_ml + round((int64_t)b.rows * heads * r.slots * 8);
