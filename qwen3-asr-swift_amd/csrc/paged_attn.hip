@@ -3,8 +3,10 @@
 // o = sum_j p_j v_j, p = softmax_j(scale q . k_j).  The keys of a sequence are its group's shared pages and its own pages; all query
 // rows that read a shared key -- of every sequence of the group, with all query heads of the KV head -- are columns of one matrix
 // product, so that a shared key crosses HBM once per group.  Partial results (max, sum, weighted sum of values) are joined per
-// row.  Both softmax statistics and the sums stay in fp32; the probabilities are rounded to bf16 for the matrix cores (at most
-// 2^-8 relative each, which averages out over the keys of a row).
+// row.  Both softmax statistics and the sums stay in fp32; a probability meets the matrix cores as the sum of two bf16 numbers, its
+// rounding and the rounding of what that leaves (2^-16 of it is lost at most).  Rounded to bf16 once, they took the results' error against 64
+// bits from 0.00166, which is their own rounding's, to 0.0021-0.0025; the second product costs 40.1 -> 42.0 us where query rows are
+// many (12 x 7 scored) and nothing that shows where HBM bounds (96 x 5: 120.5, 120.7; 16 x 8: 149.0, 149.3).
 //
 // HBM-bound: 2 * head_dim * 2 bytes per key and KV head against 16 * QT columns.  A wave works on tiles of 32 keys: the K rows,
 // loaded whole, become MFMA A fragments of S^T = K Q^T through an LDS tile of the wave's own; the exponentiated scores are as
@@ -326,7 +328,7 @@ struct Wave {
     int lowest;                   // keys below it are seen by all of them
     int active;                   // groups of 16 queries that there are
     // Weights are powers of two above m, a bound that no score so far exceeds by more than SLACK: it is only moved, and the sums
-    // with it, when one does.  So weights are below 2^SLACK; fp32 sums and the relative rounding to bf16 are as good there.
+    // with it, when one does.  So weights are below 2^SLACK; fp32 sums and relative roundings are as good there.
     static constexpr float SLACK = 8.f;
     float m[QT], less[QT], l[QT];   // less: -m, 0 while there is no m; l: of this lane's keys only, until the end
     f32x4 o[QT][NDT];             // lane (li, lg) holds values 16 dt + 4 lg .. of query 16 qt + li
@@ -410,7 +412,7 @@ struct Wave {
         for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int ks = 0; ks < NKS; ++ks) ka[h][ks].u = *(const uint4*)(kr + 16 * h * KROW + 64 * ks);
-        Frag pf[QT];
+        Frag pf[QT], pr[QT];   // the weights rounded to bf16, and what that left over
 #pragma unroll
         for (int g = 0; g < QT; g += PAIR) {
             if (g > 0 && g >= active) break;   // wave-uniform
@@ -462,7 +464,14 @@ struct Wave {
                     pe[j] = __builtin_amdgcn_exp2f(fmaf(s[i][j >> 2][j & 3], p.scale_log2, less[qt]));
                     l[qt] += pe[j];
                 }
-                pf[qt].u = make_uint4(pack_bf16x2(pe[0], pe[1]), pack_bf16x2(pe[2], pe[3]), pack_bf16x2(pe[4], pe[5]), pack_bf16x2(pe[6], pe[7]));
+                uint32_t whole[4], rest[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    whole[j] = pack_bf16x2(pe[2 * j], pe[2 * j + 1]);
+                    rest[j] = pack_bf16x2(pe[2 * j] - __uint_as_float(whole[j] << 16), pe[2 * j + 1] - __uint_as_float(whole[j] & 0xffff0000u));
+                }
+                pf[qt].u = make_uint4(whole[0], whole[1], whole[2], whole[3]);
+                pr[qt].u = make_uint4(rest[0], rest[1], rest[2], rest[3]);
             }
         }
         __builtin_amdgcn_wave_barrier();   // the V rows go where the K rows were
@@ -491,6 +500,7 @@ struct Wave {
 #pragma unroll
             for (int qt = 0; qt < QT; ++qt) {
                 if (qt >= PAIR && qt / PAIR * PAIR >= active) break;
+                o[qt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va.v, pr[qt].v, o[qt][dt], 0, 0, 0);
                 o[qt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va.v, pf[qt].v, o[qt][dt], 0, 0, 0);
             }
         }
