@@ -240,8 +240,9 @@ enum {
 /* Numbers in device arrays cannot be refused by the host, so every call checks them on the device.  fork, free, reserve and
  * compact do all of their work or, where an entry is wrong, none of it; write leaves out what is wrong, and the results of an
  * attention that reports an error are not to be used.  The first
- * such error since the last reset of the status is kept: status[0] = code, [1] = number of the (first) wrong entry in the list,
- * [2] = pages short of (NO_PAGES), and [3] = pages in use after the last compact.  Calls on the model's own stream (stream
+ * such error since the last reset of the status is kept: status[0] = code, [1] = number of the wrong entry in the list (where several are
+ * wrong, fork, free and reserve tell the first, write and attention any of them; NO_PAGES: the number of entries), [2] = pages short of
+ * (NO_PAGES), and [3] = pages in use after the last compact.  Calls on the model's own stream (stream
  * NULL) return the error that is kept, if any, and reset the status; after calls on another stream the host asks here: waits for the
  * stream, copies the status to out (host, 4 numbers) and, where clear is non-zero, sets it to zeros.  Not under graph capture. */
 int q3asr_pages_status(q3asr_model* m, const q3asr_kv_pages* c, int32_t* out, int clear, void* stream);

@@ -70,7 +70,7 @@ struct __attribute__((aligned(16))) Segment {
     int r0, M, seq, k0, k1, limit;
     int start;    // place in the row of all tiles: stream h * query tiles + q (KV head h, query tile q) takes ntiles + 1 places from
                   // start + stream * (ntiles + 1) on, one for its beginning and one per tile
-    int whole;    // 1: its rows read nothing else
+    int tag;      // 2 * the entry of the batch that errors name, a group's first sequence for its own segment; + 1: its rows read nothing else
 };
 constexpr int SHARED = 0x7fffffff;
 // Where a row's parts are: tiles of its group's and of its own segment (0: none), their starts, first rows and query tiles.
@@ -176,7 +176,7 @@ __device__ __forceinline__ void read_batch(const AttnParams& p, const PlanMemory
             i0 = cu[g];
             i1 = cu[g + 1];
             if (i0 < 0 || i1 < i0 || i1 > p.n) {
-                if (tell) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, g);
+                if (tell) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, min(max(i0, 0), last));   // where the group would begin
                 i0 = i1 = 0;
             }
         }
@@ -249,14 +249,14 @@ __device__ __forceinline__ Total plan_segments(const AttnParams& p, const PlanMe
         if (w < p.n_groups) {
             if (mem.from[w] > 0) {
                 const Entry first = mem.entry[mem.lead[w]];
-                sg = Segment{first.r0, (mem.rows[mem.cu[w + 1]] - first.r0) * p.group, first.seq, 0, mem.from[w], SHARED, 0, 0};
+                sg = Segment{first.r0, (mem.rows[mem.cu[w + 1]] - first.r0) * p.group, first.seq, 0, mem.from[w], SHARED, 0, 2 * mem.lead[w]};
             }
         } else if (w < all) {
             const int i = w - p.n_groups;
             e = mem.entry[i];
             const Member m = member_of(p, mem, i, tell);
             g = m.group;
-            sg = Segment{e.r0, e.T * p.group, e.seq, m.behind, m.behind + min(max(0, e.len - m.behind), p.max_own), e.len - e.T + 1, 0, m.behind == 0};
+            sg = Segment{e.r0, e.T * p.group, e.seq, m.behind, m.behind + min(max(0, e.len - m.behind), p.max_own), e.len - e.T + 1, 0, 2 * i + (m.behind == 0)};
         }
         const int tiles = (sg.k1 - sg.k0 + 31) >> 5;
         const int streams = (sg.M + (1 << p.shift_q) - 1) >> p.shift_q;
@@ -335,12 +335,12 @@ struct Wave {
     int ids, id_base;             // page numbers of 64 times 16 keys from key id_base on, one per lane
     __device__ Wave(const AttnParams& p_, char* tile_) : p(p_), lane(threadIdx.x & 63), li(threadIdx.x & 15), lg((threadIdx.x & 63) >> 4), tile(tile_) {}
 
-    __device__ void page_numbers(int seq, int base, int k1) {
+    __device__ void page_numbers(const Segment& sg, int base) {
         id_base = base;
-        const int key = min(base + 16 * lane, k1 - 1);
-        ids = p.table[(int64_t)seq * p.max_seq_pages + (key >> p.pt_shift)];
+        const int key = min(base + 16 * lane, sg.k1 - 1);
+        ids = p.table[(int64_t)sg.seq * p.max_seq_pages + (key >> p.pt_shift)];
         if ((unsigned)ids >= (unsigned)p.pages) {
-            pages_error(p.status, Q3ASR_PAGES_BAD_INDEX, 0);
+            pages_error(p.status, Q3ASR_PAGES_BAD_INDEX, sg.tag >> 1);
             ids = 0;
         }
     }
@@ -570,7 +570,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_stream_kernel(AttnParams p)
         }
     }
     int64_t head = (int64_t)kvh * p.head_stride;
-    auto window = [&] { w.page_numbers(sg.seq, sg.k0 + 32 * rel, sg.k1); };
+    auto window = [&] { w.page_numbers(sg, sg.k0 + 32 * rel); };
     window();
     w.load(p.K, w.kf, head, sg.k0 + 32 * rel, sg.k1);
     w.load(p.V, w.vf, head, sg.k0 + 32 * rel, sg.k1);
@@ -617,7 +617,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_stream_kernel(AttnParams p)
             const int streams = (now.M + 16 * QT - 1) / (16 * QT);
             const int tile0 = now.start + (now_kvh * streams + now_first / (16 * QT)) * (now_tiles + 1) + 1;   // the first tile's place
             const int before = tile0 / total.per, piece = pos / total.per - before;
-            const bool direct = now.whole && (tile0 + now_tiles - 1) / total.per == before;
+            const bool direct = (now.tag & 1) && (tile0 + now_tiles - 1) / total.per == before;
             const int slot = (now.limit == SHARED ? 0 : p.slots_p) + piece;
 #pragma unroll
             for (int qt = 0; qt < QT; ++qt) {
@@ -781,14 +781,14 @@ __global__ __launch_bounds__(64 * PLAIN_WAVES) void paged_attn_plain_kernel(Attn
         return;
     }
     const Entry e = entry_of(p, i, true);
-    const Segment sg{e.r0, e.T * p.group, e.seq, 0, min(e.len, PLAIN_KEYS), e.len - e.T + 1, 0, 1};
+    const Segment sg{e.r0, e.T * p.group, e.seq, 0, min(e.len, PLAIN_KEYS), e.len - e.T + 1, 0, 2 * i + 1};
     const int first = (x - i * p.tiles_q) * 16 * QT, ntiles = (sg.k1 + 31) >> 5;
     if (first >= sg.M) return;
     Wave<D, QT, true> w(p, lds + wave * Rows<D>::TILE);
     const int64_t head = (int64_t)kvh * p.head_stride;
     int t = wave;
     if (t < ntiles) {
-        w.page_numbers(sg.seq, 0, sg.k1);
+        w.page_numbers(sg, 0);
         w.load(p.K, w.kf, head, 32 * t, sg.k1);
         w.load(p.V, w.vf, head, 32 * t, sg.k1);
     }
