@@ -268,8 +268,8 @@ int q3asr_pages_compact(q3asr_model* m, const q3asr_kv_pages* c, void* stream);
  * others, wherever in the list or a group it stands.  Rows from cu_rows[n] on (a padded batch) are left alone.  Optionally, consecutive sequences of the list form groups
  * (group g: entries cu_groups[g] .. cu_groups[g + 1)) whose first shared[g] tokens lie in the same pages; those are then read
  * once for the group.  shared[g] counts at most the tokens before the step's rows and is rounded down to whole pages.  The host
- * numbers bound what the arrays hold; smaller bounds make smaller grids.  rows is below 2^24, and rows * heads / 16 times
- * max_len / 32 stays below 2^30. */
+ * numbers bound what the arrays hold; smaller bounds make smaller grids.  rows is below 2^24, and
+ * rows * heads / 16 + n * kv_heads times max_len / 32 + 2 stays below 2^30 - 2^15. */
 typedef struct q3asr_attn_batch {
     const int32_t* seqs;       /* [n] */
     const int32_t* cu_rows;    /* [n + 1], from 0 to at most rows */

@@ -289,8 +289,8 @@ static void check_attention(const q3asr_kv_pages* c, const q3asr_attn_batch* b, 
     }
     // tiles of 32 keys by 16 rows, and one for every beginning, are counted in 32 bits: at most one incomplete tile of rows per sequence
     // and group and KV head, twice for shared and own keys
-    const int64_t tiles = ((int64_t)b->max_len + 63) / 32, streams = (int64_t)b->rows * heads / 16 + (int64_t)b->n * c->kv_heads;
-    Q3_REQUIRE(2 * streams < (1ll << 31) / tiles, "paged_attention: too many rows for so many tokens in one call");
+    const int64_t tiles = ((int64_t)b->max_len + 63) / 32, streams = ((int64_t)b->rows * heads + 15) / 16 + (int64_t)b->n * c->kv_heads;
+    Q3_REQUIRE(2 * streams < ((1ll << 31) - (1 << 16)) / tiles, "paged_attention: too many rows for so many tokens in one call");
 }
 
 int64_t q3asr_paged_attention_workspace(q3asr_model* m, const q3asr_kv_pages* c, const q3asr_attn_batch* b, int heads) {

@@ -148,13 +148,15 @@ struct PlanMemory {
         rows = cu + groups + 1;
     }
 };
-// The batch's entries, and what its groups share.  All threads of the workgroup; ends behind a barrier.
+// The batch's entries, and what its groups share.  All threads of the workgroup; ends behind a barrier.  False: cu_rows or cu_groups goes down
+// somewhere, so that rows or entries may count several times, and there may be more tiles than 32 bits count.
 template <int THREADS>
-__device__ __forceinline__ void read_batch(const AttnParams& p, const PlanMemory& mem, bool tell) {
+__device__ __forceinline__ bool read_batch(const AttnParams& p, const PlanMemory& mem, bool tell) {
     const int tid = threadIdx.x, lane = tid & 63;
     Entry* const entry = mem.entry;
     int *const from = mem.from, *const cu = mem.cu, *const cu_rows = mem.rows;
     const int last_g = p.n_groups - 1, last = p.n - 1;
+    bool down = false;
     for (int i = tid; i <= p.n || i <= p.n_groups; i += THREADS) {
         // all that does not depend on another load at once
         const int seq = p.seqs[min(i, last)], a = p.cu_rows[min(i, last)], b = p.cu_rows[min(i, last) + 1];
@@ -162,6 +164,7 @@ __device__ __forceinline__ void read_batch(const AttnParams& p, const PlanMemory
         __builtin_amdgcn_sched_barrier(0);
         if (i <= last) {
             entry[i] = entry_of(p, i, seq, a, b, tell);
+            down |= b < a;
             cu_rows[i] = a;
             if (i == last) cu_rows[i + 1] = b;
         }
@@ -175,6 +178,7 @@ __device__ __forceinline__ void read_batch(const AttnParams& p, const PlanMemory
         if (g < p.n_groups) {
             i0 = cu[g];
             i1 = cu[g + 1];
+            down |= i1 < i0;
             if (i0 < 0 || i1 < i0 || i1 > p.n) {
                 if (tell) pages_error(p.status, Q3ASR_PAGES_BAD_BATCH, min(max(i0, 0), last));   // where the group would begin
                 i0 = i1 = 0;
@@ -207,7 +211,7 @@ __device__ __forceinline__ void read_batch(const AttnParams& p, const PlanMemory
             if (fits) from[g] = max(0, min(min(shared, p.max_shared), first.len - first.T)) >> p.pt_shift << p.pt_shift;
         }
     }
-    __syncthreads();
+    return !__syncthreads_or(down);
 }
 // Behind read_batch: the group of entry i (-1: none), and how many of the entry's first keys are read by the group.
 struct Member {
@@ -237,7 +241,7 @@ __device__ __forceinline__ Total plan_segments(const AttnParams& p, const PlanMe
     const int tid = threadIdx.x;
     if (tell)
         for (int r = tid; r < p.rows; r += THREADS) p.parts[r].known = 0;
-    read_batch<THREADS>(p, mem, tell);
+    const bool rising = read_batch<THREADS>(p, mem, tell);
     // segments: the groups', then the sequences'
     const int all = p.n_groups + p.n;
     int carry = 0;
@@ -279,7 +283,7 @@ __device__ __forceinline__ Total plan_segments(const AttnParams& p, const PlanMe
         sg.start = before + x - count;
         if (w < all) segments[w] = sg;
         __syncthreads();   // scan is written again; the groups' segments are read below
-        if (tell && w >= p.n_groups && w < all) {
+        if (tell && rising && w >= p.n_groups && w < all) {
             RowParts rp{};
             if (g >= 0 && mem.from[g] > 0) {
                 const Segment& sh = segments[g];
@@ -296,6 +300,7 @@ __device__ __forceinline__ Total plan_segments(const AttnParams& p, const PlanMe
             for (int t = 0; t < e.T; ++t) p.parts[e.r0 + t] = rp;
         }
     }
+    if (!rising) carry = 0;   // reported; no row is computed
     const Total total{carry, max(p.per_min, (carry + STREAM_WAVES - 1) / STREAM_WAVES), all, 0};
     if (tell && tid == 0) *p.total = total;
     return total;
@@ -950,11 +955,6 @@ void launch_paged_attention(const q3asr_kv_pages& c, int layer, const bf16_t* q,
     p.parts = (RowParts*)(ws + r.at_parts);
     p.part_ml = (float2*)(ws + r.at_ml);
     p.part_o = (float*)(ws + r.at_o);
-    // places are 32-bit numbers
-    const int64_t group = p.group, own = cdiv(p.max_own, 32) + 1, sh = cdiv(p.max_shared, 32) + 1;
-    Q3_REQUIRE(r.plain || (own * cdiv((int64_t)b.max_rows * group, 16) * b.n + (shares ? sh * cdiv((int64_t)b.max_group_rows * group, 16) * b.n_groups : 0)) *
-                                  c.kv_heads < (1ll << 30),
-               "paged_attention: too much work for one call (smaller bounds in the batch make less)");
     ProfScope ps("paged_attn_kernel", 4.0 * b.rows * heads * (double)b.max_len * c.head_dim, s);
     if (c.head_dim == 64) launch_d<64>(p, r, s);
     else launch_d<128>(p, r, s);
