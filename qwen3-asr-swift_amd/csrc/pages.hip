@@ -565,7 +565,8 @@ void launch_copies(const Pages& p, int64_t most, hipStream_t s) {
     const int64_t items = std::max<int64_t>(most * p.layers * p.kv_heads * 2, RENUMBER ? 1 : 0);
     if (items <= 0) return;
     ProfScope ps("pages_copy_kernel", 0, s);
-    const int grid = (int)std::min<int64_t>(cdiv(items, COPY_THREADS / 64), 4 * device_cus());
+    constexpr int PER = COPY_THREADS / 64;
+    const int grid = (int)std::min<int64_t>((items + PER - 1) / PER, 4 * device_cus());   // items may pass 2^32
     hipLaunchKernelGGL((pages_copy_kernel<RENUMBER>), dim3(grid), dim3(COPY_THREADS), 0, s, p);
     HIP_CHECK(hipGetLastError());
 }

@@ -61,3 +61,22 @@ def test_lists_that_go_down_are_reported_and_write_nothing(tiny_model, over, n):
         c.c.attention(0, q, o, b, heads, workspace=(dev.raw(nb), nb), stream=st)
         assert c.c.status(stream=st)[0] == BAD_BATCH
         assert (dev.get(o, (8 * n, heads * dim), np.uint16) == 7).all()
+
+
+def test_runs_past_32_bits(tiny_model):
+    """Entries times layers times KV heads past 2^32: the copies' grid is counted in 64 bits.  No page is shared and none lies behind a gap, so
+    nothing is copied and the pools are never touched."""
+    from q3asr import PagedKVCache
+    n = 1024
+    with Device() as dev:
+        pool = dev.raw(16)
+        at = {"table": dev.raw(4 * n * 2), "lens": dev.raw(4 * n), "refs": dev.raw(4 * n), "status": dev.raw(16)}
+        c = PagedKVCache(tiny_model[0], k=pool, v=pool, layers=4096, pages=n, kv_heads=4096, head_dim=64, page_tokens=16, max_seqs=n, max_seq_pages=2, **at)
+        nb = c.workspace_bytes()
+        c.set_workspace(dev.raw(nb), nb)
+        c.reset()
+        c.reserve(dev.put(np.arange(n, dtype=np.int32)), dev.put(np.full(n, 3, np.int32)), n)
+        c.compact()
+        assert c.status()[:3] == (0, 0, 0)
+        assert np.array_equal(dev.get(at["table"], (n, 2), np.int32), np.stack([np.arange(n), np.full(n, -1)], 1))
+        assert (dev.get(at["lens"], n, np.int32) == 3).all() and (dev.get(at["refs"], n, np.int32) == 1).all()
