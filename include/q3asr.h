@@ -246,6 +246,7 @@ enum {
  * NULL) return the error that is kept, if any, and reset the status; after calls on another stream the host asks here: waits for the
  * stream, copies the status to out (host, 4 numbers) and, where clear is non-zero, sets it to zeros.  Not under graph capture. */
 int q3asr_pages_status(q3asr_model* m, const q3asr_kv_pages* c, int32_t* out, int clear, void* stream);
+/* Bytes of workspace that fork, free, reserve and compact need (-1: sizes that are not positive). */
 int64_t q3asr_pages_workspace(const q3asr_kv_pages* c);
 /* No sequences, all pages free, status zero.  The pages' contents stay as they are. */
 int q3asr_pages_reset(q3asr_model* m, const q3asr_kv_pages* c, void* stream);

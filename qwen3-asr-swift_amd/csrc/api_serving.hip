@@ -171,7 +171,7 @@ int q3asr_i8_linear(q3asr_model* m, const void* x, int x_dtype, int64_t ldx, con
 }
 
 int64_t q3asr_i8_workspace(q3asr_model* m, int M, int N, int K) {
-    if (!m || M <= 0 || N <= 0 || K <= 0 || K > I8_MAX_K) return -1;
+    if (!m || M <= 0 || N <= 0 || K <= 0 || K > I8_MAX_K || M > MAX_ROWS || N > MAX_ROWS) return -1;
     return quantized_bytes(M, K);
 }
 

@@ -71,7 +71,10 @@ class PagedKVCache:
 
     def workspace_bytes(self):
         """Bytes that fork, free, reserve and compact need."""
-        return int(self._lib.q3asr_pages_workspace(self._c))
+        n = int(self._lib.q3asr_pages_workspace(self._c))
+        if n < 0:
+            raise ValueError("PagedKVCache: sizes out of range")
+        return n
 
     def set_workspace(self, address, nbytes):
         self.c.workspace, self.c.workspace_bytes = address, nbytes
