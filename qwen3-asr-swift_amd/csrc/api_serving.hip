@@ -78,6 +78,7 @@ void check_batch(const q3asr_kv_pages* c, const q3asr_attn_batch* b) {
     Q3_REQUIRE(b && b->n >= 0 && b->rows >= 0, "pages: bad batch");
     if (b->n == 0 || b->rows == 0) return;
     Q3_REQUIRE(b->seqs && b->cu_rows, "pages: null argument in the batch");
+    Q3_REQUIRE(aligned(b->seqs, 4) && aligned(b->cu_rows, 4) && aligned(b->cu_groups, 4) && aligned(b->shared, 4), "pages: misaligned list in the batch");
     Q3_REQUIRE(b->n <= c->max_seqs, "pages: more entries than sequences");
     Q3_REQUIRE(b->rows <= MAX_ROWS, "pages: 2^24 rows or more");
 }
@@ -112,6 +113,7 @@ int q3asr_i8_quantize(q3asr_model* m, const void* x, int dtype, int64_t ldx, int
     Q3_REQUIRE(rows > 0 && cols > 0, "i8_quantize: empty problem");
     Q3_REQUIRE(rows <= MAX_ROWS && cols <= MAX_LD_I8, "i8_quantize: 2^24 rows or more, or more than 4194304 columns");
     check_rows("i8_quantize: x", x, dtype, ldx, cols);
+    Q3_REQUIRE(aligned(scales, 4), "i8_quantize: misaligned scales");
     Q3_REQUIRE(aligned(q, 16) && ldq % 16 == 0 && ldq >= (((int64_t)cols + 15) & ~15ll) && ldq < MAX_LD,
                "i8_quantize: rows of q must be aligned to 16 bytes and hold cols rounded up to 16");
     Call call(m, stream);
@@ -120,7 +122,7 @@ int q3asr_i8_quantize(q3asr_model* m, const void* x, int dtype, int64_t ldx, int
     Q3_API_END
 }
 
-static void check_product(const int8_t* w, int64_t ldw, const float* w_scales, int M, int N, int K, const void* out, int out_dtype, int64_t ldo) {
+static void check_product(const int8_t* w, int64_t ldw, const float* w_scales, const float* bias, int M, int N, int K, const void* out, int out_dtype, int64_t ldo) {
     Q3_REQUIRE(w && w_scales && out, "i8: null argument");
     Q3_REQUIRE(M > 0 && N > 0 && K > 0, "i8: empty problem");
     Q3_REQUIRE(K <= I8_MAX_K, "i8: K above 131056 could overflow the 32-bit sums");
@@ -128,15 +130,17 @@ static void check_product(const int8_t* w, int64_t ldw, const float* w_scales, i
     Q3_REQUIRE(M <= MAX_ROWS && N <= MAX_ROWS, "i8: 2^24 rows or output channels, or more");
     check_i8("i8: w", w, ldw, K);
     check_rows("i8: out", out, out_dtype, ldo, N);
+    Q3_REQUIRE(aligned(w_scales, 4) && aligned(bias, 4), "i8: misaligned scales or bias");
 }
 
 int q3asr_i8_matmul(q3asr_model* m, const int8_t* a, int64_t lda, const float* a_scales, const int8_t* w, int64_t ldw,
                     const float* w_scales, const float* bias, int M, int N, int K, void* out, int out_dtype, int64_t ldo, void* stream) {
     Q3_API_BEGIN
     Q3_REQUIRE(m && a && a_scales, "i8_matmul: null argument");
-    check_product(w, ldw, w_scales, M, N, K, out, out_dtype, ldo);
+    check_product(w, ldw, w_scales, bias, M, N, K, out, out_dtype, ldo);
     Q3_REQUIRE(K % 16 == 0, "i8_matmul: K must be a multiple of 16");
     check_i8("i8: a", a, lda, K);
+    Q3_REQUIRE(aligned(a_scales, 4), "i8_matmul: misaligned scales");
     Call call(m, stream);
     I8Params p;
     p.A = a; p.lda = lda; p.sa = a_scales; p.W = w; p.ldw = ldw; p.sw = w_scales; p.bias = bias;
@@ -151,7 +155,7 @@ int q3asr_i8_linear(q3asr_model* m, const void* x, int x_dtype, int64_t ldx, con
                     int64_t workspace_bytes, void* stream) {
     Q3_API_BEGIN
     Q3_REQUIRE(m && x && workspace, "i8_linear: null argument");
-    check_product(w, ldw, w_scales, M, N, K, out, out_dtype, ldo);
+    check_product(w, ldw, w_scales, bias, M, N, K, out, out_dtype, ldo);
     check_rows("i8_linear: x", x, x_dtype, ldx, K);
     Q3_REQUIRE(aligned(workspace, 16), "i8_linear: misaligned workspace");
     Q3_REQUIRE(workspace_bytes >= quantized_bytes(M, K), "i8_linear: workspace too small");
@@ -212,6 +216,7 @@ int q3asr_pages_fork(q3asr_model* m, const q3asr_kv_pages* c, const int32_t* dst
     check_cache(c, true);
     check_list(c, n);
     Q3_REQUIRE(n == 0 || (dst && src), "pages_fork: null argument");
+    Q3_REQUIRE(aligned(dst, 4) && aligned(src, 4), "pages_fork: misaligned list");
     Call call(m, stream);
     if (n > 0) launch_pages_fork(*c, dst, src, n, call.s);
     finish(call, *c);
@@ -224,6 +229,7 @@ int q3asr_pages_free(q3asr_model* m, const q3asr_kv_pages* c, const int32_t* seq
     check_cache(c, true);
     check_list(c, n);
     Q3_REQUIRE(n == 0 || seqs, "pages_free: null argument");
+    Q3_REQUIRE(aligned(seqs, 4), "pages_free: misaligned list");
     Call call(m, stream);
     if (n > 0) launch_pages_fork(*c, seqs, nullptr, n, call.s);
     finish(call, *c);
@@ -236,6 +242,7 @@ int q3asr_pages_reserve(q3asr_model* m, const q3asr_kv_pages* c, const int32_t* 
     check_cache(c, true);
     check_list(c, n);
     Q3_REQUIRE(n == 0 || (seqs && tokens), "pages_reserve: null argument");
+    Q3_REQUIRE(aligned(seqs, 4) && aligned(tokens, 4), "pages_reserve: misaligned list");
     Call call(m, stream);
     if (n > 0) launch_pages_reserve(*c, seqs, tokens, n, call.s);
     finish(call, *c);
