@@ -707,20 +707,18 @@ void launch_gemm256(const I8Params& p, hipStream_t s) {
 // wave's share of up to NS steps is requested at once.  The activation rows are rounded to 8 bits by every workgroup for itself,
 // underneath those loads: they are a few KB from the L2, and a second kernel in front would cost more than the whole product.
 // Weight rows are the MFMA "A" operand (lane: row li, bytes 16 lg ..), the activation rows in LDS the "B".
-// 1 x 2048 -> 4096: 4.5 us, of which a launch alone takes 2; 5 x 6144 -> 2048: 9.8, of which 2.6 are the rounding of 5 rows.
-// FROM: 0 bf16 rows, 1 fp32 rows, 2 rows that are rounded already.  HELD > 0: K is at least 8 and a thread's share of the rows, at
-// most HELD pieces of 8 values, is requested before the weights and held in registers, so that nothing waits behind the weights; 0:
-// any K, read twice.
-constexpr int FEW_THREADS = 512, FEW_WAVES = 8, FEW_ROWS = 16, FEW_PLAIN = 6, FEW_LDS = 100 * 1024;
+// 1 x 2048 -> 4096: 4.7 us behind others of its kind; 5 x 6144 -> 2048: 10.1, of which 2.5 are the rounding of 5 rows.
+// F32: fp32 rows, else bf16.  HELD > 0: K is at least 8 and a thread's share of the rows, at most HELD pieces of 8 values, is
+// requested before the weights and held in registers, so that nothing waits behind the weights; 0: any K, read twice.
+constexpr int FEW_THREADS = 512, FEW_WAVES = 8, FEW_ROWS = 16, FEW_LDS = 100 * 1024;
 constexpr int FEW_RED = FEW_WAVES * 256 * 4;
 __host__ __device__ inline int few_stride(int K) { return ((K + 63) & ~63) + 16; }   // rows 16 bytes apart modulo the banks
 
-template <int FROM, int NS, int HELD>
+template <bool F32, int NS, int HELD>
 __global__ __launch_bounds__(FEW_THREADS, 2) void i8_few_rows_kernel(I8Params p, I8Source src) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     __shared__ uint32_t amax[FEW_ROWS];
     __shared__ RowScale scales[FEW_ROWS];
-    constexpr bool F32 = FROM == 1;
     const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int k16 = (p.K + 15) & ~15, steps = (p.K + 63) >> 6, stride = few_stride(p.K);
@@ -777,13 +775,6 @@ __global__ __launch_bounds__(FEW_THREADS, 2) void i8_few_rows_kernel(I8Params p,
             held[i].values(v);
             if (tid + FEW_THREADS * i < pieces) *(uint2*)(xq + row_of[i] * stride + k_of[i]) = rs.template pack8<F32>(v);
         }
-    } else if constexpr (FROM == 2) {
-        request(n0, 0);
-        for (int c = tid; c < pieces; c += FEW_THREADS) {
-            const int m = c / per_row, k = (c - m * per_row) * 8;
-            *(uint2*)(xq + m * stride + k) = k < k16 ? *(const uint2*)(p.A + (int64_t)m * p.lda + k) : make_uint2(0, 0);
-        }
-        if (tid < p.M) scales[tid].scale = p.sa[tid];
     } else {
         __syncthreads();
         for (int c0 = 0; c0 < pieces; c0 += FEW_THREADS) {
@@ -848,34 +839,35 @@ __global__ __launch_bounds__(FEW_THREADS, 2) void i8_few_rows_kernel(I8Params p,
     }
 }
 
-template <int FROM, int NS, int HELD>
+template <bool F32, int NS, int HELD>
 void launch_few(const I8Params& p, const I8Source& src, hipStream_t s) {
     const int lds = FEW_RED + p.M * few_stride(p.K);
     static PerDeviceOnce once;
     once.run([&] {
-        HIP_CHECK(hipFuncSetAttribute((const void*)i8_few_rows_kernel<FROM, NS, HELD>, hipFuncAttributeMaxDynamicSharedMemorySize, FEW_RED + FEW_LDS));
+        HIP_CHECK(hipFuncSetAttribute((const void*)i8_few_rows_kernel<F32, NS, HELD>, hipFuncAttributeMaxDynamicSharedMemorySize, FEW_RED + FEW_LDS));
     });
     ProfScope ps("i8_few_rows_kernel", (double)p.N * p.K, s);
-    hipLaunchKernelGGL((i8_few_rows_kernel<FROM, NS, HELD>), dim3(std::min(cdiv(p.N, 16), 512)), dim3(FEW_THREADS), lds, s, p, src);
+    hipLaunchKernelGGL((i8_few_rows_kernel<F32, NS, HELD>), dim3(std::min(cdiv(p.N, 16), 512)), dim3(FEW_THREADS), lds, s, p, src);
     HIP_CHECK(hipGetLastError());
 }
-template <int FROM, int HELD>
+template <bool F32, int HELD>
 void launch_few_steps(const I8Params& p, const I8Source& src, hipStream_t s) {
     const int per_wave = cdiv(cdiv(p.K, 64), FEW_WAVES);
-    if (per_wave <= 4) launch_few<FROM, 4, HELD>(p, src, s);
-    else launch_few<FROM, 12, HELD>(p, src, s);
+    if (per_wave <= 4) launch_few<F32, 4, HELD>(p, src, s);
+    else launch_few<F32, 12, HELD>(p, src, s);
 }
-// Whether rounding the rows in every workgroup is cheaper than a launch of its own (us, one kernel against two): 1 x 2048 -> 4096:
-// 4.9, 7.4; 5 x 2048 -> 4096: 5.4, 7.8; 8: 6.4, 7.9; 10 (more than 4 pieces per thread): 8.1, 7.7; 16 x 1024 -> 4096: 6.4, 7.8;
-// 5 x 6144 -> 2048: 9.9, 13.2; 6: 12.3, 14.4; 5 x 2047 -> 2048: 5.8, 7.9; 8 x 1003 -> 12288: 7.6, 8.0; 10: 8.6, 7.8.
-template <int FROM>
+// Whether rounding the rows in every workgroup is cheaper than a launch of its own (us, calls of one graph, one kernel against two):
+// 1 x 2048 -> 4096: 4.7, 7.1; 5: 5.5, 7.2; 8 (4 pieces per thread): 5.7, 7.3; 12 (6): 8.2, 7.5; 1 x 6144 -> 2048: 7.2, 10.9; 5 (8 pieces):
+// 10.1, 11.2; 6 (9, in a form that holds 12): 11.5, 11.2; 8: 12.0, 11.2; 16 x 1024 -> 4096: 5.6, 5.7; 8 x 2048 -> 12288: 7.9, 9.8;
+// 12: 11.2, 9.8.  A K that leaves many of a wave's steps empty is the exception: 6 x 2816 -> 1024 (5 pieces) 9.0, 7.5.
+template <bool F32>
 bool launch_few_rows(const I8Params& p, const I8Source& src, hipStream_t s) {
     const int64_t held = cdiv((int64_t)p.M * cdiv(p.K, 64) * 8, FEW_THREADS);
     if (p.M > FEW_ROWS || held > (p.M <= 6 ? 8 : 4) || (p.M > 8 && p.N > 8192)) return false;
-    if (p.K < 8) launch_few_steps<FROM, 0>(p, src, s);
-    else if (held <= 2) launch_few_steps<FROM, 2>(p, src, s);
-    else if (held <= 4) launch_few_steps<FROM, 4>(p, src, s);
-    else launch_few_steps<FROM, 8>(p, src, s);
+    if (p.K < 8) launch_few_steps<F32, 0>(p, src, s);
+    else if (held <= 2) launch_few_steps<F32, 2>(p, src, s);
+    else if (held <= 4) launch_few_steps<F32, 4>(p, src, s);
+    else launch_few_steps<F32, 8>(p, src, s);
     return true;
 }
 
@@ -917,14 +909,13 @@ void launch_i8_quantize(const I8Source& src, int rows, int cols, int8_t* q, int6
 }
 
 bool launch_i8_linear_few_rows(const I8Params& p, const I8Source& src, hipStream_t s) {
-    return src.f32 ? launch_few_rows<1>(p, src, s) : launch_few_rows<0>(p, src, s);
+    return src.f32 ? launch_few_rows<true>(p, src, s) : launch_few_rows<false>(p, src, s);
 }
 
 void launch_i8_matmul(const I8Params& p, hipStream_t s) {
-    if (p.M <= FEW_PLAIN && p.M * (int64_t)few_stride(p.K) <= FEW_LDS) {
-        launch_few_steps<2, 0>(p, {}, s);
-        return;
-    }
+    // Few rows that are rounded already go through the smallest tiles too.  The kernel above, fed with them, took (us, calls of one graph,
+    // against the tiles) 1 x 2048 -> 4096: 4.3, 4.7; 4: 4.5, 4.7; 8: 5.0, 4.7; 1 x 6144 -> 2048: 7.2, 8.1; 6: 9.0, 8.3; 8: 9.7, 8.4; but
+    // 1 x 2816 -> 1024: 6.8, 4.9; 1 x 1024 -> 4096: 4.0, 3.3; 1 x 896 -> 4864: 5.3, 3.4; 1 x 2048 -> 12288: 7.4, 6.9; 6: 8.0, 7.1.
     // The smallest tiles that still fit the device at once win while the sums are short of workgroups, because the walk along K
     // is then all latency (us at K = 2048, and 6144 with *; 32 x 32 by 512 bytes of K, 32 x 64 by 512, by 256, 64 x 64, 128 x 128,
     // 256 x 256):  64 x 4096: 5.0, 5.7, 5.9, 8.2, 13.8, 24;  128 x 2048*: 8.7, 11.1, 12.6, 18, 37, 58;  256 x 4096: 14, 9.8, 7.7, 8.3,
