@@ -274,7 +274,7 @@ int q3asr_pages_compact(q3asr_model* m, const q3asr_kv_pages* c, void* stream);
 typedef struct q3asr_attn_batch {
     const int32_t* seqs;       /* [n] */
     const int32_t* cu_rows;    /* [n + 1], from 0 to at most rows */
-    const int32_t* cu_groups;  /* [n_groups + 1], from 0 to n, or NULL */
+    const int32_t* cu_groups;  /* [n_groups + 1], from 0 to n, or NULL; n_groups is at most n, and a group may be empty */
     const int32_t* shared;     /* [n_groups] or NULL */
     int n, rows, n_groups;
     int max_rows;              /* rows of one sequence */

@@ -199,7 +199,8 @@ __device__ __forceinline__ uint32_t wave_max_bits(uint32_t v) {
 
 // A workgroup's four waves per row (WHOLE), or one wave where rows are many and short; 8 values per lane and step.  Rows of up to
 // 2048 * HELD values (512 * HELD) stay in registers between the maximum and the rounding, longer ones (HELD 0) are read twice.
-// HBM-bound: 8100 x 2048 bf16 13.2 us (3.8 TB/s read and written, a launch's 4 included), 8100 x 6144 28 (5.3), 387 x 1003 fp32 4.6.
+// HBM-bound: 8100 x 2048 bf16 13.3 us behind others of its kind (3.7 TB/s read and written; 15.9 alone), 8100 x 6144 28 (5.3),
+// 387 x 1003 fp32 2.8.
 // With a wave per row, before bf16 rows lost their remainders: 14.3 against 13.5, 36 against 29; 8100 x 1003: 9.4 against 10.7.
 template <bool F32, int HELD, bool WHOLE>
 __global__ __launch_bounds__(256) void i8_quantize_kernel(const void* x, int64_t ldx, int rows, int cols, int8_t* q, int64_t ldq, float* scales) {

@@ -17,8 +17,8 @@
 //   stream  the tiles of all sequences and groups in one row, cut into equal parts, one per wave of a full device: no wave waits for
 //           another, and each has a tile in flight all the time.  Where a wave goes over to other rows counts like a tile.  Two
 //           launches: the waves, which find out first where every sequence's tiles begin, and the join of what was cut.
-// The stream takes 112 us for 96 groups of 5 after 405 tokens (8 KV heads of 128, 5.2 TB/s), 141 for 16 groups of 8 after 16 000 (5.9), 27
-// for 12 groups of 7 x 24 rows after 1111 (14 heads of 64, compute and parts); the join 5-8; plain 7.4 for 4 sequences of 406 keys.
+// The stream takes 111 us for 96 groups of 5 after 405 tokens (8 KV heads of 128, 5.2 TB/s), 139 for 16 groups of 8 after 16 000 (5.9), 31
+// for 12 groups of 7 x up to 24 rows after 1111 (14 heads of 64, compute and parts); the join 5-8; plain 7.7 for 4 sequences of 406 keys.
 // Measured against 4-wave work items of up to 1024 keys, sorted by size: rounding to four tiles and joining cost 1.2 to 1.4 times
 // the mean load there.
 #include "paged.h"
@@ -157,7 +157,7 @@ __device__ __forceinline__ bool read_batch(const AttnParams& p, const PlanMemory
     int *const from = mem.from, *const cu = mem.cu, *const cu_rows = mem.rows;
     const int last_g = p.n_groups - 1, last = p.n - 1;
     bool down = false;
-    for (int i = tid; i <= p.n || i <= p.n_groups; i += THREADS) {
+    for (int i = tid; i <= p.n; i += THREADS) {   // there are no more groups than entries
         // all that does not depend on another load at once
         const int seq = p.seqs[min(i, last)], a = p.cu_rows[min(i, last)], b = p.cu_rows[min(i, last) + 1];
         const int group = last_g < 0 ? 0 : p.cu_groups[min(i, last_g + 1)], shared = last_g < 0 ? 0 : p.shared[min(i, last_g)];
@@ -317,9 +317,9 @@ struct Rows {
     static constexpr int TILE = 32 * VROW;
 };
 
-// ONCE: no key is read by several waves, so its rows need not stay in a cache.  Loads that say so take 144 us where others take 161
-// (256 sequences after 900 tokens, 8 KV heads of 128); where three query tiles read each key they take 34 against 27 (7 x 24 rows
-// after 1111 tokens, 12 groups, 14 heads of 64).
+// ONCE: no key is read by several waves, so its rows need not stay in a cache.  A step whose loads say so takes 152 us where others take 171
+// (256 sequences of 900 tokens, 8 KV heads of 128); where query tiles read the same keys it takes 66 against 60 (three of them: 12 x 7 x 24
+// rows after 1111 tokens, 14 heads of 64) and 93 against 61 (17: 2 x 14 x 19 rows after 3584, 16 / 8 heads of 128).
 template <int D, int QT, bool ONCE>
 struct Wave {
     static constexpr int NKS = D / 32, NDT = D / 16, LPR = D / 8, RPI = 64 / LPR, IV = 16 / RPI, PAIR = QT < 2 ? 1 : 2;
@@ -855,21 +855,22 @@ Plan plan_for(const q3asr_kv_pages& c, const q3asr_attn_batch& b, int heads) {
     Plan r{};
     const int group = heads / c.kv_heads;
     // A small step is all latency: whole sequences that fit the device at once, shared or not, in one launch (head_dim 128: two
-    // workgroups per CU, 64: three, or four that follow soon).  us against the stream, the write of the step included: 128 sequences
-    // of 20 and of 900 tokens, 4 KV heads of 128: 11, 26 (there PLAIN_ITEMS is reached); 8 KV heads: 17, 40 against 13, 29; 256 of 20,
-    // 210, 450 and 900 tokens, 4 KV heads of 64: 11, 15, 18, 25 against 12, 19, 22, 24.
+    // workgroups per CU, 64: three, or four that follow soon).  us against the stream, the write of the step included, no keys in the
+    // caches: 128 sequences of 20 and of 900 tokens, 4 KV heads of 128: 11.6, 44 against 12.0, 48 (there PLAIN_ITEMS is reached); 8 KV heads:
+    // 18.1, 85 against 13.0, 83; 256 of 20, 210, 450 and 900 tokens, 4 KV heads of 64: 11.5, 17.4, 24, 42 against 11.6, 20.5, 30, 48.
     r.qt = (int64_t)b.max_rows * group <= 16 ? 1 : 2;
     r.tiles_q = cdiv((int64_t)b.max_rows * group, 16 * r.qt);
     r.plain = b.max_len <= PLAIN_KEYS && (int64_t)b.n * r.tiles_q * c.kv_heads <= (c.head_dim == 128 ? PLAIN_ITEMS : 2 * PLAIN_ITEMS);
     if (r.plain) return r;
     const bool shares = groups_count(c, b);
     const int64_t rows = (int64_t)(shares ? b.max_group_rows : b.max_rows) * group;
-    // as many rows at once as the registers of two waves per SIMD hold (64 x 128 sums do not fit; 64 x 64 against 32 x 64 at three
-    // waves: 34 against 39 us for 7 x 24 rows after 1111 tokens, 12 groups, 14 heads)
+    // as many rows at once as the registers of two waves per SIMD hold (64 x 128 sums do not fit).  64 x 64 sums against 32 x 64, us of a
+    // step after 1111 tokens, 12 groups, 14 heads: 7 x 24 rows 61, 63; 7 x 48: 96, 97; 7 x up to 24, which fill 87 of 128 rows: 46, 45;
+    // after 3584, 2 groups, 16 / 8 heads: 14 x 19 rows 45, 41.
     r.qt = rows <= 16 ? 1 : rows <= 32 || c.head_dim == 128 ? 2 : 4;
     r.once = rows <= 16 * r.qt;
     // Parts of a row: tiles of its longest segment by the least tiles of a wave, and one for where it begins.  More parts spread a few
-    // long sequences over the device; their memory is kept to 64 MB (but 16 parts).
+    // long sequences over the device; the shared and the own segments' are kept to 64 MB each, or 16 where that is more, and one.
     const int64_t part = (int64_t)b.rows * heads * (c.head_dim * 4 + 8);
     const int most = (int)std::max<int64_t>(16, std::min<int64_t>(1024, (64ll << 20) / part));
     const int own = shares ? b.max_own : b.max_len, longest = std::max({own, shares ? b.max_shared : 0, 1});
